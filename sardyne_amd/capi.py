@@ -120,6 +120,46 @@ class SdyMvArgs(ctypes.Structure):
                 ("epilogue", _int), ("nw", _vp), ("eps", ctypes.c_float), ("ws_ready", ctypes.c_int)]
 
 
+_long, _float = ctypes.c_long, ctypes.c_float
+
+
+class SdyRopeScaling(ctypes.Structure):
+    """sdy_rope_scaling (sardyne_amd/csrc/sdy_ops.h)."""
+    _fields_ = [("kind", _int), ("factor", _float), ("orig_ctx", _int), ("beta_fast", _float), ("beta_slow", _float),
+                ("attn_factor", _float), ("low_freq", _float), ("high_freq", _float)]
+
+
+class SdyRopeAtArgs(ctypes.Structure):
+    """sdy_rope_at_args (sardyne_amd/csrc/sdy_ops.h)."""
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("q_stride", _long), ("k_stride", _long), ("v_stride", _long),
+                ("q_out", _vp), ("q_out_stride", _long), ("k_rows", _vp), ("v_rows", _vp), ("head_stride", _long),
+                ("kv_type", _int), ("n_slot", _int), ("pos", _vp), ("slot", _vp), ("freq", _vp), ("mscale", _float),
+                ("n_rot", _int), ("interleaved", _int), ("q_norm", _vp), ("k_norm", _vp), ("eps", _float),
+                ("n_tok", _int), ("n_head", _int), ("n_kv_head", _int), ("hd", _int)]
+
+
+class SdyAttnTreeArgs(ctypes.Structure):
+    """sdy_attn_tree_args (sardyne_amd/csrc/sdy_ops.h)."""
+    _fields_ = [("q", _vp), ("q_stride", _long), ("k_cache", _vp), ("v_cache", _vp), ("head_stride", _long),
+                ("k_draft", _vp), ("v_draft", _vp), ("draft_stride", _long), ("kv_type", _int), ("parent", _vp),
+                ("n_past", _vp), ("max_past", _int), ("n_tok", _int), ("n_head", _int), ("n_kv_head", _int),
+                ("hd", _int), ("out", _vp), ("out_stride", _long), ("part", _vp)]
+
+
+class SdySampleArgs(ctypes.Structure):
+    """sdy_sample_args (sardyne_amd/csrc/sdy_ops.h)."""
+    _fields_ = [("logits", _vp), ("stride", _long), ("n_rows", _int), ("n_vocab", _int), ("temp", _vp),
+                ("top_k", _vp), ("top_p", _vp), ("min_p", _vp), ("u", _vp), ("token", _vp), ("prob", _vp), ("ws", _vp)]
+
+
+class SdyTreeCommitArgs(ctypes.Structure):
+    """sdy_tree_commit_args (sardyne_amd/csrc/sdy_ops.h)."""
+    _fields_ = [("token", _vp), ("parent", _vp), ("sampled", _vp), ("n_tok", _int), ("n_past", _vp), ("k_draft", _vp),
+                ("v_draft", _vp), ("draft_stride", _long), ("draft_layer_stride", _long), ("k_cache", _vp),
+                ("v_cache", _vp), ("head_stride", _long), ("layer_stride", _long), ("kv_type", _int), ("max_seq", _int),
+                ("n_layer", _int), ("n_kv_head", _int), ("hd", _int), ("path", _vp), ("n_acc", _vp), ("step", _vp)]
+
+
 _DEVICE_SIGNATURES = {
     "sdy_last_error": (ctypes.c_char_p, []),
     "op_last_error": (ctypes.c_char_p, []),
@@ -229,10 +269,19 @@ _DEVICE_SIGNATURES = {
                                 ctypes.POINTER(SdyMvArgs), _vp, _vp]),
     "sdy_moe_sort": (_int, [_vp, _int, _int, _int, _int, _vp, _vp, _vp, _vp, _vp]),
     "sdy_gather_rows": (_int, [_vp, _vp, _int, _int, _vp, _vp]),
+    "sdy_rope_freqs": (_int, [_vp, ctypes.POINTER(_float), _int, _float, ctypes.POINTER(SdyRopeScaling)]),
+    "sdy_qk_rope_at": (_int, [ctypes.POINTER(SdyRopeAtArgs), _vp]),
+    "sdy_attn_tree_ok": (_int, [_int, _int, _int, _int]),
+    "sdy_attn_tree_floats": (_sz, [_int, _int, _int, _int, _int]),
+    "sdy_attn_tree": (_int, [ctypes.POINTER(SdyAttnTreeArgs), _vp]),
+    "sdy_sample_ws_bytes": (_sz, [_int, _int]),
+    "sdy_sample": (_int, [ctypes.POINTER(SdySampleArgs), _vp]),
+    "sdy_tree_commit": (_int, [ctypes.POINTER(SdyTreeCommitArgs), _vp]),
 }
 
 EPI_NONE, EPI_SWIGLU = 0, 1
 KV_F32, KV_F16 = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_YARN, ROPE_LLAMA3 = 0, 1, 2, 3
 
 
 def lib_path() -> pathlib.Path:

@@ -94,6 +94,107 @@ int sdy_attn_decode_split(const float *q, const float *k, const float *v, const 
                           float eps, const float *rope_cos, const float *rope_sin, const int32_t *step_dev, int n_head,
                           int n_kv_head, int hd, int interleaved, float *k_cache, float *v_cache, long head_stride,
                           int max_seq, float *part, unsigned *count, float *out, void *xq_q8k, sdy_stream s);
+/* ---- one step of speculative decoding: a drafted tree of tokens evaluated together. Node t of n_tok has the parent
+ * parent[t] (device int32), a lower index; one outside [0, t) makes t a root, and below -1 marks a place without a node (so
+ * that a recorded step of a fixed size replays for smaller trees). The calls are asynchronous on s, allocate nothing and
+ * keep nothing between calls; every array is device memory of the calling thread's current device. */
+
+/* Scaling of rotary positions for contexts beyond the original one */
+enum { SDY_ROPE_PLAIN = 0, SDY_ROPE_LINEAR = 1, SDY_ROPE_YARN = 2, SDY_ROPE_LLAMA3 = 3 };
+typedef struct {
+    int kind;                    /* SDY_ROPE_* */
+    float factor;                /* the context's growth (not PLAIN) */
+    int orig_ctx;                /* YARN, LLAMA3: the context of training */
+    float beta_fast, beta_slow;  /* YARN: turns over orig_ctx that keep, or take the whole of, the scaling (32, 1) */
+    float attn_factor;           /* YARN: the factor on cos and sin; 0: 0.1 ln(factor) + 1 */
+    float low_freq, high_freq;   /* LLAMA3: turns over orig_ctx between which the scaling fades (1, 4) */
+} sdy_rope_scaling;
+/* Host only: freq[n_rot / 2] and *mscale of sdy_qk_rope_at for base theta; sc may be NULL (PLAIN). */
+int sdy_rope_freqs(double *freq, float *mscale, int n_rot, float theta, const sdy_rope_scaling *sc);
+
+/* Rotary positions of tokens with a position and a slot each (drafted trees, several conversations' tokens, prompts that
+ * go to scattered slots): the q heads' rotated rows to q_out, the rotated k and the v rows to slots of K/V memory. */
+typedef struct {
+    const float *q, *k, *v;      /* token rows t * q_stride ... floats apart; q or k (with v) may be NULL */
+    long q_stride, k_stride, v_stride;
+    float *q_out;                /* rows q_out_stride apart; may be q with the same stride, no other overlap */
+    long q_out_stride;
+    void *k_rows, *v_rows;       /* [n_kv_head][n_slot][hd] of kv_type, heads head_stride elements apart */
+    long head_stride;
+    int kv_type, n_slot;
+    const int32_t *pos, *slot;   /* [n_tok]; slot NULL: pos. A slot outside [0, n_slot): no row is written; of several
+                                    tokens with one slot the last one's row is. Any int32 position */
+    const double *freq;          /* [n_rot / 2] (sdy_rope_freqs): angle pos * freq[i] */
+    float mscale;                /* the factor on cos and sin */
+    int n_rot, interleaved;      /* dims of a head that turn, the first; pairs (2i, 2i+1) or (i, i + n_rot/2) */
+    const float *q_norm, *k_norm; /* [hd] RMSNorm weights of a head before it turns, or NULL */
+    float eps;
+    int n_tok, n_head, n_kv_head, hd; /* hd even, at most 512 */
+} sdy_rope_at_args;
+int sdy_qk_rope_at(const sdy_rope_at_args *a, sdy_stream s);
+
+/* Attention of the nodes: node t sees every cached position below *n_past, itself and the nodes above it. K/V rows of the
+ * nodes are in memory of their own (as sdy_qk_rope_at writes them with slot = node), so the cache holds accepted
+ * positions only. Within tolerance (f32 sums in the kernel's order), the same on every call. An unused place's output row,
+ * and with *n_past outside [0, max_past] every row, is left as it was. */
+typedef struct {
+    const float *q;              /* rotated queries, rows q_stride floats apart */
+    long q_stride;
+    const void *k_cache, *v_cache; /* [n_kv_head][..][hd] of kv_type, heads head_stride elements apart */
+    long head_stride;
+    const void *k_draft, *v_draft; /* node t's rows at t * hd of each kv head, heads draft_stride elements apart */
+    long draft_stride;
+    int kv_type;
+    const int32_t *parent;       /* [n_tok] */
+    const int32_t *n_past;       /* device int: the number of cached positions */
+    int max_past;                /* bound on *n_past (the scratch's size and the launch's) */
+    int n_tok, n_head, n_kv_head, hd; /* n_tok at most 256; hd 64, 128 or 256 */
+    float *out;                  /* rows out_stride floats apart */
+    long out_stride;
+    float *part;                 /* scratch of sdy_attn_tree_floats floats; not for two calls at once */
+} sdy_attn_tree_args;
+int sdy_attn_tree_ok(int n_tok, int n_head, int n_kv_head, int hd);
+size_t sdy_attn_tree_floats(int n_tok, int n_head, int n_kv_head, int hd, int max_past);
+int sdy_attn_tree(const sdy_attn_tree_args *a, sdy_stream s);
+
+/* A token per row of logits. In the order of a row's logits, the greatest first and of equal ones the lowest index: the
+ * first top_k tokens stay (<= 0: all); of these the shortest prefix whose probabilities (at temperature temp) reach top_p of
+ * their sum (>= 1: all, <= 0: the first); of these the ones with at least min_p times the first one's probability; the first
+ * always. The token is the first by index at which the running sum of the kept probabilities exceeds u of their whole
+ * (u in [0, 1), clamped). temp <= 0: the first token. -inf and NaN logits are never chosen; a row of nothing else gives
+ * token -1 and prob 0; beside +inf logits no others count. Probabilities below 2^(ceil log2 n_vocab - 62) of the greatest count as 0. */
+typedef struct {
+    const float *logits;         /* rows stride floats apart */
+    long stride;
+    int n_rows, n_vocab;         /* n_vocab at most 2^22 */
+    const float *temp;           /* [n_rows] each, or NULL: temperature 1, no top-k, no top-p, no min-p */
+    const int32_t *top_k;
+    const float *top_p, *min_p;
+    const float *u;              /* [n_rows] uniform numbers */
+    int32_t *token;              /* [n_rows] */
+    float *prob;                 /* [n_rows] the token's probability among the kept, or NULL */
+    void *ws;                    /* scratch of sdy_sample_ws_bytes bytes; not for two calls at once */
+} sdy_sample_args;
+size_t sdy_sample_ws_bytes(int n_rows, int n_vocab);
+int sdy_sample(const sdy_sample_args *a, sdy_stream s);
+
+/* The accepted path: node 0 (the step's own token), then from each node the lowest child whose token is the one sampled at
+ * its parent. Node path[i]'s K/V rows go to position *n_past + i of every layer's cache; nodes beyond max_seq are not
+ * accepted. With *n_past outside [0, max_seq) or no node 0, nothing is (n_acc 0, step and caches left as they were). */
+typedef struct {
+    const int32_t *token, *parent, *sampled; /* [n_tok] the drafted tokens, their parents, the token sampled at each node */
+    int n_tok;                   /* at most 256 */
+    const int32_t *n_past;       /* device int */
+    const void *k_draft, *v_draft; /* [n_layer][n_kv_head][..][hd] of kv_type, strides in elements */
+    long draft_stride, draft_layer_stride;
+    void *k_cache, *v_cache;     /* [n_layer][n_kv_head][max_seq][hd] */
+    long head_stride, layer_stride;
+    int kv_type, max_seq, n_layer, n_kv_head, hd;
+    int32_t *path;               /* [n_tok] the accepted nodes in order, then -1 */
+    int32_t *n_acc;              /* [1] */
+    int32_t *step;               /* [2] the next token and its position, as the one-token steps read them; not n_past's memory */
+} sdy_tree_commit_args;
+int sdy_tree_commit(const sdy_tree_commit_args *a, sdy_stream s);
 #ifdef __cplusplus
 }
 #endif
