@@ -4,6 +4,19 @@
 // rows of t and the nodes above it (parent, its parent, ...), one softmax over them, and the weighted sum of the V rows.
 // A parent outside [0, t) makes t a root; below -1 it marks a place without a node: its output row stays as it was and no
 // node attends to it.
+//
+//   k_tree_part<HD, KT, RW, KW>  one workgroup per (span of positions, kv head, block of 32 RW rows); a row is a node and one
+//   of the query heads that share the kv head, so a K/V tile is read once for all of them. Span 0 is the drafted rows. RW
+//   waves share each tile of 32 positions, KW groups of them take tiles in turn. Per tile a wave computes
+//   S^T = K Q^T (a lane holds one row's 16 scores), the running maximum and sum, and O^T += V^T P.
+//   k_tree_merge<HD>  one workgroup per node and head: the spans' (m, l, O) in span order.
+//
+// Products on the f16 matrix cores at f32's precision: an f32 is the sum of two f16 (22 bits and a sign) once its row is
+// scaled by a power of two that brings the row's greatest value to 2^13 .. 2^14; the rest's least bit is then 2^-24, 2^-38 of
+// that value. q, P and an f32 cache's K and V are split so, an f16 cache's rows are taken as they are; of the split products
+// low x low, at most 2^-22 of the whole, is left out. Powers of two go back exactly (ldexp): K's and q's into the scores, V's
+// into P and, where a tile's greatest grows, into O. The running maximum is kept as a whole number (rounded up), so that its
+// rescales are exact too, and P is 2^14 times the weight: f16's least bit is 2^-39 of the greatest weight.
 #include <type_traits>
 
 #include "sdy_attn_dev.h"
@@ -13,83 +26,585 @@
 
 namespace {
 
-constexpr int MAX_NODES = 256, THREADS = 256;
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-SDY_DEV float block_reduce(float v, float *sh, bool max) {
-    for (int off = 32; off >= 1; off >>= 1) {
-        const float o = __shfl_xor(v, off);
-        v = max ? fmaxf(v, o) : v + o;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return max ? fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3])) : (sh[0] + sh[1]) + (sh[2] + sh[3]);
+constexpr int MAX_NODES = 256;
+constexpr int KB = 32;         // positions per tile
+constexpr int TOP = 13;        // a scaled row's greatest value is 2^TOP .. 2^(TOP + 1)
+constexpr float P_BITS = 14;   // P is 2^14 times the weight
+constexpr int MAX_PARTS = 513;
+constexpr int MAX_PAST = 1 << 28;  // 512 spans of at most 2^30 bytes hold them
+
+struct TreeArgs {
+    sdy_attn_tree_args a;
+    int rows;       // per kv head: n_tok * (n_head / n_kv_head)
+    int n_block;    // row blocks
+    int n_span;     // spans of cached positions (the grid's; those in use follow from n_past)
+    int granule;    // positions of one round of a workgroup: 32 KW
+    float log_scale;  // log2(e) / sqrt(head_dim)
+    float *part;    // [1 + n_span][n_kv_head * rows][HD], then the (m, l) [1 + n_span][n_kv_head * rows][2]
+};
+
+// The rounds (granules) per span and the spans in use for so many positions.
+SDY_DEV int span_rounds(const TreeArgs &A, int past) {
+    const int n = (past + A.granule - 1) / A.granule;
+    return (n + A.n_span - 1) / A.n_span;
+}
+SDY_DEV int spans_used(const TreeArgs &A, int past) {
+    const int per = span_rounds(A, past), n = (past + A.granule - 1) / A.granule;
+    return per ? (n + per - 1) / per : 0;
 }
 
-// One workgroup per node and head: 256 keys at a time, a key per thread, then a dim per thread.
-template <class KT>
-__global__ __launch_bounds__(THREADS) void k_attn_tree(sdy_attn_tree_args a, float scale) {
-    __shared__ float q[256], p[THREADS], sh[4];
-    __shared__ int key[THREADS], n_anc;
-    const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-    const int past = *a.n_past;
-    if (past < 0 || past > a.max_past || a.parent[t] < -1) return;
-    const int g = h / (a.n_head / a.n_kv_head);
-    if (tid < a.hd) q[tid] = a.q[(size_t)t * a.q_stride + (size_t)h * a.hd + tid];
-    if (tid == 0) {
-        int n = 0;
-        for (int u = t;;) {
-            key[n++] = u;
-            const int up = a.parent[u];
-            if (up < 0 || up >= u || a.parent[up] < -1) break;
-            u = up;
+template <int HD, class KT, int RW, int KW>
+struct Lds {
+    static constexpr bool F32 = std::is_same<KT, float>::value;
+    static constexpr int NP = F32 ? 2 : 1;    // f16 parts of a K or V value
+    static constexpr int RS = HD + 8;         // f16 of a row: consecutive rows start 4 banks apart
+    static constexpr int PLANE = 32 * RS;
+    static constexpr size_t tile = (size_t)2 * NP * PLANE * 2;   // bytes, K parts then V parts
+    static constexpr size_t tiles = KW * tile;
+    static constexpr size_t scales = KW * 32 * 3 * 4;            // ek, ev, bad
+    static constexpr size_t masks = MAX_NODES * (MAX_NODES / 32) * 4 + MAX_NODES * 2;
+    static constexpr int OS = HD + 4;
+    static constexpr size_t merge = KW > 1 ? (size_t)KW * 32 * RW * (OS + 2) * 4 : 0;
+    static constexpr size_t body = tiles > merge ? (tiles > masks ? tiles : masks) : (merge > masks ? merge : masks);
+    static constexpr size_t bytes = body + scales;
+};
+
+// Two f32 as two f16 pairs, hi + lo = x up to 2^-23 of x (while lo is at least f16's least normal)
+SDY_DEV void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
+    const f16x2 h = __builtin_convertvector(f32x2{a, b}, f16x2);
+    const f16x2 l = __builtin_convertvector(f32x2{a - (float)h[0], b - (float)h[1]}, f16x2);
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, l);
+}
+
+// The exponent of a row's greatest |value|, from 2^-100 on (smaller rows count as that), and the power of two that brings the
+// row to 2^TOP. An infinity or a NaN stays one.
+SDY_DEV int row_exp(float most) {
+    const int e = (int)(__float_as_uint(most) >> 23) - 127;
+    return e > -100 ? e : -100;
+}
+SDY_DEV float exp_scale(int e) { return __uint_as_float((uint32_t)(127 + TOP - e) << 23); }
+
+// Rows of K and V on their way to LDS: thread tg of a group of 64 RW holds chunks of CE consecutive elements of one row.
+template <int HD, class KT, int RW>
+struct Stage {
+    static constexpr bool F32 = std::is_same<KT, float>::value;
+    static constexpr int LPR = 2 * RW;                              // lanes of a row
+    static constexpr int CE = F32 ? 4 : (HD / 8 >= LPR ? 8 : 4);    // elements of a chunk
+    static constexpr int NC = HD / CE / LPR;                        // chunks of a lane
+    static constexpr int W = CE * (int)sizeof(KT) / 4;              // words of a chunk
+    static_assert(NC >= 1 && HD == NC * CE * LPR, "a row's chunks divide over its lanes");
+    uint32_t r[NC][W];
+    SDY_DEV void load(__amdgpu_buffer_rsrc_t rs, uint32_t key, int tg) {
+        const uint32_t o = (key + (uint32_t)(tg / LPR)) * (uint32_t)(HD * sizeof(KT)) + (uint32_t)(tg % LPR) * (CE * sizeof(KT));
+#pragma unroll
+        for (int i = 0; i < NC; i++) {
+            const uint32_t at = o + (uint32_t)(i * LPR * CE * sizeof(KT));
+            if constexpr (W == 4) {
+                const auto u = __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0);
+                for (int w = 0; w < 4; w++) r[i][w] = u[w];
+            } else {
+                const auto u = __builtin_amdgcn_raw_buffer_load_b64(rs, at, 0, 0);
+                for (int w = 0; w < 2; w++) r[i][w] = u[w];
+            }
         }
-        n_anc = n;
+    }
+    // Whether this thread's row has an infinity or a NaN
+    SDY_DEV bool unfit() const {
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < NC; i++)
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                if constexpr (F32) any |= (r[i][w] & 0x7F800000u) == 0x7F800000u;
+                else any |= (r[i][w] & 0x7C00u) == 0x7C00u || (r[i][w] & 0x7C000000u) == 0x7C000000u;
+            }
+#pragma unroll
+        for (int off = 1; off < LPR; off *= 2) any |= (uint32_t)__shfl_xor((int)any, off);
+        return any != 0;
+    }
+    SDY_DEV void clear() {
+#pragma unroll
+        for (int i = 0; i < NC; i++)
+#pragma unroll
+            for (int w = 0; w < W; w++) r[i][w] = 0;
+    }
+    // The row's parts to the planes at dst (row tg / LPR), its exponent to *exps
+    SDY_DEV void store(uint16_t *dst, int *exps, int tg) const {
+        constexpr int RS = HD + 8;
+        const int row = tg / LPR, c0 = tg % LPR;
+        uint16_t *d = dst + row * RS + c0 * CE;
+        if constexpr (F32) {
+            float most = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NC; i++)
+#pragma unroll
+                for (int w = 0; w < 4; w += 2)
+                    most = fmaxf(most, fmaxf(fabsf(__uint_as_float(r[i][w])), fabsf(__uint_as_float(r[i][w + 1]))));
+#pragma unroll
+            for (int off = 1; off < LPR; off *= 2) most = fmaxf(most, __shfl_xor(most, off));
+            const int e = row_exp(most);
+            const float sc = exp_scale(e);
+            if (c0 == 0) exps[row] = e - TOP;
+#pragma unroll
+            for (int i = 0; i < NC; i++) {
+                u32x2 hi, lo;
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    uint32_t h, l;
+                    split2(__uint_as_float(r[i][2 * w]) * sc, __uint_as_float(r[i][2 * w + 1]) * sc, h, l);
+                    hi[w] = h;
+                    lo[w] = l;
+                }
+                *reinterpret_cast<u32x2 *>(d + i * LPR * CE) = hi;
+                *reinterpret_cast<u32x2 *>(d + 32 * RS + i * LPR * CE) = lo;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NC; i++) {
+                if constexpr (W == 4) *reinterpret_cast<u32x4 *>(d + i * LPR * CE) = u32x4{r[i][0], r[i][1], r[i][2], r[i][3]};
+                else *reinterpret_cast<u32x2 *>(d + i * LPR * CE) = u32x2{r[i][0], r[i][1]};
+            }
+        }
+    }
+};
+
+// Which nodes each node sees, as bits: mask[t] starts as t itself, then takes that of the farthest node known above it and
+// that one's farthest in turn, doubling the distance, so 8 rounds reach all of 256. In: parents. All threads of the block.
+SDY_DEV void ancestor_masks(const int32_t *parent, int n, uint32_t (*mask)[MAX_NODES / 32], int16_t *up) {
+    const int tid = threadIdx.x;
+    if (tid < MAX_NODES) {
+        int p = tid < n ? parent[tid] : -2;
+        for (int w = 0; w < MAX_NODES / 32; w++) mask[tid][w] = p >= -1 && w == tid / 32 ? 1u << (tid % 32) : 0u;
+        if (p < 0 || p >= tid || parent[p] < -1) p = -1;
+        up[tid] = (int16_t)p;
     }
     __syncthreads();
-    const KT *kc = (const KT *)a.k_cache + (size_t)g * a.head_stride, *vc = (const KT *)a.v_cache + (size_t)g * a.head_stride;
-    const KT *kd = (const KT *)a.k_draft + (size_t)g * a.draft_stride, *vd = (const KT *)a.v_draft + (size_t)g * a.draft_stride;
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    for (int j0 = 0; j0 < past + n_anc; j0 += THREADS) {
-        const int left = past + n_anc - j0, j = j0 + tid;
-        float s = -INFINITY;
-        if (tid < left) {
-            const KT *k = j < past ? kc + (size_t)j * a.hd : kd + (size_t)key[j - past] * a.hd;
-            float d = 0.0f;
-            for (int i = 0; i < a.hd; i += 4) {
-                const sdy_f32x4 v = KvElt<KT>::ld4(k, i);
-                for (int e = 0; e < 4; e++) d = __builtin_fmaf(q[i + e], v[e], d);
+    for (int round = 0; round < 8; round++) {
+        uint32_t add[MAX_NODES / 32];
+        int far = -1;
+        if (tid < MAX_NODES) {
+            const int p = up[tid];
+            if (p >= 0) {
+                far = up[p];
+                for (int w = 0; w < MAX_NODES / 32; w++) add[w] = mask[p][w];
+            } else {
+                for (int w = 0; w < MAX_NODES / 32; w++) add[w] = 0;
             }
-            s = d * scale;
         }
-        const float m_new = fmaxf(m, block_reduce(s, sh, true));
-        const float mu = m_new == -INFINITY ? 0.0f : m_new;
-        const float e = __expf(s - mu), corr = __expf(m - mu);
-        p[tid] = e;
-        l = l * corr + block_reduce(e, sh, false);
-        m = m_new;
         __syncthreads();
-        o *= corr;
-        if (tid < a.hd)
-            for (int i = 0; i < left && i < THREADS; i++) {
-                const KT *v = j0 + i < past ? vc + (size_t)(j0 + i) * a.hd : vd + (size_t)key[j0 + i - past] * a.hd;
-                o = __builtin_fmaf(p[i], KvElt<KT>::ld(v, tid), o);
-            }
+        if (tid < MAX_NODES) {
+            for (int w = 0; w < MAX_NODES / 32; w++) mask[tid][w] |= add[w];
+            up[tid] = (int16_t)far;
+        }
         __syncthreads();
     }
-    if (tid < a.hd) a.out[(size_t)t * a.out_stride + (size_t)h * a.hd + tid] = o / l;
+}
+
+template <int HD, class KT, int RW, int KW>
+__global__ __launch_bounds__(64 * RW * KW) void k_tree_part(TreeArgs A) {
+    using L = Lds<HD, KT, RW, KW>;
+    constexpr bool F32 = L::F32;
+    constexpr int NP = L::NP, RS = L::RS, ND = HD / 32, NS = HD / 16, GROUP = 64 * RW;
+    extern __shared__ __align__(16) unsigned char lds_bytes[];
+    const sdy_attn_tree_args &a = A.a;
+    const int past = *a.n_past;
+    if (past < 0 || past > a.max_past) return;
+    // all row blocks of one span and kv head on one XCD (workgroups are dealt to the 8 in turn): its L2 holds the tile
+    const int pairs = (1 + A.n_span) * a.n_kv_head;
+    const int id = (int)blockIdx.x, pair = (id / 8 / A.n_block) * 8 + id % 8, block = id / 8 % A.n_block;
+    if (pair >= pairs) return;
+    const int part = pair / a.n_kv_head, g = pair - part * a.n_kv_head;
+    const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, ql = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rw = wave % RW, kw = wave / RW, tg = tid - kw * GROUP;
+    const bool draft = part == 0;
+    int lo = 0, hi = a.n_tok;
+    if (!draft) {
+        const int per = span_rounds(A, past) * A.granule;
+        const long l0 = (long)(part - 1) * per, h0 = l0 + per;
+        if (l0 >= past) return;  // the merge does not look at it
+        lo = (int)l0;
+        hi = h0 < past ? (int)h0 : past;
+    }
+    const int rep = a.n_head / a.n_kv_head;
+    const int row = (block * RW + rw) * 32 + ql;
+    const bool live = row < A.rows;
+    const int node = live ? row / rep : 0;
+
+    uint16_t *const kt = reinterpret_cast<uint16_t *>(lds_bytes + kw * L::tile), *const vt = kt + NP * L::PLANE;
+    int *const ek = reinterpret_cast<int *>(lds_bytes + L::body) + kw * 96, *const ev = ek + 32;
+    float *const bad = reinterpret_cast<float *>(ek + 64);
+
+    uint32_t sees[MAX_NODES / 32];
+    if (draft) {
+        uint32_t(*mask)[MAX_NODES / 32] = reinterpret_cast<uint32_t(*)[MAX_NODES / 32]>(lds_bytes);
+        ancestor_masks(a.parent, a.n_tok, mask, reinterpret_cast<int16_t *>(mask + MAX_NODES));
+        for (int w = 0; w < MAX_NODES / 32; w++) sees[w] = live ? mask[node][w] : 0u;
+        __syncthreads();
+    }
+
+    // the rows' queries: step i holds dims 16 i + 8 hh .. + 7
+    f16x8 qh[NS], qlo[NS];
+    int eq = 0;
+    {
+        const float *q = a.q + (size_t)node * a.q_stride + (size_t)(g * rep + (live ? row - node * rep : 0)) * HD + 8 * hh;
+        float most = 0.0f;
+        float4 v[2 * NS];
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+            v[2 * i] = *reinterpret_cast<const float4 *>(q + 16 * i);
+            v[2 * i + 1] = *reinterpret_cast<const float4 *>(q + 16 * i + 4);
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * NS; i++)
+            most = fmaxf(most, fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
+        most = fmaxf(most, __shfl_xor(most, 32));
+        eq = row_exp(most);
+        const float sc = exp_scale(eq);
+        eq -= TOP;
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+            u32x4 h, l;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const float4 x = v[2 * i + e];
+                uint32_t h0, l0, h1, l1;
+                split2(x.x * sc, x.y * sc, h0, l0);
+                split2(x.z * sc, x.w * sc, h1, l1);
+                h[2 * e] = h0, h[2 * e + 1] = h1, l[2 * e] = l0, l[2 * e + 1] = l1;
+            }
+            qh[i] = __builtin_bit_cast(f16x8, h);
+            qlo[i] = __builtin_bit_cast(f16x8, l);
+        }
+    }
+
+    f32x16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++) o[d] = f32x16{};
+    float m = -INFINITY, l = 0.0f;  // m whole
+    int big = -1000;                // V's exponent that O is in
+
+    const size_t elt = sizeof(KT);
+    const char *kbase = (const char *)(draft ? a.k_draft : a.k_cache) + ((size_t)g * (draft ? a.draft_stride : a.head_stride) + (size_t)lo * HD) * elt;
+    const char *vbase = (const char *)(draft ? a.v_draft : a.v_cache) + ((size_t)g * (draft ? a.draft_stride : a.head_stride) + (size_t)lo * HD) * elt;
+    const int n_keys = hi - lo, size = n_keys * (int)(HD * sizeof(KT));  // (a span's bytes fit 31 bits: the host sees to it)
+    // positions past the span's end read as zeros and are masked below
+    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void *)kbase, (short)0, size, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void *)vbase, (short)0, size, 0x00020000);
+    const int rounds = (n_keys + KB * KW - 1) / (KB * KW);
+    Stage<HD, KT, RW> sk, sv;
+    sk.load(rk, (uint32_t)(kw * KB), tg);
+    sv.load(rv, (uint32_t)(kw * KB), tg);
+    auto sync = [&]() {
+        if constexpr (RW > 1) __syncthreads();
+        else sdy_wave_sync();
+    };
+    for (int it = 0; it < rounds; it++) {
+        const int k0 = (it * KW + kw) * KB;  // within the span
+        if (draft) {  // a row with an infinity or a NaN is NaN for those that see it and nothing for the others
+            const bool u = sv.unfit();
+            if (u) sv.clear();
+            if (tg % Stage<HD, KT, RW>::LPR == 0) bad[tg / Stage<HD, KT, RW>::LPR] = u ? NAN : 0.0f;
+        }
+        sk.store(kt, ek, tg);
+        sv.store(vt, ev, tg);
+        sync();
+        if (it + 1 < rounds) {
+            sk.load(rk, (uint32_t)(k0 + KW * KB), tg);
+            sv.load(rv, (uint32_t)(k0 + KW * KB), tg);
+        }
+        if (k0 < n_keys) {
+            f32x16 s = f32x16{}, sl = f32x16{};
+            const uint16_t *kr = kt + ql * RS + 8 * hh;
+#pragma unroll
+            for (int i = 0; i < NS; i++) {
+                const f16x8 k = *reinterpret_cast<const f16x8 *>(kr + 16 * i);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[i], s, 0, 0, 0);
+                sl = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qlo[i], sl, 0, 0, 0);
+                if constexpr (F32) {
+                    const f16x8 k2 = *reinterpret_cast<const f16x8 *>(kr + 32 * RS + 16 * i);
+                    sl = __builtin_amdgcn_mfma_f32_32x32x16_f16(k2, qh[i], sl, 0, 0, 0);
+                }
+            }
+            // register r: position 8 (r / 4) + 4 hh + r % 4 of the tile
+            float p[16], mt = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                int e[4] = {eq, eq, eq, eq};
+                if constexpr (F32) {
+                    const int4 x = *reinterpret_cast<const int4 *>(ek + 8 * b + 4 * hh);
+                    e[0] += x.x, e[1] += x.y, e[2] += x.z, e[3] += x.w;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) p[4 * b + j] = ldexpf(s[4 * b + j] + sl[4 * b + j], e[j]) * A.log_scale;
+            }
+            if (draft) {
+                const uint32_t bits = sees[k0 / KB] >> (4 * hh);
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int k = 8 * (r >> 2) + (r & 3);
+                    p[r] = bits >> k & 1 ? p[r] + bad[k + 4 * hh] : -INFINITY;
+                }
+            } else if (k0 + KB > n_keys) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) p[r] = k0 + 8 * (r >> 2) + 4 * hh + (r & 3) < n_keys ? p[r] : -INFINITY;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r++) mt = fmaxf(mt, p[r]);
+            mt = fmaxf(mt, __shfl_xor(mt, 32));
+            const float m_new = fmaxf(m, ceilf(mt));
+            const float mu = m_new == -INFINITY ? 0.0f : m_new;  // nothing seen yet: every weight is 0
+            const float ref = mu - P_BITS;
+            float ls = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                p[r] = __builtin_amdgcn_exp2f(p[r] - ref);
+                ls += p[r];
+            }
+            // exact: both maxima are whole
+            int down = m == -INFINITY ? -300 : (int)fmaxf(m - mu, -300.0f);
+            l = ldexpf(l, down) + ls;
+            m = m_new;
+            if constexpr (F32) {
+                int4 x[4];
+                int most = -1000;
+#pragma unroll
+                for (int b = 0; b < 4; b++) {
+                    x[b] = *reinterpret_cast<const int4 *>(ev + 8 * b + 4 * hh);
+                    const int y = x[b].x > x[b].y ? x[b].x : x[b].y, z = x[b].z > x[b].w ? x[b].z : x[b].w;
+                    const int w = y > z ? y : z;
+                    most = w > most ? w : most;
+                }
+                const int other = __shfl_xor(most, 32);
+                most = other > most ? other : most;
+                most = most > big ? most : big;
+#pragma unroll
+                for (int b = 0; b < 4; b++) {
+                    p[4 * b] = ldexpf(p[4 * b], x[b].x - most);
+                    p[4 * b + 1] = ldexpf(p[4 * b + 1], x[b].y - most);
+                    p[4 * b + 2] = ldexpf(p[4 * b + 2], x[b].z - most);
+                    p[4 * b + 3] = ldexpf(p[4 * b + 3], x[b].w - most);
+                }
+                down += big - most;
+                big = most;
+            }
+            if (__ballot(down != 0)) {
+#pragma unroll
+                for (int d = 0; d < ND; d++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[d][e] = ldexpf(o[d][e], down);
+            }
+            // step u: positions 16 u + 4 hh .. + 3 and 16 u + 8 + 4 hh .. + 3 of the tile, the scores' registers 8 u ..
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                u32x4 h, w;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    uint32_t h0, l0;
+                    split2(p[8 * u + 2 * j], p[8 * u + 2 * j + 1], h0, l0);
+                    h[j] = h0;
+                    w[j] = l0;
+                }
+                const f16x8 ph = __builtin_bit_cast(f16x8, h), pl = __builtin_bit_cast(f16x8, w);
+                // V^T by transposing reads: 16 lanes give the addresses of 4 rows x 16 dims (4 each) and get a dim's 4 rows
+                auto vread = [&](int plane, int d) {
+                    uint16_t *at = vt + plane * L::PLANE + (16 * u + 4 * hh + ((lane & 15) >> 2)) * RS + 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at);
+                    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(at + 8 * RS));
+                    return __builtin_bit_cast(f16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+                };
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    const f16x8 v = vread(0, d);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[d], 0, 0, 0);
+                    if constexpr (F32) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vread(1, d), ph, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[d], 0, 0, 0);
+                }
+            }
+        }
+        sync();
+    }
+    l += __shfl_xor(l, 32);
+    if constexpr (F32) {
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[d][e] = ldexpf(o[d][e], big);
+    }
+
+    const long all = (long)a.n_kv_head * A.rows;
+    float *const po = A.part + ((long)part * all + (long)g * A.rows) * HD;
+    float *const pm = A.part + (long)(1 + A.n_span) * all * HD + 2 * ((long)part * all + (long)g * A.rows);
+    if constexpr (KW == 1) {
+        if (live) {
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int b = 0; b < 4; b++)
+                    *reinterpret_cast<float4 *>(po + (long)row * HD + 32 * d + 8 * b + 4 * hh) =
+                        make_float4(o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]);
+            if (hh == 0) *reinterpret_cast<float2 *>(pm + 2 * row) = make_float2(m, l);
+        }
+    } else {
+        // the groups' (m, l, O) in group order
+        constexpr int ROWS = 32 * RW, OS = L::OS;
+        float *const om = reinterpret_cast<float *>(lds_bytes), *const ml = om + KW * ROWS * OS;
+        __syncthreads();
+        const int lr = rw * 32 + ql;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int b = 0; b < 4; b++)
+                *reinterpret_cast<float4 *>(om + (kw * ROWS + lr) * OS + 32 * d + 8 * b + 4 * hh) =
+                    make_float4(o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]);
+        if (hh == 0) {
+            ml[2 * (kw * ROWS + lr)] = m;
+            ml[2 * (kw * ROWS + lr) + 1] = l;
+        }
+        __syncthreads();
+        for (int i = tid; i < ROWS * HD / 4; i += 64 * RW * KW) {
+            const int r = i / (HD / 4), c = 4 * (i - r * (HD / 4)), gr = block * ROWS + r;
+            if (gr >= A.rows) continue;
+            float M = -INFINITY, ls = 0.0f;
+#pragma unroll
+            for (int w = 0; w < KW; w++) M = fmaxf(M, ml[2 * (w * ROWS + r)]);
+            const float mu = M == -INFINITY ? 0.0f : M;
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < KW; w++) {
+                const float x = __builtin_amdgcn_exp2f(ml[2 * (w * ROWS + r)] - mu);
+                const float4 y = *reinterpret_cast<const float4 *>(om + (w * ROWS + r) * OS + c);
+                ls += ml[2 * (w * ROWS + r) + 1] * x;
+                sum.x += y.x * x, sum.y += y.y * x, sum.z += y.z * x, sum.w += y.w * x;
+            }
+            *reinterpret_cast<float4 *>(po + (long)gr * HD + c) = sum;
+            if (c == 0) *reinterpret_cast<float2 *>(pm + 2 * gr) = make_float2(M, ls);
+        }
+    }
+}
+
+// The parts of one node and head in part order: 256 / (HD / 4) groups of lanes take parts in turn.
+template <int HD>
+__global__ __launch_bounds__(256) void k_tree_merge(TreeArgs A) {
+    constexpr int LN = HD / 4, NG = 256 / LN;
+    __shared__ float2 ml[MAX_PARTS];
+    __shared__ float red[4];
+    __shared__ float4 sums[NG][LN];
+    __shared__ float ls[NG];
+    const sdy_attn_tree_args &a = A.a;
+    const int past = *a.n_past, tid = threadIdx.x;
+    const int t = blockIdx.x, h = blockIdx.y;
+    if (past < 0 || past > a.max_past || a.parent[t] < -1) return;
+    const int n = 1 + spans_used(A, past), rep = a.n_head / a.n_kv_head, g = h / rep;
+    const long all = (long)a.n_kv_head * A.rows, row = (long)g * A.rows + (long)t * rep + (h - g * rep);
+    const float2 *pm = reinterpret_cast<const float2 *>(A.part + (long)(1 + A.n_span) * all * HD) + row;
+    float M = -INFINITY;
+    for (int p = tid; p < n; p += 256) {
+        ml[p] = pm[p * all];
+        M = fmaxf(M, ml[p].x);
+    }
+    for (int off = 32; off >= 1; off >>= 1) M = fmaxf(M, __shfl_xor(M, off));
+    if ((tid & 63) == 0) red[tid >> 6] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const int grp = tid / LN, ln = tid - grp * LN;
+    const float4 *po = reinterpret_cast<const float4 *>(A.part + row * HD) + ln;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float lsum = 0.0f;
+#pragma unroll 4
+    for (int p = grp; p < n; p += NG) {
+        const float4 y = po[p * all * LN];
+        const float x = __builtin_amdgcn_exp2f(ml[p].x - M);
+        lsum += ml[p].y * x;
+        sum.x += y.x * x, sum.y += y.y * x, sum.z += y.z * x, sum.w += y.w * x;
+    }
+    sums[grp][ln] = sum;
+    if (ln == 0) ls[grp] = lsum;
+    __syncthreads();
+    if (grp == 0) {
+        lsum = 0.0f;
+        sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < NG; i++) {
+            const float4 y = sums[i][ln];
+            lsum += ls[i];
+            sum.x += y.x, sum.y += y.y, sum.z += y.z, sum.w += y.w;
+        }
+        reinterpret_cast<float4 *>(a.out + (size_t)t * a.out_stride + (size_t)h * HD)[ln] =
+            make_float4(sum.x / lsum, sum.y / lsum, sum.z / lsum, sum.w / lsum);
+    }
+}
+
+// How the work is split, from the sizes alone.
+struct Plan {
+    int rw, kw, rows, n_block, n_span;
+};
+Plan plan_of(int n_tok, int n_head, int n_kv_head, int hd, int max_past) {
+    Plan p;
+    p.rows = n_tok * (n_head / n_kv_head);
+    p.rw = p.rows <= 32 && hd < 256 ? 1 : p.rows <= 64 ? 2 : 4;
+    p.kw = 4 / p.rw;
+    p.n_block = (p.rows + 32 * p.rw - 1) / (32 * p.rw);
+    const int granule = KB * p.kw;
+    const long pairs = (long)n_kv_head * p.n_block, rounds = ((long)max_past + granule - 1) / granule;
+    long n = (512 - pairs) / pairs;
+    if (n > rounds) n = rounds;
+    if (n > MAX_PARTS - 1) n = MAX_PARTS - 1;
+    // a span's bytes (at most 2^31 - 1 for a buffer resource)
+    const long least = (rounds * granule * hd * 4 + (1l << 30) - 1) >> 30;
+    if (n < least) n = least;
+    p.n_span = (int)(n < 1 ? 1 : n);
+    return p;
+}
+
+template <int HD, class KT, int RW, int KW>
+int launch_part(const TreeArgs &A, hipStream_t st) {
+    static size_t granted = 0;
+    const void *fn = (const void *)k_tree_part<HD, KT, RW, KW>;
+    const int rc = sdy_lds_limit(fn, Lds<HD, KT, RW, KW>::bytes, &granted);
+    if (rc) return rc;
+    SDY_NOTE_KERNEL((k_tree_part<HD, KT, RW, KW>));
+    const long pairs = (long)(1 + A.n_span) * A.a.n_kv_head;
+    hipLaunchKernelGGL((k_tree_part<HD, KT, RW, KW>), dim3((unsigned)((pairs + 7) / 8 * 8 * A.n_block)), dim3(64 * RW * KW),
+                       (Lds<HD, KT, RW, KW>::bytes), st, A);
+    return sdy_check_launch("attn_tree");
+}
+
+template <int HD, class KT>
+int launch_rows(const TreeArgs &A, int rw, hipStream_t st) {
+    if constexpr (HD < 256)
+        if (rw == 1) return launch_part<HD, KT, 1, 4>(A, st);
+    return rw == 2 ? launch_part<HD, KT, 2, 2>(A, st) : launch_part<HD, KT, 4, 1>(A, st);
+}
+
+template <int HD>
+int launch_tree(const TreeArgs &A, int rw, hipStream_t st) {
+    const int rc = A.a.kv_type == SDY_KV_F16 ? launch_rows<HD, uint16_t>(A, rw, st) : launch_rows<HD, float>(A, rw, st);
+    if (rc) return rc;
+    hipLaunchKernelGGL(k_tree_merge<HD>, dim3(A.a.n_tok, A.a.n_head), dim3(256), 0, st, A);
+    return sdy_check_launch("attn_tree merge");
 }
 
 }  // namespace
 
 extern "C" int sdy_attn_tree_ok(int n_tok, int n_head, int n_kv_head, int hd) {
-    return n_tok >= 1 && n_tok <= MAX_NODES && n_head >= 1 && n_kv_head >= 1 && n_head % n_kv_head == 0 &&
+    return n_tok >= 1 && n_tok <= MAX_NODES && n_head >= 1 && n_head <= 65535 && n_kv_head >= 1 && n_head % n_kv_head == 0 &&
            (hd == 64 || hd == 128 || hd == 256);
 }
 
 extern "C" size_t sdy_attn_tree_floats(int n_tok, int n_head, int n_kv_head, int hd, int max_past) {
-    if (!sdy_attn_tree_ok(n_tok, n_head, n_kv_head, hd) || max_past < 0) return 0;
-    return 64;
+    if (!sdy_attn_tree_ok(n_tok, n_head, n_kv_head, hd) || max_past < 0 || max_past > MAX_PAST) return 0;
+    const Plan p = plan_of(n_tok, n_head, n_kv_head, hd, max_past);
+    return (size_t)(1 + p.n_span) * n_kv_head * p.rows * (hd + 2);
 }
 
 extern "C" int sdy_attn_tree(const sdy_attn_tree_args *a, sdy_stream s) {
@@ -102,7 +617,7 @@ extern "C" int sdy_attn_tree(const sdy_attn_tree_args *a, sdy_stream s) {
     if (!elt) return sdy_fail(-1, "attn_tree: KV type %d", a->kv_type);
     if (!a->q || !a->k_draft || !a->v_draft || !a->parent || !a->n_past || !a->out || !a->part)
         return sdy_fail(-1, "attn_tree: q, the drafted rows, parent, n_past, out and part are needed");
-    if (a->max_past < 0 || (a->max_past > 0 && (!a->k_cache || !a->v_cache)))
+    if (a->max_past < 0 || a->max_past > MAX_PAST || (a->max_past > 0 && (!a->k_cache || !a->v_cache)))
         return sdy_fail(-1, "attn_tree: max_past %d and the caches", a->max_past);
     if (a->n_kv_head > 1 && (a->head_stride < (long)a->max_past * a->hd || a->draft_stride < (long)a->n_tok * a->hd))
         return sdy_fail(-1, "attn_tree: a kv head's rows (%d cached, %d drafted) reach into the next one's (strides %ld, %ld)",
@@ -114,10 +629,15 @@ extern "C" int sdy_attn_tree(const sdy_attn_tree_args *a, sdy_stream s) {
     if (a->q_stride < (long)a->n_head * a->hd || a->out_stride < (long)a->n_head * a->hd)
         return sdy_fail(-1, "attn_tree: q and out rows of %d x %d floats (strides %ld, %ld)", a->n_head, a->hd, a->q_stride,
                         a->out_stride);
-    const float scale = 1.0f / sqrtf((float)a->hd);
-    if (a->kv_type == SDY_KV_F16)
-        hipLaunchKernelGGL(k_attn_tree<uint16_t>, dim3(a->n_tok, a->n_head), dim3(THREADS), 0, (hipStream_t)s, *a, scale);
-    else
-        hipLaunchKernelGGL(k_attn_tree<float>, dim3(a->n_tok, a->n_head), dim3(THREADS), 0, (hipStream_t)s, *a, scale);
-    return sdy_check_launch("attn_tree");
+    const Plan p = plan_of(a->n_tok, a->n_head, a->n_kv_head, a->hd, a->max_past);
+    TreeArgs A;
+    A.a = *a;
+    A.rows = p.rows;
+    A.n_block = p.n_block;
+    A.n_span = p.n_span;
+    A.granule = KB * p.kw;
+    A.log_scale = (float)(1.4426950408889634074 / sqrt((double)a->hd));
+    A.part = a->part;
+    hipStream_t st = (hipStream_t)s;
+    return a->hd == 64 ? launch_tree<64>(A, p.rw, st) : a->hd == 128 ? launch_tree<128>(A, p.rw, st) : launch_tree<256>(A, p.rw, st);
 }

@@ -147,7 +147,7 @@ typedef struct {
     int kv_type;
     const int32_t *parent;       /* [n_tok] */
     const int32_t *n_past;       /* device int: the number of cached positions */
-    int max_past;                /* bound on *n_past (the scratch's size and the launch's) */
+    int max_past;                /* bound on *n_past (the scratch's size and the launch's), at most 2^28 */
     int n_tok, n_head, n_kv_head, hd; /* n_tok at most 256; hd 64, 128 or 256 */
     float *out;                  /* rows out_stride floats apart */
     long out_stride;

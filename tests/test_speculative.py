@@ -45,7 +45,7 @@ def tree_args(**kw):
     (dict(n_tok=257), "n_tok"), (dict(n_tok=-1), "n_tok"), (dict(n_head=7), "multiple"), (dict(n_kv_head=0), "multiple"),
     (dict(hd=96), "head_dim"), (dict(kv_type=3), "KV type"), (dict(q=None), "needed"), (dict(k_draft=None), "needed"),
     (dict(v_draft=None), "needed"), (dict(parent=None), "needed"), (dict(n_past=None), "needed"), (dict(out=None), "needed"),
-    (dict(part=None), "needed"), (dict(max_past=-1), "max_past"), (dict(k_cache=None), "cache"), (dict(v_cache=None), "cache"),
+    (dict(part=None), "needed"), (dict(max_past=-1), "max_past"), (dict(max_past=(1 << 28) + 1, head_stride=1 << 40), "max_past"), (dict(k_cache=None), "cache"), (dict(v_cache=None), "cache"),
     (dict(head_stride=64 * 49), "next one"), (dict(draft_stride=64 * 4), "next one"), (dict(q=P + 4), "aligned"),
     (dict(out=P + 8), "aligned"), (dict(q_stride=514), "aligned"), (dict(out_stride=513), "aligned"),
     (dict(k_cache=P + 2), "aligned"), (dict(kv_type=1, head_stride=64 * 50 + 4), "aligned"), (dict(q_stride=508), "rows of"),
