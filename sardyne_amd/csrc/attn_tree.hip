@@ -11,12 +11,13 @@
 //   S^T = K Q^T (a lane holds one row's 16 scores), the running maximum and sum, and O^T += V^T P.
 //   k_tree_merge<HD>  one workgroup per node and head: the spans' (m, l, O) in span order.
 //
-// Products on the f16 matrix cores at f32's precision: an f32 is the sum of two f16 (22 bits and a sign) once its row is
-// scaled by a power of two that brings the row's greatest value to 2^13 .. 2^14; the rest's least bit is then 2^-24, 2^-38 of
-// that value. q, P and an f32 cache's K and V are split so, an f16 cache's rows are taken as they are; of the split products
-// low x low, at most 2^-22 of the whole, is left out. Powers of two go back exactly (ldexp): K's and q's into the scores, V's
-// into P and, where a tile's greatest grows, into O. The running maximum is kept as a whole number (rounded up), so that its
-// rescales are exact too, and P is 2^14 times the weight: f16's least bit is 2^-39 of the greatest weight.
+// Products on the f16 matrix cores at f32's precision: an f32 is the sum of two f16 (22 bits and a sign) once it is scaled by
+// a power of two that keeps it well inside f16's range. q, P and an f32 cache's K and V are split so, an f16 cache's values are
+// taken as they are; of the split products low x low, at most 2^-22 of the whole, is left out. A row of q goes by its own
+// greatest value; a span's K and V by the greatest met so far, brought to 2^13 .. 2^16 (f16's least bit is then 2^-38 of it),
+// a power that changes with the first tile and seldom after. Powers of two go back exactly: K's and q's into the scores'
+// factor, V's into O (ldexp). The running maximum is kept as a whole number (rounded up), so that its rescales are exact too,
+// and P is 2^14 times the weight: f16's least bit is 2^-39 of the greatest weight.
 #include <type_traits>
 
 #include "sdy_attn_dev.h"
@@ -37,7 +38,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int MAX_NODES = 256;
 constexpr int KB = 32;         // positions per tile
-constexpr int TOP = 13;        // a scaled row's greatest value is 2^TOP .. 2^(TOP + 1)
+constexpr int TOP = 13;        // the greatest value is scaled to 2^TOP .. 2^(TOP + 1), later ones up to 2^(TOP + 3)
 constexpr float P_BITS = 14;   // P is 2^14 times the weight
 constexpr int MAX_PARTS = 513;
 constexpr int MAX_PAST = 1 << 28;  // 512 spans of at most 2^30 bytes hold them
@@ -70,25 +71,33 @@ struct Lds {
     static constexpr int PLANE = 32 * RS;
     static constexpr size_t tile = (size_t)2 * NP * PLANE * 2;   // bytes, K parts then V parts
     static constexpr size_t tiles = KW * tile;
-    static constexpr size_t scales = KW * 32 * 3 * 4;            // ek, ev, bad
+    static constexpr size_t flags = KW * 32 * 4 + 16;            // bad, the greatest |K| and |V|
     static constexpr size_t masks = MAX_NODES * (MAX_NODES / 32) * 4 + MAX_NODES * 2;
     static constexpr int OS = HD + 4;
     static constexpr size_t merge = KW > 1 ? (size_t)KW * 32 * RW * (OS + 2) * 4 : 0;
     static constexpr size_t body = tiles > merge ? (tiles > masks ? tiles : masks) : (merge > masks ? merge : masks);
-    static constexpr size_t bytes = body + scales;
+    static constexpr size_t bytes = body + flags;
 };
 
 // Two f32 as two f16 pairs, hi + lo = x up to 2^-23 of x (while lo is at least f16's least normal)
 SDY_DEV void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
+    float minus = -1.0f;  // (not left as a constant: one mixed multiply-add instead of a conversion and a difference)
+    __asm__("" : "+s"(minus));
     const f16x2 h = __builtin_convertvector(f32x2{a, b}, f16x2);
-    const f16x2 l = __builtin_convertvector(f32x2{a - (float)h[0], b - (float)h[1]}, f16x2);
+    const f16x2 l = __builtin_convertvector(f32x2{__builtin_fmaf((float)h[0], minus, a), __builtin_fmaf((float)h[1], minus, b)}, f16x2);
     hi = __builtin_bit_cast(uint32_t, h);
     lo = __builtin_bit_cast(uint32_t, l);
 }
 
-// The exponent of a row's greatest |value|, from 2^-100 on (smaller rows count as that), and the power of two that brings the
-// row to 2^TOP. An infinity or a NaN stays one.
-SDY_DEV int row_exp(float most) {
+// max(m, |a|, |b|) in one instruction (fmaxf makes its operands canonical first)
+SDY_DEV float max3_abs(float m, uint32_t a, uint32_t b) {
+    __asm__("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(a), "v"(b));
+    return m;
+}
+
+// The exponent of a greatest |value|, from 2^-100 on (smaller ones count as that), and the power of two that brings it to
+// 2^TOP. An infinity or a NaN stays one.
+SDY_DEV int exp_of(float most) {
     const int e = (int)(__float_as_uint(most) >> 23) - 127;
     return e > -100 ? e : -100;
 }
@@ -118,7 +127,7 @@ struct Stage {
             }
         }
     }
-    // Whether this thread's row has an infinity or a NaN
+    // Whether this row (of LPR threads) has an infinity or a NaN
     SDY_DEV bool unfit() const {
         uint32_t any = 0;
 #pragma unroll
@@ -138,25 +147,22 @@ struct Stage {
 #pragma unroll
             for (int w = 0; w < W; w++) r[i][w] = 0;
     }
-    // The row's parts to the planes at dst (row tg / LPR), its exponent to *exps
-    SDY_DEV void store(uint16_t *dst, int *exps, int tg) const {
+    // The greatest |value| of this thread's
+    SDY_DEV float most() const {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NC; i++)
+#pragma unroll
+            for (int w = 0; w < W; w += 2) m = max3_abs(m, r[i][w], r[i][w + 1]);
+        return m;
+    }
+    // The row's parts (f32: of the values times sc) to the planes at dst
+    SDY_DEV void store(uint16_t *dst, float sc, int tg) const {
         constexpr int RS = HD + 8;
-        const int row = tg / LPR, c0 = tg % LPR;
-        uint16_t *d = dst + row * RS + c0 * CE;
-        if constexpr (F32) {
-            float most = 0.0f;
+        uint16_t *d = dst + (tg / LPR) * RS + (tg % LPR) * CE;
 #pragma unroll
-            for (int i = 0; i < NC; i++)
-#pragma unroll
-                for (int w = 0; w < 4; w += 2)
-                    most = fmaxf(most, fmaxf(fabsf(__uint_as_float(r[i][w])), fabsf(__uint_as_float(r[i][w + 1]))));
-#pragma unroll
-            for (int off = 1; off < LPR; off *= 2) most = fmaxf(most, __shfl_xor(most, off));
-            const int e = row_exp(most);
-            const float sc = exp_scale(e);
-            if (c0 == 0) exps[row] = e - TOP;
-#pragma unroll
-            for (int i = 0; i < NC; i++) {
+        for (int i = 0; i < NC; i++) {
+            if constexpr (F32) {
                 u32x2 hi, lo;
 #pragma unroll
                 for (int w = 0; w < 2; w++) {
@@ -167,12 +173,10 @@ struct Stage {
                 }
                 *reinterpret_cast<u32x2 *>(d + i * LPR * CE) = hi;
                 *reinterpret_cast<u32x2 *>(d + 32 * RS + i * LPR * CE) = lo;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < NC; i++) {
-                if constexpr (W == 4) *reinterpret_cast<u32x4 *>(d + i * LPR * CE) = u32x4{r[i][0], r[i][1], r[i][2], r[i][3]};
-                else *reinterpret_cast<u32x2 *>(d + i * LPR * CE) = u32x2{r[i][0], r[i][1]};
+            } else if constexpr (W == 4) {
+                *reinterpret_cast<u32x4 *>(d + i * LPR * CE) = u32x4{r[i][0], r[i][1], r[i][2], r[i][3]};
+            } else {
+                *reinterpret_cast<u32x2 *>(d + i * LPR * CE) = u32x2{r[i][0], r[i][1]};
             }
         }
     }
@@ -241,8 +245,8 @@ __global__ __launch_bounds__(64 * RW * KW) void k_tree_part(TreeArgs A) {
     const int node = live ? row / rep : 0;
 
     uint16_t *const kt = reinterpret_cast<uint16_t *>(lds_bytes + kw * L::tile), *const vt = kt + NP * L::PLANE;
-    int *const ek = reinterpret_cast<int *>(lds_bytes + L::body) + kw * 96, *const ev = ek + 32;
-    float *const bad = reinterpret_cast<float *>(ek + 64);
+    float *const bad = reinterpret_cast<float *>(lds_bytes + L::body) + kw * 32;
+    unsigned *const greatest = reinterpret_cast<unsigned *>(lds_bytes + L::body) + KW * 32;
 
     uint32_t sees[MAX_NODES / 32];
     if (draft) {
@@ -268,7 +272,7 @@ __global__ __launch_bounds__(64 * RW * KW) void k_tree_part(TreeArgs A) {
         for (int i = 0; i < 2 * NS; i++)
             most = fmaxf(most, fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
         most = fmaxf(most, __shfl_xor(most, 32));
-        eq = row_exp(most);
+        eq = exp_of(most);
         const float sc = exp_scale(eq);
         eq -= TOP;
 #pragma unroll
@@ -291,7 +295,8 @@ __global__ __launch_bounds__(64 * RW * KW) void k_tree_part(TreeArgs A) {
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = f32x16{};
     float m = -INFINITY, l = 0.0f;  // m whole
-    int big = -1000;                // V's exponent that O is in
+    int xk = F32 ? -101 : TOP, xv = xk;  // the exponents that K's and V's scales go by (none yet for f32)
+    float factor = ldexpf(A.log_scale, eq);
 
     const size_t elt = sizeof(KT);
     const char *kbase = (const char *)(draft ? a.k_draft : a.k_cache) + ((size_t)g * (draft ? a.draft_stride : a.head_stride) + (size_t)lo * HD) * elt;
@@ -310,93 +315,97 @@ __global__ __launch_bounds__(64 * RW * KW) void k_tree_part(TreeArgs A) {
     };
     for (int it = 0; it < rounds; it++) {
         const int k0 = (it * KW + kw) * KB;  // within the span
-        if (draft) {  // a row with an infinity or a NaN is NaN for those that see it and nothing for the others
-            const bool u = sv.unfit();
-            if (u) sv.clear();
+        if (draft) {
+            // an empty place's rows are left out; rows with an infinity or a NaN are NaN for those that see them and nothing
+            // for the others
+            const int t = k0 + tg / Stage<HD, KT, RW>::LPR;
+            const bool u = sk.unfit() || sv.unfit();
+            if (u || t >= a.n_tok || a.parent[t] < -1) {
+                sk.clear();
+                sv.clear();
+            }
             if (tg % Stage<HD, KT, RW>::LPR == 0) bad[tg / Stage<HD, KT, RW>::LPR] = u ? NAN : 0.0f;
         }
-        sk.store(kt, ek, tg);
-        sv.store(vt, ev, tg);
+        if constexpr (F32) {
+            float mk = sk.most(), mv = sv.most();
+            const bool over = exp_of(mk) > xk + 2 || exp_of(mv) > xv + 2;
+            bool any;
+            if constexpr (RW > 1) any = __syncthreads_or(over);
+            else any = __ballot(over) != 0;
+            if (any) {  // new scales, the same for all that share tiles
+                for (int off = 32; off >= 1; off >>= 1) {
+                    mk = fmaxf(mk, __shfl_xor(mk, off));
+                    mv = fmaxf(mv, __shfl_xor(mv, off));
+                }
+                if constexpr (RW > 1) {
+                    if (tid < 2) greatest[tid] = 0;
+                    __syncthreads();
+                    if (lane == 0) {
+                        atomicMax(&greatest[0], __float_as_uint(mk));
+                        atomicMax(&greatest[1], __float_as_uint(mv));
+                    }
+                    __syncthreads();
+                    mk = __uint_as_float(greatest[0]);
+                    mv = __uint_as_float(greatest[1]);
+                }
+                if (exp_of(mk) > xk) xk = exp_of(mk);
+                const int x = exp_of(mv) > xv ? exp_of(mv) : xv;
+                factor = ldexpf(A.log_scale, eq + xk - TOP);
+#pragma unroll
+                for (int d = 0; d < ND; d++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[d][e] = ldexpf(o[d][e], xv - x);
+                xv = x;
+            }
+        }
+        sk.store(kt, exp_scale(xk), tg);
+        sv.store(vt, exp_scale(xv), tg);
         sync();
         if (it + 1 < rounds) {
             sk.load(rk, (uint32_t)(k0 + KW * KB), tg);
             sv.load(rv, (uint32_t)(k0 + KW * KB), tg);
         }
         if (k0 < n_keys) {
-            f32x16 s = f32x16{}, sl = f32x16{};
+            f32x16 s = f32x16{};
             const uint16_t *kr = kt + ql * RS + 8 * hh;
 #pragma unroll
             for (int i = 0; i < NS; i++) {
                 const f16x8 k = *reinterpret_cast<const f16x8 *>(kr + 16 * i);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qlo[i], s, 0, 0, 0);
+                if constexpr (F32)
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8 *>(kr + 32 * RS + 16 * i), qh[i], s, 0, 0, 0);
                 s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[i], s, 0, 0, 0);
-                sl = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qlo[i], sl, 0, 0, 0);
-                if constexpr (F32) {
-                    const f16x8 k2 = *reinterpret_cast<const f16x8 *>(kr + 32 * RS + 16 * i);
-                    sl = __builtin_amdgcn_mfma_f32_32x32x16_f16(k2, qh[i], sl, 0, 0, 0);
-                }
             }
             // register r: position 8 (r / 4) + 4 hh + r % 4 of the tile
-            float p[16], mt = -INFINITY;
-#pragma unroll
-            for (int b = 0; b < 4; b++) {
-                int e[4] = {eq, eq, eq, eq};
-                if constexpr (F32) {
-                    const int4 x = *reinterpret_cast<const int4 *>(ek + 8 * b + 4 * hh);
-                    e[0] += x.x, e[1] += x.y, e[2] += x.z, e[3] += x.w;
-                }
-#pragma unroll
-                for (int j = 0; j < 4; j++) p[4 * b + j] = ldexpf(s[4 * b + j] + sl[4 * b + j], e[j]) * A.log_scale;
-            }
             if (draft) {
+                __asm__ volatile("");  // (a branch: not worth a select per score)
                 const uint32_t bits = sees[k0 / KB] >> (4 * hh);
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const int k = 8 * (r >> 2) + (r & 3);
-                    p[r] = bits >> k & 1 ? p[r] + bad[k + 4 * hh] : -INFINITY;
+                    s[r] = bits >> k & 1 ? s[r] + bad[k + 4 * hh] : -INFINITY;
                 }
             } else if (k0 + KB > n_keys) {
+                __asm__ volatile("");
 #pragma unroll
-                for (int r = 0; r < 16; r++) p[r] = k0 + 8 * (r >> 2) + 4 * hh + (r & 3) < n_keys ? p[r] : -INFINITY;
+                for (int r = 0; r < 16; r++) s[r] = k0 + 8 * (r >> 2) + 4 * hh + (r & 3) < n_keys ? s[r] : -INFINITY;
             }
+            float mt = s[0];
 #pragma unroll
-            for (int r = 0; r < 16; r++) mt = fmaxf(mt, p[r]);
+            for (int r = 1; r < 16; r++) mt = fmaxf(mt, s[r]);
             mt = fmaxf(mt, __shfl_xor(mt, 32));
-            const float m_new = fmaxf(m, ceilf(mt));
+            const float m_new = fmaxf(m, ceilf(mt * factor));
             const float mu = m_new == -INFINITY ? 0.0f : m_new;  // nothing seen yet: every weight is 0
-            const float ref = mu - P_BITS;
-            float ls = 0.0f;
+            float p[16], ls = 0.0f;
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                p[r] = __builtin_amdgcn_exp2f(p[r] - ref);
+                p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], factor, P_BITS - mu));
                 ls += p[r];
             }
             // exact: both maxima are whole
-            int down = m == -INFINITY ? -300 : (int)fmaxf(m - mu, -300.0f);
+            const int down = m == -INFINITY ? -300 : (int)fmaxf(m - mu, -300.0f);
             l = ldexpf(l, down) + ls;
             m = m_new;
-            if constexpr (F32) {
-                int4 x[4];
-                int most = -1000;
-#pragma unroll
-                for (int b = 0; b < 4; b++) {
-                    x[b] = *reinterpret_cast<const int4 *>(ev + 8 * b + 4 * hh);
-                    const int y = x[b].x > x[b].y ? x[b].x : x[b].y, z = x[b].z > x[b].w ? x[b].z : x[b].w;
-                    const int w = y > z ? y : z;
-                    most = w > most ? w : most;
-                }
-                const int other = __shfl_xor(most, 32);
-                most = other > most ? other : most;
-                most = most > big ? most : big;
-#pragma unroll
-                for (int b = 0; b < 4; b++) {
-                    p[4 * b] = ldexpf(p[4 * b], x[b].x - most);
-                    p[4 * b + 1] = ldexpf(p[4 * b + 1], x[b].y - most);
-                    p[4 * b + 2] = ldexpf(p[4 * b + 2], x[b].z - most);
-                    p[4 * b + 3] = ldexpf(p[4 * b + 3], x[b].w - most);
-                }
-                down += big - most;
-                big = most;
-            }
             if (__ballot(down != 0)) {
 #pragma unroll
                 for (int d = 0; d < ND; d++)
@@ -438,7 +447,7 @@ __global__ __launch_bounds__(64 * RW * KW) void k_tree_part(TreeArgs A) {
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) o[d][e] = ldexpf(o[d][e], big);
+            for (int e = 0; e < 16; e++) o[d][e] = ldexpf(o[d][e], xv - TOP);
     }
 
     const long all = (long)a.n_kv_head * A.rows;
