@@ -166,7 +166,7 @@ int sdy_attn_tree(const sdy_attn_tree_args *a, sdy_stream s);
 typedef struct {
     const float *logits;         /* rows stride floats apart */
     long stride;
-    int n_rows, n_vocab;         /* n_vocab at most 2^22 */
+    int n_rows, n_vocab;         /* at most 65535, 2^22 */
     const float *temp;           /* [n_rows] each, or NULL: temperature 1, no top-k, no top-p, no min-p */
     const int32_t *top_k;
     const float *top_p, *min_p;

@@ -70,7 +70,7 @@ def sample_args(**kw):
 
 
 @pytest.mark.parametrize("kw,word", [
-    (dict(n_rows=-1), "n_rows"), (dict(n_vocab=0), "n_vocab"), (dict(n_vocab=(1 << 22) + 1), "n_vocab"),
+    (dict(n_rows=-1), "n_rows"), (dict(n_rows=65536), "n_rows"), (dict(n_vocab=0), "n_vocab"), (dict(n_vocab=(1 << 22) + 1), "n_vocab"),
     (dict(stride=99), "apart"), (dict(logits=None), "needed"), (dict(u=None), "needed"), (dict(token=None), "needed"),
     (dict(ws=None), "needed"), (dict(ws=P + 8), "aligned")])
 def test_sample_refusals(kw, word):
