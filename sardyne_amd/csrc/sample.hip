@@ -13,7 +13,8 @@
 // into pieces, a workgroup each (as many as fill the GPU), and read three times, the second and third from the caches:
 //   k_sample_max   each piece's greatest and lowest logit;
 //   k_sample_bins  each piece's tokens counted, and their w added, by distance from the greatest logit in 1024 bins;
-//   k_sample_list  from the bins, the one in which the prefix ends (with a small top_k all up to there): its tokens;
+//   k_sample_cut   one workgroup per row: the bin in which the prefix ends, and what is before it;
+//   k_sample_list  that bin's tokens (with a small top_k all up to there);
 //   k_sample_pick  one workgroup per row: these tokens sorted, the prefix's end among them, the pieces' sums, and the token
 //                  in its piece. A row whose end lies among more than 4096 tokens (nearly equal logits) is searched digit by
 //                  digit instead.
@@ -23,9 +24,9 @@
 
 namespace {
 
-constexpr int THREADS = 1024, WAVES = THREADS / 64;
+constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int MAX_VOCAB = 1 << 22;  // a token's place in the order fits 32 + 22 bits
-constexpr int BINS = THREADS;       // a thread each
+constexpr int BINS = 1024, PER = BINS / THREADS;  // a thread's bins
 constexpr int LIST = 4096;          // tokens that are sorted
 constexpr int SMALL_K = 1024;       // up to here the bins' sums are not made: the first top_k tokens are listed themselves
 constexpr int MAX_PIECES = 16;
@@ -48,20 +49,20 @@ struct Work {
     unsigned long long first[MAX_PIECES];  // the greatest place
     unsigned long long sums[MAX_PIECES];   // kept w before the listed bins
     float low[MAX_PIECES];                 // the lowest finite logit
-    int mode, n_list, bin_k, pad;
-    unsigned long long before;             // count or sum before the listed bins
+    unsigned offset[MAX_PIECES];           // where a piece's listed tokens start
+    int mode, n_list, b0, b1;              // the listed bins b0 .. b1
+    unsigned long long before;             // count or sum before them
     unsigned long long want;               // the sum that the prefix has to reach
     unsigned long long list[LIST];
 };
-// after them: per row and piece, BINS counts; then BINS sums
+// after them: per row and piece, BINS sums; then BINS counts
 
 enum { ROW_ALONE = 0,  // the first token, or none
        ROW_ALL,        // nothing is left out
        ROW_TOP,        // the listed tokens hold the whole prefix
        ROW_SUM,        // the prefix ends by its sum (or min-p) in the listed bins
        ROW_COUNT,      // the first top_k tokens end in the listed bin
-       ROW_SLOW,       // it ends among too many tokens to list
-       ROW_KNOWN };    // where it ends has been found
+       ROW_SLOW };     // it ends among too many tokens to list
 
 struct Args {
     sdy_sample_args a;
@@ -96,14 +97,20 @@ struct Row {
         if (!(min_p > 0.0f)) min_p = 0.0f;
         one = __longlong_as_double((1023ll + A.shift) << 52);
     }
+    // from the pieces' maxima, by each wave for itself
     SDY_DEV void maxima(const Args &A, int row) {
         const Work &w = A.work[row];
-        first = 0;
-        float low = INFINITY;
-        for (int c = 0; c < A.pieces; c++) {
-            first = w.first[c] > first ? w.first[c] : first;
-            low = fminf(low, w.low[c]);
+        const int c = (int)(threadIdx.x & 63) < A.pieces ? threadIdx.x & 63 : 0;
+        uint64_t m = w.first[c];
+        float low = w.low[c];
+#pragma unroll
+        for (int off = MAX_PIECES / 2; off >= 1; off /= 2) {
+            const uint64_t o = __shfl_xor((unsigned long long)m, off);
+            m = o > m ? o : m;
+            low = fminf(low, __shfl_xor(low, off));
         }
+        first = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(m >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)m);
+        low = __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(low)));
         best = value_at(first);
         none = !(best > -INFINITY);
         alone = none || !(temp > 0.0f);
@@ -112,6 +119,7 @@ struct Row {
         const float range = fminf(best - low, 43.0f * temp);
         per_bin = range > 0.0f ? (float)BINS / range : 0.0f;
     }
+    SDY_DEV bool sums() const { return !top_k || top_k > SMALL_K; }  // whether the bins' sums are made
     SDY_DEV bool cut() const { return top_k || top_p < 1.0f || min_p > 0.0f; }
     SDY_DEV double weight(float v) const {
         if (v == best) return 1.0;
@@ -123,10 +131,29 @@ struct Row {
     SDY_DEV int bin(float v) const { return v == best ? 0 : (int)fminf((best - v) * per_bin, (float)(BINS - 1)); }
 };
 
-// f(logit, index) of the tokens [lo, hi), eight loads in flight
+// f(logit, index) of the tokens [lo, hi) (lo a multiple of 4), four 16-byte loads in flight where the row allows them
 template <class F>
 SDY_DEV void each(const float *x, int lo, int hi, const F &f) {
-    for (int i0 = lo + (int)threadIdx.x; i0 < hi; i0 += 8 * THREADS) {
+    int i = lo;
+    if (((uintptr_t)x & 15) == 0) {
+        const int end = lo + (hi - lo) / 4 * 4;
+        for (int i0 = lo + 4 * (int)threadIdx.x; i0 < end; i0 += 16 * THREADS) {
+            float4 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) v[u] = *reinterpret_cast<const float4 *>(x + (i0 + 4 * u * THREADS < end ? i0 + 4 * u * THREADS : lo));
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int j = i0 + 4 * u * THREADS;
+                if (j >= end) continue;
+                f(v[u].x, j);
+                f(v[u].y, j + 1);
+                f(v[u].z, j + 2);
+                f(v[u].w, j + 3);
+            }
+        }
+        i = end;
+    }
+    for (int i0 = i + (int)threadIdx.x; i0 < hi; i0 += 8 * THREADS) {
         float v[8];
 #pragma unroll
         for (int u = 0; u < 8; u++) v[u] = x[i0 + u * THREADS < hi ? i0 + u * THREADS : hi - 1];
@@ -136,12 +163,19 @@ SDY_DEV void each(const float *x, int lo, int hi, const F &f) {
     }
 }
 
-struct Shared {
+struct Parts {
     float low[WAVES];
-    unsigned count[2048];
-    unsigned long long sum[2048];
     unsigned long long part[WAVES];
     unsigned long long found, before;
+};
+struct Shared : Parts {
+    union {
+        struct {
+            unsigned long long sum[2048];
+            unsigned count[2048];
+        };
+        unsigned long long w[LIST];  // the sorted tokens' w
+    };
 };
 
 SDY_DEV uint64_t wave_sum(uint64_t v) {
@@ -149,7 +183,7 @@ SDY_DEV uint64_t wave_sum(uint64_t v) {
     return v;
 }
 
-SDY_DEV uint64_t block_sum(uint64_t v, Shared &sh) {
+SDY_DEV uint64_t block_sum(uint64_t v, Parts &sh) {
     v = wave_sum(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh.part[threadIdx.x >> 6] = v;
@@ -159,7 +193,7 @@ SDY_DEV uint64_t block_sum(uint64_t v, Shared &sh) {
     return r;
 }
 
-SDY_DEV uint64_t block_max(uint64_t v, Shared &sh) {
+SDY_DEV uint64_t block_max(uint64_t v, Parts &sh) {
     for (int off = 32; off >= 1; off >>= 1) {
         const uint64_t o = __shfl_xor((unsigned long long)v, off);
         v = o > v ? o : v;
@@ -209,7 +243,7 @@ SDY_DEV uint64_t prefix_end(const Row &r, uint64_t least, bool by_sum, uint64_t 
 }
 
 // The sum over the threads before this one; *whole the sum over all.
-SDY_DEV uint64_t block_scan(uint64_t v, uint64_t *whole, Shared &sh) {
+SDY_DEV uint64_t block_scan(uint64_t v, uint64_t *whole, Parts &sh) {
     uint64_t run = v;
     for (int off = 1; off < 64; off *= 2) {
         const uint64_t o = __shfl_up((unsigned long long)run, off);
@@ -228,7 +262,7 @@ SDY_DEV uint64_t block_scan(uint64_t v, uint64_t *whole, Shared &sh) {
 }
 
 __global__ __launch_bounds__(THREADS) void k_sample_max(Args A) {
-    __shared__ Shared sh;
+    __shared__ Parts sh;
     const int c = blockIdx.x, row = blockIdx.y;
     const float *x = A.a.logits + (size_t)row * A.a.stride;
     const int lo = c * A.len, hi = lo + A.len < A.a.n_vocab ? lo + A.len : A.a.n_vocab;
@@ -250,7 +284,9 @@ __global__ __launch_bounds__(THREADS) void k_sample_max(Args A) {
 }
 
 __global__ __launch_bounds__(THREADS) void k_sample_bins(Args A) {
-    __shared__ Shared sh;
+    __shared__ Parts sh;
+    __shared__ unsigned count[BINS];
+    __shared__ unsigned long long sums_of[BINS];
     const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
     Row r;
     r.params(A, row);
@@ -264,36 +300,21 @@ __global__ __launch_bounds__(THREADS) void k_sample_bins(Args A) {
         if (tid == 0) A.work[row].sums[c] = sum;
         return;
     }
-    const bool sums = !r.top_k || r.top_k > SMALL_K;
-    sh.count[tid] = 0;
-    sh.sum[tid] = 0;
+    const bool sums = r.sums();
+    for (int b = tid; b < BINS; b += THREADS) count[b] = 0, sums_of[b] = 0;
     __syncthreads();
     each(r.x, lo, hi, [&](float v, int) {
         if (!(v > -INFINITY)) return;
         const int b = r.bin(v);
-        atomicAdd(&sh.count[b], 1u);
-        if (sums) atomicAdd(&sh.sum[b], (unsigned long long)r.fixed(v));
+        atomicAdd(&count[b], 1u);
+        if (sums) atomicAdd(&sums_of[b], (unsigned long long)r.fixed(v));
     });
     __syncthreads();
-    const size_t at = ((size_t)row * A.pieces + c) * BINS + tid;
-    A.count[at] = sh.count[tid];
-    if (sums) A.sum[at] = sh.sum[tid];
-}
-
-// The row's bins: this thread's count, sum, and the count in the pieces before c.
-SDY_DEV void bins_of(const Args &A, int row, int c, bool sums, unsigned *count, unsigned *before, uint64_t *sum) {
-    unsigned n = 0, nb = 0;
-    uint64_t w = 0;
-    const size_t at = (size_t)row * A.pieces * BINS + threadIdx.x;
-    for (int p = 0; p < A.pieces; p++) {
-        const unsigned x = A.count[at + (size_t)p * BINS];
-        n += x;
-        if (p < c) nb += x;
-        if (sums) w += A.sum[at + (size_t)p * BINS];
+    const size_t at = ((size_t)row * A.pieces + c) * BINS;
+    for (int b = tid; b < BINS; b += THREADS) {
+        A.count[at + b] = count[b];
+        if (sums) A.sum[at + b] = sums_of[b];
     }
-    *count = n;
-    *before = nb;
-    *sum = w;
 }
 
 // The least sum that reaches top_p of the whole
@@ -302,57 +323,80 @@ SDY_DEV uint64_t wanted(float top_p, uint64_t whole) {
     return want > 1.0 ? (uint64_t)want : 1;
 }
 
-// The first bin up to which there are `want` of v (the last one with any if there are fewer), and what is before it.
-SDY_DEV int bin_that_reaches(uint64_t v, uint64_t want, uint64_t *before, Shared &sh) {
-    uint64_t whole;
-    const uint64_t b = block_scan(v, &whole, sh);
-    if (want > whole) want = whole;
-    if (threadIdx.x == 0) sh.found = 0, sh.before = 0;
-    __syncthreads();
-    if (v && b < want && b + v >= want) sh.found = threadIdx.x, sh.before = b;
-    __syncthreads();
-    *before = sh.before;
-    const int f = (int)sh.found;
-    __syncthreads();
-    return f;
+// The row's bins PER * tid .. of this thread: counts and sums over the pieces.
+SDY_DEV void bins_of(const Args &A, int row, bool sums, uint64_t count[PER], uint64_t sum[PER]) {
+    static_assert(PER == 4, "a thread's bins are one 16-byte load of counts");
+    const size_t at = (size_t)row * A.pieces * BINS + PER * threadIdx.x;
+    for (int e = 0; e < PER; e++) count[e] = sum[e] = 0;
+#pragma unroll 4
+    for (int p = 0; p < A.pieces; p++) {
+        const uint4 n = *reinterpret_cast<const uint4 *>(A.count + at + (size_t)p * BINS);
+        count[0] += n.x, count[1] += n.y, count[2] += n.z, count[3] += n.w;
+        if (sums) {
+            const ulonglong2 a = *reinterpret_cast<const ulonglong2 *>(A.sum + at + (size_t)p * BINS);
+            const ulonglong2 b = *reinterpret_cast<const ulonglong2 *>(A.sum + at + (size_t)p * BINS + 2);
+            sum[0] += a.x, sum[1] += a.y, sum[2] += b.x, sum[3] += b.y;
+        }
+    }
 }
 
-__global__ __launch_bounds__(THREADS) void k_sample_list(Args A) {
-    __shared__ Shared sh;
-    __shared__ unsigned n_mine;
-    const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
+// The threads' bins: v's running sums, the whole, the bin at which `want` is reached (the last one with any if it never is)
+// and what is before it.
+struct Reach {
+    uint64_t whole, before;
+    int bin;
+};
+SDY_DEV Reach bin_that_reaches(const uint64_t v[PER], uint64_t want, float top_p, Parts &sh) {
+    Reach r;
+    const uint64_t mine = v[0] + v[1] + v[2] + v[3];
+    uint64_t run = block_scan(mine, &r.whole, sh);
+    if (top_p < 1.0f) want = wanted(top_p, r.whole);
+    if (want > r.whole) want = r.whole;
+    if (threadIdx.x == 0 && r.whole == 0) sh.found = 0, sh.before = 0;
+    if (run < want && run + mine >= want) {
+        int e = 0;
+        while (e < PER - 1 && run + v[e] < want) run += v[e++];
+        sh.found = PER * threadIdx.x + e;
+        sh.before = run;
+    }
+    __syncthreads();
+    r.bin = (int)sh.found;
+    r.before = sh.before;
+    return r;
+}
+
+__global__ __launch_bounds__(THREADS) void k_sample_cut(Args A) {
+    __shared__ Parts sh;
+    __shared__ unsigned listed_of[MAX_PIECES];
+    const int row = blockIdx.x, tid = threadIdx.x;
     Work &w = A.work[row];
     Row r;
     r.params(A, row);
     r.maxima(A, row);
     if (r.alone || !r.cut()) {
-        if (c == 0 && tid == 0) w.mode = r.alone ? ROW_ALONE : ROW_ALL;
+        if (tid == 0) w.mode = r.alone ? ROW_ALONE : ROW_ALL;
         return;
     }
-    const bool sums = !r.top_k || r.top_k > SMALL_K;
-    unsigned count, mine_before;
-    uint64_t sum;
-    bins_of(A, row, c, sums, &count, &mine_before, &sum);
-    int b0 = 0, b1 = BINS - 1, mode = ROW_SUM, bk = 0;
-    uint64_t before = 0, want = ~0ull;
+    const bool sums = r.sums();
+    uint64_t count[PER], sum[PER];
+    bins_of(A, row, sums, count, sum);
+    int b0 = 0, b1 = BINS - 1, mode = ROW_SUM;
+    uint64_t want = ~0ull;
     if (r.top_k) {
-        bk = bin_that_reaches(count, (uint64_t)r.top_k, &before, sh);
-        uint64_t all;
-        block_scan(tid <= bk ? count : 0, &all, sh);
-        b1 = bk;
+        const Reach k = bin_that_reaches(count, (uint64_t)r.top_k, 1.0f, sh);
+        b1 = k.bin;
         mode = ROW_TOP;
-        if (all > LIST) {
-            b0 = bk;
+        uint64_t all = 0;
+        for (int e = 0; e < PER; e++) all += PER * tid + e <= b1 ? count[e] : 0;
+        if (block_sum(all, sh) > LIST) {
+            b0 = b1;
             mode = sums ? ROW_COUNT : ROW_SLOW;
-        } else {
-            before = 0;
         }
     } else {
         if (r.top_p < 1.0f) {
-            uint64_t whole;
-            block_scan(sum, &whole, sh);
-            want = wanted(r.top_p, whole);
-            b0 = b1 = bin_that_reaches(sum, want, &before, sh);
+            const Reach p = bin_that_reaches(sum, 0, r.top_p, sh);
+            want = wanted(r.top_p, p.whole);
+            b0 = b1 = p.bin;
         }
         if (r.min_p > 0.0f) {
             // the bins that the border can be in: their arithmetic is in 32 bits
@@ -362,46 +406,89 @@ __global__ __launch_bounds__(THREADS) void k_sample_list(Args A) {
             b0 = r.top_p < 1.0f && b0 < lo ? b0 : lo;
             b1 = hi < b1 ? hi : b1;
         }
-        uint64_t b = block_sum(tid < b0 ? sum : 0, sh);
-        before = b;
     }
-    uint64_t listed;
-    const bool in = tid >= b0 && tid <= b1;
-    listed = block_sum(in ? count : 0, sh);
-    const uint64_t offset = block_sum(in ? mine_before : 0, sh);
-    const uint64_t above = block_sum(sums && tid < b0 ? A.sum[((size_t)row * A.pieces + c) * BINS + tid] : 0, sh);
+    uint64_t listed = 0, before = 0;
+    for (int e = 0; e < PER; e++) {
+        const int b = PER * tid + e;
+        listed += b >= b0 && b <= b1 ? count[e] : 0;
+        before += b < b0 ? (mode == ROW_COUNT ? count[e] : sum[e]) : 0;
+    }
+    listed = block_sum(listed, sh);
+    before = block_sum(before, sh);
     if (listed > LIST) mode = ROW_SLOW;
     if (tid == 0) {
-        w.sums[c] = above;
-        n_mine = (unsigned)offset;
-        if (c == 0) {
-            w.mode = mode;
-            w.n_list = (int)listed;
-            w.bin_k = bk;
-            w.before = before;
-            w.want = want;
+        w.mode = mode;
+        w.n_list = (int)listed;
+        w.b0 = b0;
+        w.b1 = b1;
+        w.before = before;
+        w.want = want;
+    }
+    // per piece, a wave each in turn: its listed tokens, then their offsets, and its sum before the listed bins
+    const int lane = tid & 63;
+    for (int p = tid >> 6; p < A.pieces; p += WAVES) {
+        const size_t at = ((size_t)row * A.pieces + p) * BINS;
+        uint64_t n = 0, s = 0;
+        for (int b = b0 + lane; b <= b1; b += 64) n += A.count[at + b];
+        if (sums)
+            for (int b = lane; b < b0; b += 64) s += A.sum[at + b];
+        n = wave_sum(n);
+        s = wave_sum(s);
+        if (lane == 0) {
+            listed_of[p] = (unsigned)n;
+            w.sums[p] = s;
         }
     }
-    if (mode == ROW_SLOW) return;
+    __syncthreads();
+    if (tid < A.pieces) {
+        unsigned n = 0;
+        for (int p = 0; p < tid; p++) n += listed_of[p];
+        w.offset[tid] = n;
+    }
+}
+
+__global__ __launch_bounds__(THREADS) void k_sample_list(Args A) {
+    __shared__ unsigned next;
+    const int c = blockIdx.x, row = blockIdx.y;
+    Work &w = A.work[row];
+    const int mode = w.mode;
+    if (mode != ROW_TOP && mode != ROW_SUM && mode != ROW_COUNT) return;
+    Row r;
+    r.params(A, row);
+    r.maxima(A, row);
+    const int b0 = w.b0, b1 = w.b1;
+    if (threadIdx.x == 0) next = w.offset[c];
     __syncthreads();
     const int lo = c * A.len, hi = lo + A.len < r.n ? lo + A.len : r.n;
     each(r.x, lo, hi, [&](float v, int i) {
         if (!(v > -INFINITY)) return;
         const int b = r.bin(v);
-        if (b >= b0 && b <= b1) w.list[atomicAdd(&n_mine, 1u)] = place_of(v, i);
+        if (b >= b0 && b <= b1) w.list[atomicAdd(&next, 1u)] = place_of(v, i);
     });
 }
 
-// list[0 .. n) in falling order (a power of two from n on is sorted, padded with zeros)
+// list[0 .. n) in falling order, all different. Up to 256: each one's rank counted, one round. Above: a bitonic sort of the
+// next power of two, padded with zeros.
 SDY_DEV void sort_falling(unsigned long long *list, int n) {
-    int n2 = 1;
+    __syncthreads();
+    if (n <= THREADS) {
+        const unsigned long long mine = (int)threadIdx.x < n ? list[threadIdx.x] : 0;
+        int rank = 0;
+#pragma unroll 8
+        for (int i = 0; i < n; i++) rank += list[i] > mine;
+        __syncthreads();
+        if ((int)threadIdx.x < n) list[rank] = mine;
+        __syncthreads();
+        return;
+    }
+    int n2 = 2 * THREADS;
     while (n2 < n) n2 *= 2;
     for (int i = n + threadIdx.x; i < n2; i += THREADS) list[i] = 0;
     __syncthreads();
     for (int k = 2; k <= n2; k *= 2)
         for (int j = k / 2; j > 0; j /= 2) {
             for (int t = threadIdx.x; t < n2 / 2; t += THREADS) {
-                const int i = (t / j) * 2 * j + t % j;
+                const int i = ((t & ~(j - 1)) << 1) | (t & (j - 1));
                 const unsigned long long x = list[i], y = list[i + j];
                 if ((x < y) == ((i & k) == 0)) list[i] = y, list[i + j] = x;
             }
@@ -411,7 +498,7 @@ SDY_DEV void sort_falling(unsigned long long *list, int n) {
 
 // The piece [lo, hi) narrowed to the token at which the running sum of kept(i) passes `left`
 template <class F>
-SDY_DEV int narrow(int lo, int hi, uint64_t left, const F &kept, Shared &sh) {
+SDY_DEV int narrow(int lo, int hi, uint64_t left, const F &kept, Parts &sh) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     while (hi - lo > 1) {
         const int len = (hi - lo + WAVES - 1) / WAVES;
@@ -438,18 +525,28 @@ SDY_DEV uint64_t share(float u, uint64_t whole) {
     return t < whole ? t : whole - 1;
 }
 
+struct Pick {
+    Shared sh;
+    unsigned long long list[LIST];
+    unsigned long long sums[MAX_PIECES];
+    int n_list;
+};
+
 __global__ __launch_bounds__(THREADS) void k_sample_pick(Args A) {
-    __shared__ Shared sh;
-    __shared__ unsigned long long list[LIST];
-    __shared__ unsigned long long sums[MAX_PIECES];
-    __shared__ int n_list;
+    extern __shared__ __align__(16) unsigned char lds_bytes[];
+    Pick &k = *reinterpret_cast<Pick *>(lds_bytes);
+    Shared &sh = k.sh;
+    unsigned long long *const list = k.list;
     const sdy_sample_args &a = A.a;
     const int row = blockIdx.x, tid = threadIdx.x;
-    Work &w = A.work[row];
+    const Work &w = A.work[row];
+    int mode = w.mode, n = w.n_list;
+    if (mode == ROW_TOP || mode == ROW_SUM || mode == ROW_COUNT)
+        for (int i = tid; i < n; i += THREADS) list[i] = w.list[i];
     Row r;
     r.params(A, row);
     r.maxima(A, row);
-    if (r.alone) {
+    if (mode == ROW_ALONE) {
         if (tid == 0) {
             a.token[row] = r.none ? -1 : index_at(r.first);
             if (a.prob) a.prob[row] = r.none ? 0.0f : 1.0f;
@@ -457,7 +554,6 @@ __global__ __launch_bounds__(THREADS) void k_sample_pick(Args A) {
         return;
     }
     const float u = a.u[row];
-    int mode = w.mode, n = w.n_list;
     uint64_t least = 0;  // the place that the prefix ends at
     auto kept_place = [&](uint64_t at) -> uint64_t {
         if (at < least) return 0;
@@ -466,131 +562,110 @@ __global__ __launch_bounds__(THREADS) void k_sample_pick(Args A) {
     };
     auto kept = [&](int i) { return kept_place(place_of(r.x[i], i)); };
     auto take = [&](int i, uint64_t v, uint64_t whole) {
-        if (tid == 0) {
-            a.token[row] = i;
-            if (a.prob) a.prob[row] = (float)((double)v / (double)whole);
-        }
+        a.token[row] = i;
+        if (a.prob) a.prob[row] = (float)((double)v / (double)whole);
     };
-    if (mode == ROW_TOP || mode == ROW_SUM || mode == ROW_COUNT) {
-        for (int i = tid; i < n; i += THREADS) list[i] = w.list[i];
-        __syncthreads();
-        sort_falling(list, n);
-    }
-    // thread t holds the sorted tokens t * LIST / THREADS ..
-    constexpr int PER = LIST / THREADS;
-    auto weights = [&](uint64_t v[PER], int limit) {
+    if (mode == ROW_TOP || mode == ROW_SUM || mode == ROW_COUNT) sort_falling(list, n);
+    // thread t holds the sorted tokens t * per .. t * per + per - 1 of the first `limit`; sh.w[i] is the i-th one's w
+    auto weights = [&](int limit, int per) {
         uint64_t s = 0;
-#pragma unroll
-        for (int e = 0; e < PER; e++) {
-            const int i = tid * PER + e;
-            v[e] = i < limit ? r.fixed(value_at(list[i])) : 0;
-            s += v[e];
-        }
+        for (int i = tid * per; i < limit && i < tid * per + per; i++) s += sh.w[i] = r.fixed(value_at(list[i]));
         return s;
     };
-    // the place that a prefix by sum ends at, `before` of it standing ahead of the list
+    // the place that a prefix by sum ends at, `before` of it standing ahead of the list. want 0: top_p of the list
     auto end_by_sum = [&](int limit, uint64_t before, uint64_t want) {
-        uint64_t v[PER], whole;
-        uint64_t run = before + block_scan(weights(v, limit), &whole, sh);
+        const int per = (limit + THREADS - 1) / THREADS;
+        __syncthreads();  // (sh.w shares its memory)
+        uint64_t whole;
+        uint64_t run = before + block_scan(weights(limit, per), &whole, sh);
+        if (want == 0) want = wanted(r.top_p, whole);
         uint64_t last = ~0ull;
-#pragma unroll
-        for (int e = 0; e < PER; e++) {
-            const int i = tid * PER + e;
-            if (i < limit && run < want) last = list[i];
-            run += v[e];
+        for (int i = tid * per; i < limit && i < tid * per + per && run < want; i++) {
+            last = list[i];
+            run += sh.w[i];
         }
-        const uint64_t m = block_max(last == ~0ull ? 0 : ~last, sh);  // the least of them
+        const uint64_t m = block_max(~last, sh);  // the least of them
         return m ? ~m : 0ull;
     };
-    if (mode == ROW_COUNT) {  // many tokens by count: the end of the first top_k is known now, and with it their sum
-        const int rest = r.top_k - (int)w.before, end = rest < n ? rest : n;  // of the list
-        least = list[end - 1];
-        if (r.top_p < 1.0f) {
-            unsigned count, none;
-            uint64_t sum, whole, before;
-            bins_of(A, row, 0, true, &count, &none, &sum);
-            const uint64_t above = block_sum(tid < w.bin_k ? sum : 0, sh);
-            uint64_t v[PER];
-            whole = above + block_sum(weights(v, end), sh);
-            const uint64_t want = wanted(r.top_p, whole);
-            if (above < want) {
-                least = end_by_sum(end, above, want);
-            } else {  // the sum ends in an earlier bin, whose tokens nobody has listed
-                const int b = bin_that_reaches(tid < w.bin_k ? sum : 0, want, &before, sh);
-                const uint64_t c = block_sum(tid == b ? count : 0, sh);
-                if (c > LIST) {
-                    mode = ROW_SLOW;
-                } else {
-                    if (tid == 0) n_list = 0;
-                    __syncthreads();
-                    each(r.x, 0, r.n, [&](float x, int i) {
-                        if (x > -INFINITY && r.bin(x) == b) list[atomicAdd(&n_list, 1)] = place_of(x, i);
-                    });
-                    __syncthreads();
-                    sort_falling(list, (int)c);
-                    least = end_by_sum((int)c, before, want);
-                }
-            }
-        }
-        if (mode == ROW_COUNT) mode = ROW_KNOWN;
-    } else if (mode == ROW_TOP) {
+    if (mode == ROW_TOP) {
         if (n > r.top_k) n = r.top_k;
-        if (r.top_p < 1.0f) {
-            uint64_t v[PER];
-            const uint64_t whole = block_sum(weights(v, n), sh);
-            least = end_by_sum(n, 0, wanted(r.top_p, whole));
-        }
+        if (r.top_p < 1.0f) least = end_by_sum(n, 0, 0);
         // the kept ones, a prefix of the list, by index: the place's halves change sides
-        int end = 0;
+        uint64_t end = 0;
         for (int i = tid; i < n; i += THREADS) {
             const uint64_t at = list[i];
             const bool in = at >= least && (at == r.first || !(r.weight(value_at(at)) < (double)r.min_p));
             end += in;
             list[i] = in ? (at & (MAX_VOCAB - 1)) << 32 | at >> 22 : 0;
         }
-        n = (int)block_sum((uint64_t)end, sh);
+        n = (int)block_sum(end, sh);
         sort_falling(list, n);
-        uint64_t v[PER], sum = 0, whole;
-#pragma unroll
-        for (int e = 0; e < PER; e++) {
-            const int i = tid * PER + e;
-            v[e] = i < n ? r.fixed(value_at((list[i] & 0xFFFFFFFFu) << 22)) : 0;
-            sum += v[e];
-        }
+        const int per = (n + THREADS - 1) / THREADS;
+        uint64_t sum = 0, whole;
+        for (int i = tid * per; i < n && i < tid * per + per; i++) sum += sh.w[i] = r.fixed(value_at((list[i] & 0xFFFFFFFFu) << 22));
         uint64_t run = block_scan(sum, &whole, sh);
         const uint64_t left = share(u, whole);
         if (run <= left && left < run + sum) {
-#pragma unroll
-            for (int e = 0; e < PER; e++) {
-                if (run <= left && left < run + v[e]) {
-                    const int i = tid * PER + e;
-                    a.token[row] = MAX_VOCAB - 1 - (int)(list[i] >> 32);
-                    if (a.prob) a.prob[row] = (float)((double)v[e] / (double)whole);
-                }
-                run += v[e];
-            }
+            int i = tid * per;
+            while (run + sh.w[i] <= left) run += sh.w[i++];
+            take(MAX_VOCAB - 1 - (int)(list[i] >> 32), sh.w[i], whole);
         }
         return;
-    } else if (mode == ROW_SUM || mode == ROW_ALL) {
-        if (tid < A.pieces) sums[tid] = w.sums[tid];
+    }
+    if (mode == ROW_SUM || mode == ROW_ALL) {
+        if (tid < A.pieces) k.sums[tid] = w.sums[tid];
         __syncthreads();
         if (mode == ROW_SUM) {
             if (r.top_p < 1.0f) least = end_by_sum(n, w.before, w.want);
             if (least == 0 && n) least = list[n - 1];
             for (int i = tid; i < n; i += THREADS) {
                 const uint64_t v = kept_place(list[i]);
-                if (v) atomicAdd(&sums[index_at(list[i]) / A.len], (unsigned long long)v);
+                if (v) atomicAdd(&k.sums[index_at(list[i]) / A.len], (unsigned long long)v);
             }
             __syncthreads();
         }
         uint64_t whole = 0;
-        for (int p = 0; p < A.pieces; p++) whole += sums[p];
+        for (int p = 0; p < A.pieces; p++) whole += k.sums[p];
         uint64_t left = share(u, whole);
         int p = 0;
-        while (p < A.pieces - 1 && sums[p] <= left) left -= sums[p++];
+        while (p < A.pieces - 1 && k.sums[p] <= left) left -= k.sums[p++];
         const int lo = p * A.len, i = narrow(lo, lo + A.len < r.n ? lo + A.len : r.n, left, kept, sh);
-        take(i, kept(i), whole);
+        if (tid == 0) take(i, kept(i), whole);
         return;
+    }
+    if (mode == ROW_COUNT) {  // many tokens by count: the end of the first top_k is known now, and with it their sum
+        const int rest = r.top_k - (int)w.before, end = rest < n ? rest : n;  // of the list
+        least = list[end - 1];
+        if (r.top_p < 1.0f) {
+            uint64_t count[PER], sum[PER], ahead = 0, in_list = 0;
+            bins_of(A, row, true, count, sum);
+            for (int e = 0; e < PER; e++) {
+                if (PER * tid + e >= w.b0) sum[e] = 0;
+                ahead += sum[e];
+            }
+            ahead = block_sum(ahead, sh);
+            in_list = block_sum(weights(end, (end + THREADS - 1) / THREADS), sh);
+            const uint64_t want = wanted(r.top_p, ahead + in_list);
+            if (ahead < want) {
+                least = end_by_sum(end, ahead, want);
+            } else {  // the sum ends in an earlier bin, whose tokens nobody has listed
+                const Reach b = bin_that_reaches(sum, want, 1.0f, sh);
+                uint64_t c = 0;
+                for (int e = 0; e < PER; e++) c += PER * tid + e == b.bin ? count[e] : 0;
+                c = block_sum(c, sh);
+                if (c > LIST) {
+                    mode = ROW_SLOW;
+                } else {
+                    if (tid == 0) k.n_list = 0;
+                    __syncthreads();
+                    each(r.x, 0, r.n, [&](float x, int i) {
+                        if (x > -INFINITY && r.bin(x) == b.bin) list[atomicAdd(&k.n_list, 1)] = place_of(x, i);
+                    });
+                    sort_falling(list, (int)c);
+                    least = end_by_sum((int)c, b.before, want);
+                }
+            }
+        }
     }
     if (mode == ROW_SLOW) {
         least = 0;
@@ -607,15 +682,14 @@ __global__ __launch_bounds__(THREADS) void k_sample_pick(Args A) {
     for (int i = tid; i < r.n; i += THREADS) whole += kept(i);
     whole = block_sum(whole, sh);
     const int i = narrow(0, r.n, share(u, whole), kept, sh);
-    take(i, kept(i), whole);
+    if (tid == 0) take(i, kept(i), whole);
 }
 
 // Pieces per row: enough workgroups for the GPU where there are few rows, none shorter than 4096 tokens.
 int pieces_of(int n_rows, int n_vocab) {
-    int p = 256 / n_rows;
-    if (p > MAX_PIECES) p = MAX_PIECES;
-    if (p > (n_vocab + 4095) / 4096) p = (n_vocab + 4095) / 4096;
-    return p < 1 ? 1 : p;
+    int p = (n_vocab + 4095) / 4096;
+    (void)n_rows;
+    return p < MAX_PIECES ? p : MAX_PIECES;
 }
 
 }  // namespace
@@ -640,15 +714,19 @@ extern "C" int sdy_sample(const sdy_sample_args *a, sdy_stream s) {
     while ((1 << log2) < a->n_vocab) log2++;
     A.shift = 62 - log2;
     A.pieces = pieces_of(a->n_rows, a->n_vocab);
-    A.len = (a->n_vocab + A.pieces - 1) / A.pieces;
+    A.len = ((a->n_vocab + A.pieces - 1) / A.pieces + 3) & ~3;
     A.work = (Work *)a->ws;
     A.sum = (unsigned long long *)(A.work + a->n_rows);
     A.count = (unsigned *)(A.sum + (size_t)a->n_rows * A.pieces * BINS);
+    static size_t granted = 0;
+    const int rc = sdy_lds_limit((const void *)k_sample_pick, sizeof(Pick), &granted);
+    if (rc) return rc;
     const dim3 grid(A.pieces, a->n_rows), block(THREADS);
     hipStream_t st = (hipStream_t)s;
     hipLaunchKernelGGL(k_sample_max, grid, block, 0, st, A);
     hipLaunchKernelGGL(k_sample_bins, grid, block, 0, st, A);
+    hipLaunchKernelGGL(k_sample_cut, dim3(a->n_rows), block, 0, st, A);
     hipLaunchKernelGGL(k_sample_list, grid, block, 0, st, A);
-    hipLaunchKernelGGL(k_sample_pick, dim3(a->n_rows), block, 0, st, A);
+    hipLaunchKernelGGL(k_sample_pick, dim3(a->n_rows), block, sizeof(Pick), st, A);
     return sdy_check_launch("sample");
 }
