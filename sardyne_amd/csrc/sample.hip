@@ -9,15 +9,15 @@
 // of integers, so no order of adding, split or atomic changes a token. A w below 2^-S, 30 T under the greatest logit for that
 // vocabulary, is never chosen.
 //
-// Every kept set is a prefix of the order, so what is looked for is where it ends, without sorting the row. The row is cut
-// into pieces, a workgroup each (as many as fill the GPU), and read three times, the second and third from the caches:
+// Every kept set is a prefix of the order, so what is looked for is where it ends, without sorting the row. Rows of up to
+// 4096 tokens are a workgroup's work in LDS (k_sample_small). A longer row is cut into pieces, a workgroup each, and read
+// three times, the second and third from the caches:
 //   k_sample_max   each piece's greatest and lowest logit;
 //   k_sample_bins  each piece's tokens counted, and their w added, by distance from the greatest logit in 1024 bins;
 //   k_sample_cut   one workgroup per row: the bin in which the prefix ends, and what is before it;
 //   k_sample_list  that bin's tokens (with a small top_k all up to there);
-//   k_sample_pick  one workgroup per row: these tokens sorted, the prefix's end among them, the pieces' sums, and the token
-//                  in its piece. A row whose end lies among more than 4096 tokens (nearly equal logits) is searched digit by
-//                  digit instead.
+//   k_sample_pick  one workgroup per row: the prefix's end among these tokens, the pieces' sums, and the token in its piece.
+//                  A row whose end lies among more than 4096 tokens (nearly equal logits) is searched digit by digit instead.
 #include "sdy_device.h"
 #include "sdy_internal.h"
 #include "sdy_ops.h"
@@ -26,8 +26,8 @@ namespace {
 
 constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int MAX_VOCAB = 1 << 22;  // a token's place in the order fits 32 + 22 bits
-constexpr int BINS = 1024, PER = BINS / THREADS;  // a thread's bins
-constexpr int LIST = 4096;          // tokens that are sorted
+constexpr int BINS = 1024;
+constexpr int LIST = 4096;          // tokens that one workgroup holds
 constexpr int SMALL_K = 1024;       // up to here the bins' sums are not made: the first top_k tokens are listed themselves
 constexpr int MAX_PIECES = 16;
 
@@ -69,8 +69,8 @@ struct Args {
     int shift;    // S
     int pieces, len;
     Work *work;
-    unsigned *count;           // [n_rows][pieces][BINS]
     unsigned long long *sum;   // [n_rows][pieces][BINS]
+    unsigned *count;           // [n_rows][pieces][BINS]
 };
 
 struct Row {
@@ -97,6 +97,16 @@ struct Row {
         if (!(min_p > 0.0f)) min_p = 0.0f;
         one = __longlong_as_double((1023ll + A.shift) << 52);
     }
+    SDY_DEV void start(uint64_t place, float low) {
+        first = place;
+        best = value_at(first);
+        none = !(best > -INFINITY);
+        alone = none || !(temp > 0.0f);
+        inv_t = 1.0 / (double)temp;
+        // over the whole of the finite logits, or as far down as a w counts (2^-62 is exp(-43))
+        const float range = fminf(best - low, 43.0f * temp);
+        per_bin = range > 0.0f ? (float)BINS / range : 0.0f;
+    }
     // from the pieces' maxima, by each wave for itself
     SDY_DEV void maxima(const Args &A, int row) {
         const Work &w = A.work[row];
@@ -109,15 +119,8 @@ struct Row {
             m = o > m ? o : m;
             low = fminf(low, __shfl_xor(low, off));
         }
-        first = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(m >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)m);
-        low = __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(low)));
-        best = value_at(first);
-        none = !(best > -INFINITY);
-        alone = none || !(temp > 0.0f);
-        inv_t = 1.0 / (double)temp;
-        // over the whole of the finite logits, or as far down as a w counts (2^-62 is exp(-43))
-        const float range = fminf(best - low, 43.0f * temp);
-        per_bin = range > 0.0f ? (float)BINS / range : 0.0f;
+        start((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(m >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)m),
+              __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(low))));
     }
     SDY_DEV bool sums() const { return !top_k || top_k > SMALL_K; }  // whether the bins' sums are made
     SDY_DEV bool cut() const { return top_k || top_p < 1.0f || min_p > 0.0f; }
@@ -127,6 +130,11 @@ struct Row {
         return exp(((double)v - (double)best) * inv_t);
     }
     SDY_DEV uint64_t fixed(float v) const { return (uint64_t)(weight(v) * one); }  // w as a whole number of 2^-S
+    // the same where min-p leaves the token, else 0
+    SDY_DEV uint64_t fixed_kept(uint64_t place) const {
+        const double w = weight(value_at(place));
+        return place == first || !(w < (double)min_p) ? (uint64_t)(w * one) : 0;
+    }
     // never less for a lower logit
     SDY_DEV int bin(float v) const { return v == best ? 0 : (int)fminf((best - v) * per_bin, (float)(BINS - 1)); }
 };
@@ -163,19 +171,13 @@ SDY_DEV void each(const float *x, int lo, int hi, const F &f) {
     }
 }
 
+// ---- sums over a block of W waves
+
+template <int W>
 struct Parts {
-    float low[WAVES];
-    unsigned long long part[WAVES];
-    unsigned long long found, before;
-};
-struct Shared : Parts {
-    union {
-        struct {
-            unsigned long long sum[2048];
-            unsigned count[2048];
-        };
-        unsigned long long w[LIST];  // the sorted tokens' w
-    };
+    float low[W];
+    unsigned long long part[W];
+    unsigned long long key, val, run;  // what one thread found
 };
 
 SDY_DEV uint64_t wave_sum(uint64_t v) {
@@ -183,17 +185,19 @@ SDY_DEV uint64_t wave_sum(uint64_t v) {
     return v;
 }
 
-SDY_DEV uint64_t block_sum(uint64_t v, Parts &sh) {
+template <int W>
+SDY_DEV uint64_t block_sum(uint64_t v, Parts<W> &sh) {
     v = wave_sum(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh.part[threadIdx.x >> 6] = v;
     __syncthreads();
     uint64_t r = 0;
-    for (int w = 0; w < WAVES; w++) r += sh.part[w];
+    for (int w = 0; w < W; w++) r += sh.part[w];
     return r;
 }
 
-SDY_DEV uint64_t block_max(uint64_t v, Parts &sh) {
+template <int W>
+SDY_DEV uint64_t block_max(uint64_t v, Parts<W> &sh) {
     for (int off = 32; off >= 1; off >>= 1) {
         const uint64_t o = __shfl_xor((unsigned long long)v, off);
         v = o > v ? o : v;
@@ -202,48 +206,13 @@ SDY_DEV uint64_t block_max(uint64_t v, Parts &sh) {
     if ((threadIdx.x & 63) == 0) sh.part[threadIdx.x >> 6] = v;
     __syncthreads();
     uint64_t r = 0;
-    for (int w = 0; w < WAVES; w++) r = sh.part[w] > r ? sh.part[w] : r;
+    for (int w = 0; w < W; w++) r = sh.part[w] > r ? sh.part[w] : r;
     return r;
 }
 
-// The place of the last token of the shortest prefix, among tokens from place `least` on, that has `want` tokens
-// (by_sum false) or a sum of `want` (true): 54 bits, 11 at a time from the top.
-SDY_DEV uint64_t prefix_end(const Row &r, uint64_t least, bool by_sum, uint64_t want, Shared &sh) {
-    uint64_t head = 0, before = 0;
-    for (int shift = 44; shift > -11; shift -= 11) {
-        const int s = shift < 0 ? 0 : shift, bits = shift < 0 ? 11 + shift : 11;
-        __syncthreads();
-        for (int i = threadIdx.x; i < 2048; i += THREADS) sh.count[i] = 0, sh.sum[i] = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < r.n; i += THREADS) {
-            const float v = r.x[i];
-            const uint64_t at = place_of(v, i);
-            if (at < least || at >> (s + bits) != head) continue;
-            const int d = (int)(at >> s) & ((1 << bits) - 1);
-            if (by_sum) atomicAdd(&sh.sum[d], (unsigned long long)r.fixed(v));
-            else atomicAdd(&sh.count[d], 1u);
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            uint64_t sum = before;
-            int d = (1 << bits) - 1;
-            for (; d > 0; d--) {
-                const uint64_t more = by_sum ? sh.sum[d] : sh.count[d];
-                if (sum + more >= want) break;
-                sum += more;
-            }
-            sh.found = d;
-            sh.before = sum;
-        }
-        __syncthreads();
-        head = head << bits | sh.found;
-        before = sh.before;
-    }
-    return head;
-}
-
 // The sum over the threads before this one; *whole the sum over all.
-SDY_DEV uint64_t block_scan(uint64_t v, uint64_t *whole, Parts &sh) {
+template <int W>
+SDY_DEV uint64_t block_scan(uint64_t v, uint64_t *whole, Parts<W> &sh) {
     uint64_t run = v;
     for (int off = 1; off < 64; off *= 2) {
         const uint64_t o = __shfl_up((unsigned long long)run, off);
@@ -253,7 +222,7 @@ SDY_DEV uint64_t block_scan(uint64_t v, uint64_t *whole, Parts &sh) {
     if ((threadIdx.x & 63) == 63) sh.part[threadIdx.x >> 6] = run;
     __syncthreads();
     uint64_t before = 0, all = 0;
-    for (int w = 0; w < WAVES; w++) {
+    for (int w = 0; w < W; w++) {
         if (w < (int)(threadIdx.x >> 6)) before += sh.part[w];
         all += sh.part[w];
     }
@@ -261,8 +230,232 @@ SDY_DEV uint64_t block_scan(uint64_t v, uint64_t *whole, Parts &sh) {
     return before + run - v;
 }
 
+// The thread whose v takes the running sum from `before` to `want`: its number in sh.key, what runs before it in sh.run (the
+// last thread where all of it is less).
+template <int W>
+SDY_DEV void reach(uint64_t v, uint64_t before, uint64_t want, Parts<W> &sh) {
+    uint64_t whole;
+    const uint64_t run = before + block_scan(v, &whole, sh);
+    if ((run < want && run + v >= want) || (threadIdx.x == 64 * W - 1 && run + v < want)) sh.key = threadIdx.x, sh.run = run;
+    __syncthreads();
+}
+
+// The least sum that reaches top_p of the whole
+SDY_DEV uint64_t wanted(float top_p, uint64_t whole) {
+    const double want = ceil((double)top_p * (double)whole);
+    return want > 1.0 ? (uint64_t)want : 1;
+}
+
+// u of the whole, in 0 .. whole - 1
+SDY_DEV uint64_t share(float u, uint64_t whole) {
+    if (!(u > 0.0f)) return 0;
+    if (u >= 1.0f) return whole - 1;
+    const uint64_t t = (uint64_t)((double)u * (double)whole);
+    return t < whole ? t : whole - 1;
+}
+
+// ---- among the tokens of one workgroup
+
+constexpr int SUB = THREADS;
+struct Lds {
+    Parts<WAVES> parts;
+    unsigned long long list[LIST];  // places
+    union {
+        unsigned long long w[LIST];  // their w
+        struct {                     // prefix_end's, which has no list
+            unsigned long long digit_sum[2048];
+            unsigned digit_count[2048];
+        };
+    };
+    unsigned long long sub_sum[SUB], near[64], near_w[64], sums[MAX_PIECES];
+    unsigned sub_count[SUB];
+    int n;
+};
+
+// Of n things with different key(i), in falling order, the one at which the running sum of val(i) from `before` on reaches
+// `want`: its key, its val and what runs before it. It exists: before < want <= before and the whole. The keys' range is cut
+// into 256 and the piece that holds it again, until 64 things are left; these count each other.
+struct Found {
+    uint64_t key, val, run;
+};
+template <class K, class V>
+SDY_DEV Found find(int n, const K &key, const V &val, uint64_t before, uint64_t want, Lds &k) {
+    const int tid = threadIdx.x;
+    uint64_t hi = 0, lo = ~0ull;
+    for (int i = tid; i < n; i += THREADS)
+        if (val(i)) {
+            const uint64_t x = key(i);
+            hi = x > hi ? x : hi;
+            lo = x < lo ? x : lo;
+        }
+    hi = block_max(hi, k.parts);
+    lo = ~block_max(~lo, k.parts);
+    if (n > 64)
+        for (;;) {
+            const int bits = 64 - __builtin_clzll((hi - lo) | 1), shift = bits > 8 ? bits - 8 : 0;
+            k.sub_sum[tid] = 0;
+            k.sub_count[tid] = 0;
+            __syncthreads();
+            for (int i = tid; i < n; i += THREADS) {
+                const uint64_t x = key(i), v = val(i);
+                if (v && x >= lo && x <= hi) {
+                    atomicAdd(&k.sub_sum[(hi - x) >> shift], (unsigned long long)v);
+                    atomicAdd(&k.sub_count[(hi - x) >> shift], 1u);
+                }
+            }
+            __syncthreads();
+            reach(k.sub_sum[tid], before, want, k.parts);
+            const int d = (int)k.parts.key, c = (int)k.sub_count[d];
+            before = k.parts.run;
+            hi -= (uint64_t)d << shift;
+            const uint64_t l = hi - ((1ull << shift) - 1);
+            if (l > lo && l <= hi) lo = l;
+            __syncthreads();
+            if (c <= 64 || shift == 0) break;
+        }
+    if (tid == 0) k.n = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += THREADS) {
+        const uint64_t x = key(i), v = val(i);
+        if (v && x >= lo && x <= hi) {
+            const int at = atomicAdd(&k.n, 1);
+            k.near[at] = x;
+            k.near_w[at] = v;
+        }
+    }
+    __syncthreads();
+    if (tid < k.n) {
+        const uint64_t x = k.near[tid], v = k.near_w[tid];
+        uint64_t run = before;
+        for (int i = 0; i < k.n; i++) run += k.near[i] > x ? k.near_w[i] : 0;
+        if (run < want && run + v >= want) k.parts.key = x, k.parts.val = v, k.parts.run = run;
+    }
+    __syncthreads();
+    const Found f = {k.parts.key, k.parts.val, k.parts.run};
+    __syncthreads();
+    return f;
+}
+
+SDY_DEV void take(const Args &A, int row, int token, uint64_t w, uint64_t whole) {
+    A.a.token[row] = token;
+    if (A.a.prob) A.a.prob[row] = (float)((double)w / (double)whole);
+}
+
+// The token of a row that is alone, or none
+SDY_DEV void take_alone(const Args &A, int row, const Row &r) {
+    A.a.token[row] = r.none ? -1 : index_at(r.first);
+    if (A.a.prob) A.a.prob[row] = r.none ? 0.0f : 1.0f;
+}
+
+// The token of a row whose kept ones are all among the n in the list.
+SDY_DEV void pick_listed(const Args &A, int row, const Row &r, int n, Lds &k) {
+    const int tid = threadIdx.x;
+    for (int i = tid; i < n; i += THREADS) k.w[i] = r.fixed(value_at(k.list[i]));
+    __syncthreads();
+    uint64_t least = 0, sum = 0;
+    auto place = [&](int i) -> uint64_t { return k.list[i]; };
+    if (r.top_k && n > r.top_k)
+        least = find(n, place, [](int) -> uint64_t { return 1; }, 0, (uint64_t)r.top_k, k).key;
+    if (r.top_p < 1.0f) {
+        for (int i = tid; i < n; i += THREADS) sum += k.list[i] >= least ? k.w[i] : 0;
+        sum = block_sum(sum, k.parts);
+        least = find(n, place, [&](int i) -> uint64_t { return k.list[i] >= least ? k.w[i] : 0; }, 0, wanted(r.top_p, sum), k).key;
+        sum = 0;
+    }
+    for (int i = tid; i < n; i += THREADS) {
+        if (k.list[i] < least) k.w[i] = 0;
+        else if (r.min_p > 0.0f) k.w[i] = r.fixed_kept(k.list[i]);
+        sum += k.w[i];
+    }
+    sum = block_sum(sum, k.parts);
+    // by index now
+    const Found f = find(n, [&](int i) -> uint64_t { return k.list[i] & (MAX_VOCAB - 1); }, [&](int i) -> uint64_t { return k.w[i]; }, 0,
+                         share(A.a.u[row], sum) + 1, k);
+    if (tid == 0) take(A, row, MAX_VOCAB - 1 - (int)f.key, f.val, sum);
+}
+
+// Of the tokens [lo, hi) the one at which the running sum of kept(i) passes `left`
+template <class F>
+SDY_DEV int narrow(int lo, int hi, uint64_t left, const F &kept, Lds &k) {
+    while (hi - lo > 1) {
+        const int per = (hi - lo + THREADS - 1) / THREADS, b = lo + (int)threadIdx.x * per, e = b + per < hi ? b + per : hi;
+        uint64_t sum = 0;
+#pragma unroll 4
+        for (int i = b; i < e; i++) sum += kept(i);
+        reach(sum, 0, left + 1, k.parts);
+        lo = lo + (int)k.parts.key * per < hi ? lo + (int)k.parts.key * per : hi - 1;
+        hi = lo + per < hi ? lo + per : hi;
+        left -= k.parts.run;
+        __syncthreads();
+    }
+    return lo;
+}
+
+// The place of the last token of the shortest prefix, among tokens from place `least` on, that has `want` tokens
+// (by_sum false) or a sum of `want` (true): 54 bits, 11 at a time from the top.
+SDY_DEV uint64_t prefix_end(const Row &r, uint64_t least, bool by_sum, uint64_t want, Lds &k) {
+    uint64_t head = 0, before = 0;
+    for (int shift = 44; shift > -11; shift -= 11) {
+        const int s = shift < 0 ? 0 : shift, bits = shift < 0 ? 11 + shift : 11;
+        __syncthreads();
+        for (int i = threadIdx.x; i < 2048; i += THREADS) k.digit_count[i] = 0, k.digit_sum[i] = 0;
+        __syncthreads();
+        each(r.x, 0, r.n, [&](float v, int i) {
+            const uint64_t at = place_of(v, i);
+            if (at < least || at >> (s + bits) != head) return;
+            const int d = (int)(at >> s) & ((1 << bits) - 1);
+            if (by_sum) atomicAdd(&k.digit_sum[d], (unsigned long long)r.fixed(v));
+            else atomicAdd(&k.digit_count[d], 1u);
+        });
+        __syncthreads();
+        // the digits from the top, 8 a thread
+        const int top = 2047 - 8 * (int)threadIdx.x;
+        uint64_t mine = 0;
+        for (int e = 0; e < 8; e++) mine += by_sum ? k.digit_sum[top - e] : k.digit_count[top - e];
+        uint64_t whole;
+        uint64_t run = before + block_scan(mine, &whole, k.parts);
+        if (threadIdx.x == 0 && before + whole < want) k.parts.key = 0, k.parts.run = before;  // (fewer than wanted: the last)
+        if (run < want && run + mine >= want) {
+            int d = top;
+            for (;; d--) {
+                const uint64_t more = by_sum ? k.digit_sum[d] : k.digit_count[d];
+                if (run + more >= want) break;
+                run += more;
+            }
+            k.parts.key = (uint64_t)d;
+            k.parts.run = run;
+        }
+        __syncthreads();
+        head = head << bits | k.parts.key;
+        before = k.parts.run;
+    }
+    return head;
+}
+
+// ---- the kernels
+
+__global__ __launch_bounds__(THREADS) void k_sample_small(Args A) {
+    extern __shared__ __align__(16) unsigned char lds_bytes[];
+    Lds &k = *reinterpret_cast<Lds *>(lds_bytes);
+    const int row = blockIdx.x, tid = threadIdx.x;
+    Row r;
+    r.params(A, row);
+    uint64_t first = 0;
+    each(r.x, 0, r.n, [&](float v, int i) {
+        const uint64_t at = place_of(v, i);
+        k.list[i] = at;
+        first = at > first ? at : first;
+    });
+    r.start(block_max(first, k.parts), 0.0f);
+    if (r.alone) {
+        if (tid == 0) take_alone(A, row, r);
+        return;
+    }
+    pick_listed(A, row, r, r.n, k);
+}
+
 __global__ __launch_bounds__(THREADS) void k_sample_max(Args A) {
-    __shared__ Parts sh;
+    __shared__ Parts<WAVES> sh;
     const int c = blockIdx.x, row = blockIdx.y;
     const float *x = A.a.logits + (size_t)row * A.a.stride;
     const int lo = c * A.len, hi = lo + A.len < A.a.n_vocab ? lo + A.len : A.a.n_vocab;
@@ -284,9 +477,9 @@ __global__ __launch_bounds__(THREADS) void k_sample_max(Args A) {
 }
 
 __global__ __launch_bounds__(THREADS) void k_sample_bins(Args A) {
-    __shared__ Parts sh;
+    __shared__ Parts<WAVES> sh;
     __shared__ unsigned count[BINS];
-    __shared__ unsigned long long sums_of[BINS];
+    __shared__ unsigned long long sum_of[BINS];
     const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
     Row r;
     r.params(A, row);
@@ -301,74 +494,30 @@ __global__ __launch_bounds__(THREADS) void k_sample_bins(Args A) {
         return;
     }
     const bool sums = r.sums();
-    for (int b = tid; b < BINS; b += THREADS) count[b] = 0, sums_of[b] = 0;
+    for (int b = tid; b < BINS; b += THREADS) count[b] = 0, sum_of[b] = 0;
     __syncthreads();
     each(r.x, lo, hi, [&](float v, int) {
         if (!(v > -INFINITY)) return;
         const int b = r.bin(v);
         atomicAdd(&count[b], 1u);
-        if (sums) atomicAdd(&sums_of[b], (unsigned long long)r.fixed(v));
+        if (sums) atomicAdd(&sum_of[b], (unsigned long long)r.fixed(v));
     });
     __syncthreads();
     const size_t at = ((size_t)row * A.pieces + c) * BINS;
     for (int b = tid; b < BINS; b += THREADS) {
         A.count[at + b] = count[b];
-        if (sums) A.sum[at + b] = sums_of[b];
+        if (sums) A.sum[at + b] = sum_of[b];
     }
 }
 
-// The least sum that reaches top_p of the whole
-SDY_DEV uint64_t wanted(float top_p, uint64_t whole) {
-    const double want = ceil((double)top_p * (double)whole);
-    return want > 1.0 ? (uint64_t)want : 1;
-}
-
-// The row's bins PER * tid .. of this thread: counts and sums over the pieces.
-SDY_DEV void bins_of(const Args &A, int row, bool sums, uint64_t count[PER], uint64_t sum[PER]) {
-    static_assert(PER == 4, "a thread's bins are one 16-byte load of counts");
-    const size_t at = (size_t)row * A.pieces * BINS + PER * threadIdx.x;
-    for (int e = 0; e < PER; e++) count[e] = sum[e] = 0;
-#pragma unroll 4
-    for (int p = 0; p < A.pieces; p++) {
-        const uint4 n = *reinterpret_cast<const uint4 *>(A.count + at + (size_t)p * BINS);
-        count[0] += n.x, count[1] += n.y, count[2] += n.z, count[3] += n.w;
-        if (sums) {
-            const ulonglong2 a = *reinterpret_cast<const ulonglong2 *>(A.sum + at + (size_t)p * BINS);
-            const ulonglong2 b = *reinterpret_cast<const ulonglong2 *>(A.sum + at + (size_t)p * BINS + 2);
-            sum[0] += a.x, sum[1] += a.y, sum[2] += b.x, sum[3] += b.y;
-        }
-    }
-}
-
-// The threads' bins: v's running sums, the whole, the bin at which `want` is reached (the last one with any if it never is)
-// and what is before it.
-struct Reach {
-    uint64_t whole, before;
-    int bin;
-};
-SDY_DEV Reach bin_that_reaches(const uint64_t v[PER], uint64_t want, float top_p, Parts &sh) {
-    Reach r;
-    const uint64_t mine = v[0] + v[1] + v[2] + v[3];
-    uint64_t run = block_scan(mine, &r.whole, sh);
-    if (top_p < 1.0f) want = wanted(top_p, r.whole);
-    if (want > r.whole) want = r.whole;
-    if (threadIdx.x == 0 && r.whole == 0) sh.found = 0, sh.before = 0;
-    if (run < want && run + mine >= want) {
-        int e = 0;
-        while (e < PER - 1 && run + v[e] < want) run += v[e++];
-        sh.found = PER * threadIdx.x + e;
-        sh.before = run;
-    }
-    __syncthreads();
-    r.bin = (int)sh.found;
-    r.before = sh.before;
-    return r;
-}
-
-__global__ __launch_bounds__(THREADS) void k_sample_cut(Args A) {
-    __shared__ Parts sh;
-    __shared__ unsigned listed_of[MAX_PIECES];
-    const int row = blockIdx.x, tid = threadIdx.x;
+// A wave per piece, 16 bins a lane; then a bin per thread.
+__global__ __launch_bounds__(BINS) void k_sample_cut(Args A) {
+    constexpr int W = BINS / 64, EACH = BINS / 64;
+    static_assert(W == MAX_PIECES, "a wave per piece");
+    __shared__ Parts<W> sh;
+    __shared__ unsigned count_of[BINS], listed_of[MAX_PIECES];
+    __shared__ unsigned long long sum_of[BINS];
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, p = tid >> 6;
     Work &w = A.work[row];
     Row r;
     r.params(A, row);
@@ -378,25 +527,41 @@ __global__ __launch_bounds__(THREADS) void k_sample_cut(Args A) {
         return;
     }
     const bool sums = r.sums();
-    uint64_t count[PER], sum[PER];
-    bins_of(A, row, sums, count, sum);
+    count_of[tid] = 0;
+    sum_of[tid] = 0;
+    unsigned n[EACH];
+    unsigned long long s[EACH];
+    const size_t at = ((size_t)row * A.pieces + p) * BINS + lane;
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        n[e] = p < A.pieces ? A.count[at + 64 * e] : 0;
+        s[e] = sums && p < A.pieces ? A.sum[at + 64 * e] : 0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        if (n[e]) atomicAdd(&count_of[64 * e + lane], n[e]);
+        if (s[e]) atomicAdd(&sum_of[64 * e + lane], s[e]);
+    }
+    __syncthreads();
+    const uint64_t count = count_of[tid], sum = sum_of[tid];
     int b0 = 0, b1 = BINS - 1, mode = ROW_SUM;
-    uint64_t want = ~0ull;
+    uint64_t want = ~0ull, whole;
     if (r.top_k) {
-        const Reach k = bin_that_reaches(count, (uint64_t)r.top_k, 1.0f, sh);
-        b1 = k.bin;
+        block_scan(count, &whole, sh);
+        reach(count, 0, (uint64_t)r.top_k < whole ? (uint64_t)r.top_k : whole, sh);
+        b1 = (int)sh.key;
         mode = ROW_TOP;
-        uint64_t all = 0;
-        for (int e = 0; e < PER; e++) all += PER * tid + e <= b1 ? count[e] : 0;
-        if (block_sum(all, sh) > LIST) {
+        if (block_sum(tid <= b1 ? count : 0, sh) > LIST) {
             b0 = b1;
             mode = sums ? ROW_COUNT : ROW_SLOW;
         }
     } else {
         if (r.top_p < 1.0f) {
-            const Reach p = bin_that_reaches(sum, 0, r.top_p, sh);
-            want = wanted(r.top_p, p.whole);
-            b0 = b1 = p.bin;
+            block_scan(sum, &whole, sh);
+            want = wanted(r.top_p, whole);
+            reach(sum, 0, want, sh);
+            b0 = b1 = (int)sh.key;
         }
         if (r.min_p > 0.0f) {
             // the bins that the border can be in: their arithmetic is in 32 bits
@@ -407,14 +572,8 @@ __global__ __launch_bounds__(THREADS) void k_sample_cut(Args A) {
             b1 = hi < b1 ? hi : b1;
         }
     }
-    uint64_t listed = 0, before = 0;
-    for (int e = 0; e < PER; e++) {
-        const int b = PER * tid + e;
-        listed += b >= b0 && b <= b1 ? count[e] : 0;
-        before += b < b0 ? (mode == ROW_COUNT ? count[e] : sum[e]) : 0;
-    }
-    listed = block_sum(listed, sh);
-    before = block_sum(before, sh);
+    const uint64_t listed = block_sum(tid >= b0 && tid <= b1 ? count : 0, sh);
+    const uint64_t before = block_sum(tid < b0 ? (mode == ROW_COUNT ? count : sum) : 0, sh);
     if (listed > LIST) mode = ROW_SLOW;
     if (tid == 0) {
         w.mode = mode;
@@ -424,26 +583,29 @@ __global__ __launch_bounds__(THREADS) void k_sample_cut(Args A) {
         w.before = before;
         w.want = want;
     }
-    // per piece, a wave each in turn: its listed tokens, then their offsets, and its sum before the listed bins
-    const int lane = tid & 63;
-    for (int p = tid >> 6; p < A.pieces; p += WAVES) {
-        const size_t at = ((size_t)row * A.pieces + p) * BINS;
-        uint64_t n = 0, s = 0;
-        for (int b = b0 + lane; b <= b1; b += 64) n += A.count[at + b];
-        if (sums)
-            for (int b = lane; b < b0; b += 64) s += A.sum[at + b];
-        n = wave_sum(n);
-        s = wave_sum(s);
-        if (lane == 0) {
-            listed_of[p] = (unsigned)n;
-            w.sums[p] = s;
-        }
+    // the piece's sum before the listed bins, and its listed tokens' number
+    uint64_t mine = 0, ahead = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        const int b = 64 * e + lane;
+        mine += b >= b0 && b <= b1 ? n[e] : 0;
+        ahead += b < b0 ? s[e] : 0;
+    }
+    mine = wave_sum(mine);
+    ahead = wave_sum(ahead);
+    if (lane == 0) {
+        listed_of[p] = (unsigned)mine;
+        w.sums[p] = ahead;
     }
     __syncthreads();
     if (tid < A.pieces) {
-        unsigned n = 0;
-        for (int p = 0; p < tid; p++) n += listed_of[p];
-        w.offset[tid] = n;
+        unsigned o = 0;
+        for (int q = 0; q < tid; q++) o += listed_of[q];
+        w.offset[tid] = o;
+    }
+    if (mode == ROW_COUNT) {  // the pick looks at the row's bins again: in the first piece's place
+        A.count[(size_t)row * A.pieces * BINS + tid] = (unsigned)count;
+        A.sum[(size_t)row * A.pieces * BINS + tid] = sum;
     }
 }
 
@@ -467,236 +629,134 @@ __global__ __launch_bounds__(THREADS) void k_sample_list(Args A) {
     });
 }
 
-// list[0 .. n) in falling order, all different. Up to 256: each one's rank counted, one round. Above: a bitonic sort of the
-// next power of two, padded with zeros.
-SDY_DEV void sort_falling(unsigned long long *list, int n) {
-    __syncthreads();
-    if (n <= THREADS) {
-        const unsigned long long mine = (int)threadIdx.x < n ? list[threadIdx.x] : 0;
-        int rank = 0;
-#pragma unroll 8
-        for (int i = 0; i < n; i++) rank += list[i] > mine;
-        __syncthreads();
-        if ((int)threadIdx.x < n) list[rank] = mine;
-        __syncthreads();
-        return;
-    }
-    int n2 = 2 * THREADS;
-    while (n2 < n) n2 *= 2;
-    for (int i = n + threadIdx.x; i < n2; i += THREADS) list[i] = 0;
-    __syncthreads();
-    for (int k = 2; k <= n2; k *= 2)
-        for (int j = k / 2; j > 0; j /= 2) {
-            for (int t = threadIdx.x; t < n2 / 2; t += THREADS) {
-                const int i = ((t & ~(j - 1)) << 1) | (t & (j - 1));
-                const unsigned long long x = list[i], y = list[i + j];
-                if ((x < y) == ((i & k) == 0)) list[i] = y, list[i + j] = x;
-            }
-            __syncthreads();
-        }
-}
-
-// The piece [lo, hi) narrowed to the token at which the running sum of kept(i) passes `left`
-template <class F>
-SDY_DEV int narrow(int lo, int hi, uint64_t left, const F &kept, Parts &sh) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    while (hi - lo > 1) {
-        const int len = (hi - lo + WAVES - 1) / WAVES;
-        const int b = lo + wave * len < hi ? lo + wave * len : hi, e = b + len < hi ? b + len : hi;
-        uint64_t sum = 0;
-        for (int i = b + lane; i < e; i += 64) sum += kept(i);
-        sum = wave_sum(sum);
-        __syncthreads();
-        if (lane == 0) sh.part[wave] = sum;
-        __syncthreads();
-        int w = 0;
-        while (w < WAVES - 1 && sh.part[w] <= left) left -= sh.part[w++];
-        lo = lo + w * len;
-        hi = lo + len < hi ? lo + len : hi;
-    }
-    return lo;
-}
-
-// u of the whole, in 0 .. whole - 1
-SDY_DEV uint64_t share(float u, uint64_t whole) {
-    if (!(u > 0.0f)) return 0;
-    if (u >= 1.0f) return whole - 1;
-    const uint64_t t = (uint64_t)((double)u * (double)whole);
-    return t < whole ? t : whole - 1;
-}
-
-struct Pick {
-    Shared sh;
-    unsigned long long list[LIST];
-    unsigned long long sums[MAX_PIECES];
-    int n_list;
-};
-
 __global__ __launch_bounds__(THREADS) void k_sample_pick(Args A) {
     extern __shared__ __align__(16) unsigned char lds_bytes[];
-    Pick &k = *reinterpret_cast<Pick *>(lds_bytes);
-    Shared &sh = k.sh;
-    unsigned long long *const list = k.list;
-    const sdy_sample_args &a = A.a;
+    Lds &k = *reinterpret_cast<Lds *>(lds_bytes);
     const int row = blockIdx.x, tid = threadIdx.x;
     const Work &w = A.work[row];
     int mode = w.mode, n = w.n_list;
     if (mode == ROW_TOP || mode == ROW_SUM || mode == ROW_COUNT)
-        for (int i = tid; i < n; i += THREADS) list[i] = w.list[i];
+        for (int i = tid; i < n; i += THREADS) k.list[i] = w.list[i];
     Row r;
     r.params(A, row);
     r.maxima(A, row);
     if (mode == ROW_ALONE) {
-        if (tid == 0) {
-            a.token[row] = r.none ? -1 : index_at(r.first);
-            if (a.prob) a.prob[row] = r.none ? 0.0f : 1.0f;
-        }
+        if (tid == 0) take_alone(A, row, r);
         return;
     }
-    const float u = a.u[row];
-    uint64_t least = 0;  // the place that the prefix ends at
-    auto kept_place = [&](uint64_t at) -> uint64_t {
-        if (at < least) return 0;
-        const double x = r.weight(value_at(at));
-        return at == r.first || !(x < (double)r.min_p) ? (uint64_t)(x * r.one) : 0;
-    };
-    auto kept = [&](int i) { return kept_place(place_of(r.x[i], i)); };
-    auto take = [&](int i, uint64_t v, uint64_t whole) {
-        a.token[row] = i;
-        if (a.prob) a.prob[row] = (float)((double)v / (double)whole);
-    };
-    if (mode == ROW_TOP || mode == ROW_SUM || mode == ROW_COUNT) sort_falling(list, n);
-    // thread t holds the sorted tokens t * per .. t * per + per - 1 of the first `limit`; sh.w[i] is the i-th one's w
-    auto weights = [&](int limit, int per) {
-        uint64_t s = 0;
-        for (int i = tid * per; i < limit && i < tid * per + per; i++) s += sh.w[i] = r.fixed(value_at(list[i]));
-        return s;
-    };
-    // the place that a prefix by sum ends at, `before` of it standing ahead of the list. want 0: top_p of the list
-    auto end_by_sum = [&](int limit, uint64_t before, uint64_t want) {
-        const int per = (limit + THREADS - 1) / THREADS;
-        __syncthreads();  // (sh.w shares its memory)
-        uint64_t whole;
-        uint64_t run = before + block_scan(weights(limit, per), &whole, sh);
-        if (want == 0) want = wanted(r.top_p, whole);
-        uint64_t last = ~0ull;
-        for (int i = tid * per; i < limit && i < tid * per + per && run < want; i++) {
-            last = list[i];
-            run += sh.w[i];
-        }
-        const uint64_t m = block_max(~last, sh);  // the least of them
-        return m ? ~m : 0ull;
-    };
     if (mode == ROW_TOP) {
-        if (n > r.top_k) n = r.top_k;
-        if (r.top_p < 1.0f) least = end_by_sum(n, 0, 0);
-        // the kept ones, a prefix of the list, by index: the place's halves change sides
-        uint64_t end = 0;
-        for (int i = tid; i < n; i += THREADS) {
-            const uint64_t at = list[i];
-            const bool in = at >= least && (at == r.first || !(r.weight(value_at(at)) < (double)r.min_p));
-            end += in;
-            list[i] = in ? (at & (MAX_VOCAB - 1)) << 32 | at >> 22 : 0;
-        }
-        n = (int)block_sum(end, sh);
-        sort_falling(list, n);
-        const int per = (n + THREADS - 1) / THREADS;
-        uint64_t sum = 0, whole;
-        for (int i = tid * per; i < n && i < tid * per + per; i++) sum += sh.w[i] = r.fixed(value_at((list[i] & 0xFFFFFFFFu) << 22));
-        uint64_t run = block_scan(sum, &whole, sh);
-        const uint64_t left = share(u, whole);
-        if (run <= left && left < run + sum) {
-            int i = tid * per;
-            while (run + sh.w[i] <= left) run += sh.w[i++];
-            take(MAX_VOCAB - 1 - (int)(list[i] >> 32), sh.w[i], whole);
-        }
+        __syncthreads();
+        pick_listed(A, row, r, n, k);
         return;
     }
+    const float u = A.a.u[row];
+    uint64_t least = 0;  // the place that the prefix ends at
+    auto kept = [&](int i) -> uint64_t {
+        const uint64_t at = place_of(r.x[i], i);
+        return at < least ? 0 : r.fixed_kept(at);
+    };
+    auto place = [&](int i) -> uint64_t { return k.list[i]; };
+    auto w_of = [&](int i) -> uint64_t { return k.w[i]; };
     if (mode == ROW_SUM || mode == ROW_ALL) {
         if (tid < A.pieces) k.sums[tid] = w.sums[tid];
-        __syncthreads();
         if (mode == ROW_SUM) {
-            if (r.top_p < 1.0f) least = end_by_sum(n, w.before, w.want);
-            if (least == 0 && n) least = list[n - 1];
-            for (int i = tid; i < n; i += THREADS) {
-                const uint64_t v = kept_place(list[i]);
-                if (v) atomicAdd(&k.sums[index_at(list[i]) / A.len], (unsigned long long)v);
-            }
+            uint64_t sum = 0, last = ~0ull;
             __syncthreads();
+            for (int i = tid; i < n; i += THREADS) {
+                sum += k.w[i] = r.fixed(value_at(k.list[i]));
+                last = k.list[i] < last ? k.list[i] : last;
+            }
+            sum = block_sum(sum, k.parts);
+            if (r.top_p < 1.0f && w.before + sum >= w.want) least = find(n, place, w_of, w.before, w.want, k).key;
+            else if (n) least = ~block_max(~last, k.parts);
+            for (int i = tid; i < n; i += THREADS) {
+                const uint64_t v = k.list[i] < least ? 0 : r.min_p > 0.0f ? r.fixed_kept(k.list[i]) : k.w[i];
+                if (v) atomicAdd(&k.sums[index_at(k.list[i]) / A.len], (unsigned long long)v);
+            }
         }
+        __syncthreads();
         uint64_t whole = 0;
         for (int p = 0; p < A.pieces; p++) whole += k.sums[p];
         uint64_t left = share(u, whole);
         int p = 0;
         while (p < A.pieces - 1 && k.sums[p] <= left) left -= k.sums[p++];
-        const int lo = p * A.len, i = narrow(lo, lo + A.len < r.n ? lo + A.len : r.n, left, kept, sh);
-        if (tid == 0) take(i, kept(i), whole);
+        const int lo = p * A.len, i = narrow(lo, lo + A.len < r.n ? lo + A.len : r.n, left, kept, k);
+        if (tid == 0) take(A, row, i, kept(i), whole);
         return;
     }
     if (mode == ROW_COUNT) {  // many tokens by count: the end of the first top_k is known now, and with it their sum
-        const int rest = r.top_k - (int)w.before, end = rest < n ? rest : n;  // of the list
-        least = list[end - 1];
+        __syncthreads();
+        for (int i = tid; i < n; i += THREADS) k.w[i] = r.fixed(value_at(k.list[i]));
+        const uint64_t rest = (uint64_t)r.top_k - w.before;
+        if (rest < (uint64_t)n) least = find(n, place, [](int) -> uint64_t { return 1; }, 0, rest, k).key;
+        else if (n) {
+            uint64_t last = ~0ull;
+            for (int i = tid; i < n; i += THREADS) last = k.list[i] < last ? k.list[i] : last;
+            least = ~block_max(~last, k.parts);
+        }
         if (r.top_p < 1.0f) {
-            uint64_t count[PER], sum[PER], ahead = 0, in_list = 0;
-            bins_of(A, row, true, count, sum);
-            for (int e = 0; e < PER; e++) {
-                if (PER * tid + e >= w.b0) sum[e] = 0;
-                ahead += sum[e];
-            }
-            ahead = block_sum(ahead, sh);
-            in_list = block_sum(weights(end, (end + THREADS - 1) / THREADS), sh);
-            const uint64_t want = wanted(r.top_p, ahead + in_list);
+            const size_t at = (size_t)row * A.pieces * BINS;
+            uint64_t sum = 0, ahead = 0;
+            __syncthreads();
+            for (int i = tid; i < n; i += THREADS) sum += k.list[i] < least ? (k.w[i] = 0) : k.w[i];
+            sum = block_sum(sum, k.parts);
+            for (int b = tid; b < w.b0; b += THREADS) ahead += A.sum[at + b];
+            ahead = block_sum(ahead, k.parts);
+            const uint64_t want = wanted(r.top_p, ahead + sum);
             if (ahead < want) {
-                least = end_by_sum(end, ahead, want);
+                least = find(n, place, w_of, ahead, want, k).key;
             } else {  // the sum ends in an earlier bin, whose tokens nobody has listed
-                const Reach b = bin_that_reaches(sum, want, 1.0f, sh);
-                uint64_t c = 0;
-                for (int e = 0; e < PER; e++) c += PER * tid + e == b.bin ? count[e] : 0;
-                c = block_sum(c, sh);
-                if (c > LIST) {
+                const Found b = find(w.b0, [](int i) -> uint64_t { return (uint64_t)(BINS - i); }, [&](int i) -> uint64_t { return A.sum[at + i]; }, 0, want, k);
+                const int bin = BINS - (int)b.key;
+                n = (int)A.count[at + bin];
+                if (n > LIST) {
                     mode = ROW_SLOW;
                 } else {
-                    if (tid == 0) k.n_list = 0;
+                    if (tid == 0) k.n = 0;
                     __syncthreads();
                     each(r.x, 0, r.n, [&](float x, int i) {
-                        if (x > -INFINITY && r.bin(x) == b.bin) list[atomicAdd(&k.n_list, 1)] = place_of(x, i);
+                        if (x > -INFINITY && r.bin(x) == bin) {
+                            const int to = atomicAdd(&k.n, 1);
+                            k.list[to] = place_of(x, i);
+                            k.w[to] = r.fixed(x);
+                        }
                     });
-                    sort_falling(list, (int)c);
-                    least = end_by_sum((int)c, b.before, want);
+                    __syncthreads();
+                    least = find(n, place, w_of, b.run, want, k).key;
                 }
             }
         }
     }
     if (mode == ROW_SLOW) {
         least = 0;
-        if (r.top_k) least = prefix_end(r, 0, false, (uint64_t)r.top_k, sh);
+        if (r.top_k) least = prefix_end(r, 0, false, (uint64_t)r.top_k, k);
         if (r.top_p < 1.0f) {
             uint64_t sum = 0;
-            for (int i = tid; i < r.n; i += THREADS)
-                if (place_of(r.x[i], i) >= least) sum += r.fixed(r.x[i]);
-            sum = block_sum(sum, sh);
-            least = prefix_end(r, least, true, wanted(r.top_p, sum), sh);
+            each(r.x, 0, r.n, [&](float v, int i) {
+                if (place_of(v, i) >= least) sum += r.fixed(v);
+            });
+            sum = block_sum(sum, k.parts);
+            least = prefix_end(r, least, true, wanted(r.top_p, sum), k);
         }
     }
     uint64_t whole = 0;
     for (int i = tid; i < r.n; i += THREADS) whole += kept(i);
-    whole = block_sum(whole, sh);
-    const int i = narrow(0, r.n, share(u, whole), kept, sh);
-    if (tid == 0) take(i, kept(i), whole);
+    whole = block_sum(whole, k.parts);
+    const int i = narrow(0, r.n, share(u, whole), kept, k);
+    if (tid == 0) take(A, row, i, kept(i), whole);
 }
 
-// Pieces per row: enough workgroups for the GPU where there are few rows, none shorter than 4096 tokens.
-int pieces_of(int n_rows, int n_vocab) {
-    int p = (n_vocab + 4095) / 4096;
-    (void)n_rows;
+int pieces_of(int n_vocab) {
+    const int p = (n_vocab + LIST - 1) / LIST;
     return p < MAX_PIECES ? p : MAX_PIECES;
 }
 
 }  // namespace
 
 extern "C" size_t sdy_sample_ws_bytes(int n_rows, int n_vocab) {
-    if (n_rows < 1 || n_vocab < 1 || n_vocab > MAX_VOCAB) return 0;
-    return (size_t)n_rows * (sizeof(Work) + (size_t)pieces_of(n_rows, n_vocab) * BINS * 12);
+    if (n_rows < 1 || n_rows > 65535 || n_vocab < 1 || n_vocab > MAX_VOCAB) return 0;
+    if (n_vocab <= LIST) return 16;
+    return (size_t)n_rows * (sizeof(Work) + (size_t)pieces_of(n_vocab) * BINS * 12);
 }
 
 extern "C" int sdy_sample(const sdy_sample_args *a, sdy_stream s) {
@@ -713,20 +773,25 @@ extern "C" int sdy_sample(const sdy_sample_args *a, sdy_stream s) {
     int log2 = 0;
     while ((1 << log2) < a->n_vocab) log2++;
     A.shift = 62 - log2;
-    A.pieces = pieces_of(a->n_rows, a->n_vocab);
+    A.pieces = pieces_of(a->n_vocab);
     A.len = ((a->n_vocab + A.pieces - 1) / A.pieces + 3) & ~3;
     A.work = (Work *)a->ws;
     A.sum = (unsigned long long *)(A.work + a->n_rows);
     A.count = (unsigned *)(A.sum + (size_t)a->n_rows * A.pieces * BINS);
-    static size_t granted = 0;
-    const int rc = sdy_lds_limit((const void *)k_sample_pick, sizeof(Pick), &granted);
+    static size_t granted[2];
+    const bool small = a->n_vocab <= LIST;
+    const int rc = sdy_lds_limit(small ? (const void *)k_sample_small : (const void *)k_sample_pick, sizeof(Lds), &granted[small]);
     if (rc) return rc;
-    const dim3 grid(A.pieces, a->n_rows), block(THREADS);
+    const dim3 rows(a->n_rows), grid(A.pieces, a->n_rows), block(THREADS);
     hipStream_t st = (hipStream_t)s;
-    hipLaunchKernelGGL(k_sample_max, grid, block, 0, st, A);
-    hipLaunchKernelGGL(k_sample_bins, grid, block, 0, st, A);
-    hipLaunchKernelGGL(k_sample_cut, dim3(a->n_rows), block, 0, st, A);
-    hipLaunchKernelGGL(k_sample_list, grid, block, 0, st, A);
-    hipLaunchKernelGGL(k_sample_pick, dim3(a->n_rows), block, sizeof(Pick), st, A);
+    if (small) {
+        hipLaunchKernelGGL(k_sample_small, rows, block, sizeof(Lds), st, A);
+    } else {
+        hipLaunchKernelGGL(k_sample_max, grid, block, 0, st, A);
+        hipLaunchKernelGGL(k_sample_bins, grid, block, 0, st, A);
+        hipLaunchKernelGGL(k_sample_cut, rows, dim3(BINS), 0, st, A);
+        hipLaunchKernelGGL(k_sample_list, grid, block, 0, st, A);
+        hipLaunchKernelGGL(k_sample_pick, rows, block, sizeof(Lds), st, A);
+    }
     return sdy_check_launch("sample");
 }
