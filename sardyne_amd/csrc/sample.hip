@@ -30,6 +30,7 @@ constexpr int BINS = 1024;
 constexpr int LIST = 4096;          // tokens that one workgroup holds
 constexpr int SMALL_K = 1024;       // up to here the bins' sums are not made: the first top_k tokens are listed themselves
 constexpr int MAX_PIECES = 16;
+constexpr int FEW_ROWS = 16;        // up to here 1024 threads to a piece
 
 // A logit's place in the order: 32 bits that grow with x (-0 as 0, NaN as -inf), then 22 that fall with the index.
 SDY_DEV float value_at(uint64_t place) {
@@ -140,18 +141,18 @@ struct Row {
 };
 
 // f(logit, index) of the tokens [lo, hi) (lo a multiple of 4), four 16-byte loads in flight where the row allows them
-template <class F>
+template <int T = THREADS, class F>
 SDY_DEV void each(const float *x, int lo, int hi, const F &f) {
     int i = lo;
     if (((uintptr_t)x & 15) == 0) {
         const int end = lo + (hi - lo) / 4 * 4;
-        for (int i0 = lo + 4 * (int)threadIdx.x; i0 < end; i0 += 16 * THREADS) {
+        for (int i0 = lo + 4 * (int)threadIdx.x; i0 < end; i0 += 16 * T) {
             float4 v[4];
 #pragma unroll
-            for (int u = 0; u < 4; u++) v[u] = *reinterpret_cast<const float4 *>(x + (i0 + 4 * u * THREADS < end ? i0 + 4 * u * THREADS : lo));
+            for (int u = 0; u < 4; u++) v[u] = *reinterpret_cast<const float4 *>(x + (i0 + 4 * u * T < end ? i0 + 4 * u * T : lo));
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                const int j = i0 + 4 * u * THREADS;
+                const int j = i0 + 4 * u * T;
                 if (j >= end) continue;
                 f(v[u].x, j);
                 f(v[u].y, j + 1);
@@ -161,13 +162,13 @@ SDY_DEV void each(const float *x, int lo, int hi, const F &f) {
         }
         i = end;
     }
-    for (int i0 = i + (int)threadIdx.x; i0 < hi; i0 += 8 * THREADS) {
+    for (int i0 = i + (int)threadIdx.x; i0 < hi; i0 += 8 * T) {
         float v[8];
 #pragma unroll
-        for (int u = 0; u < 8; u++) v[u] = x[i0 + u * THREADS < hi ? i0 + u * THREADS : hi - 1];
+        for (int u = 0; u < 8; u++) v[u] = x[i0 + u * T < hi ? i0 + u * T : hi - 1];
 #pragma unroll
         for (int u = 0; u < 8; u++)
-            if (i0 + u * THREADS < hi) f(v[u], i0 + u * THREADS);
+            if (i0 + u * T < hi) f(v[u], i0 + u * T);
     }
 }
 
@@ -180,10 +181,30 @@ struct Parts {
     unsigned long long key, val, run;  // what one thread found
 };
 
-SDY_DEV uint64_t wave_sum(uint64_t v) {
-    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor((unsigned long long)v, off);
+// v of the lane that DPP control CTRL names, 0 where there is none (or the row is masked off)
+template <int CTRL, int ROWS>
+SDY_DEV uint64_t dpp_u64(uint64_t v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);
+    return (uint64_t)hi << 32 | lo;
+}
+
+// Over the wave's lanes up to this one: within rows of 16 lanes by shifts of 1, 2, 4, 8, then the rows' ends passed on.
+template <bool MAX>
+SDY_DEV uint64_t wave_run(uint64_t v) {
+    auto add = [&](uint64_t o) { v = MAX ? (o > v ? o : v) : v + o; };
+    add(dpp_u64<0x111, 0xF>(v));
+    add(dpp_u64<0x112, 0xF>(v));
+    add(dpp_u64<0x114, 0xF>(v));
+    add(dpp_u64<0x118, 0xF>(v));
+    add(dpp_u64<0x142, 0xA>(v));  // row_bcast 15 to rows 1 and 3
+    add(dpp_u64<0x143, 0xC>(v));  // row_bcast 31 to rows 2 and 3
     return v;
 }
+SDY_DEV uint64_t last_lane(uint64_t v) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63);
+}
+SDY_DEV uint64_t wave_sum(uint64_t v) { return last_lane(wave_run<false>(v)); }
 
 template <int W>
 SDY_DEV uint64_t block_sum(uint64_t v, Parts<W> &sh) {
@@ -192,20 +213,19 @@ SDY_DEV uint64_t block_sum(uint64_t v, Parts<W> &sh) {
     if ((threadIdx.x & 63) == 0) sh.part[threadIdx.x >> 6] = v;
     __syncthreads();
     uint64_t r = 0;
+#pragma unroll
     for (int w = 0; w < W; w++) r += sh.part[w];
     return r;
 }
 
 template <int W>
 SDY_DEV uint64_t block_max(uint64_t v, Parts<W> &sh) {
-    for (int off = 32; off >= 1; off >>= 1) {
-        const uint64_t o = __shfl_xor((unsigned long long)v, off);
-        v = o > v ? o : v;
-    }
+    v = last_lane(wave_run<true>(v));
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh.part[threadIdx.x >> 6] = v;
     __syncthreads();
     uint64_t r = 0;
+#pragma unroll
     for (int w = 0; w < W; w++) r = sh.part[w] > r ? sh.part[w] : r;
     return r;
 }
@@ -213,15 +233,12 @@ SDY_DEV uint64_t block_max(uint64_t v, Parts<W> &sh) {
 // The sum over the threads before this one; *whole the sum over all.
 template <int W>
 SDY_DEV uint64_t block_scan(uint64_t v, uint64_t *whole, Parts<W> &sh) {
-    uint64_t run = v;
-    for (int off = 1; off < 64; off *= 2) {
-        const uint64_t o = __shfl_up((unsigned long long)run, off);
-        if ((int)(threadIdx.x & 63) >= off) run += o;
-    }
+    const uint64_t run = wave_run<false>(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 63) sh.part[threadIdx.x >> 6] = run;
     __syncthreads();
     uint64_t before = 0, all = 0;
+#pragma unroll
     for (int w = 0; w < W; w++) {
         if (w < (int)(threadIdx.x >> 6)) before += sh.part[w];
         all += sh.part[w];
@@ -281,16 +298,17 @@ struct Found {
 template <class K, class V>
 SDY_DEV Found find(int n, const K &key, const V &val, uint64_t before, uint64_t want, Lds &k) {
     const int tid = threadIdx.x;
-    uint64_t hi = 0, lo = ~0ull;
-    for (int i = tid; i < n; i += THREADS)
-        if (val(i)) {
-            const uint64_t x = key(i);
-            hi = x > hi ? x : hi;
-            lo = x < lo ? x : lo;
-        }
-    hi = block_max(hi, k.parts);
-    lo = ~block_max(~lo, k.parts);
-    if (n > 64)
+    uint64_t hi = ~0ull, lo = 0;
+    if (n > 64) {
+        uint64_t most = 0, least = 0;
+        for (int i = tid; i < n; i += THREADS)
+            if (val(i)) {
+                const uint64_t x = key(i);
+                most = x > most ? x : most;
+                least = ~x > least ? ~x : least;
+            }
+        hi = block_max(most, k.parts);
+        lo = ~block_max(least, k.parts);
         for (;;) {
             const int bits = 64 - __builtin_clzll((hi - lo) | 1), shift = bits > 8 ? bits - 8 : 0;
             k.sub_sum[tid] = 0;
@@ -313,6 +331,7 @@ SDY_DEV Found find(int n, const K &key, const V &val, uint64_t before, uint64_t 
             __syncthreads();
             if (c <= 64 || shift == 0) break;
         }
+    }
     if (tid == 0) k.n = 0;
     __syncthreads();
     for (int i = tid; i < n; i += THREADS) {
@@ -350,6 +369,7 @@ SDY_DEV void take_alone(const Args &A, int row, const Row &r) {
 // The token of a row whose kept ones are all among the n in the list.
 SDY_DEV void pick_listed(const Args &A, int row, const Row &r, int n, Lds &k) {
     const int tid = threadIdx.x;
+    const float u = A.a.u[row];
     for (int i = tid; i < n; i += THREADS) k.w[i] = r.fixed(value_at(k.list[i]));
     __syncthreads();
     uint64_t least = 0, sum = 0;
@@ -370,7 +390,7 @@ SDY_DEV void pick_listed(const Args &A, int row, const Row &r, int n, Lds &k) {
     sum = block_sum(sum, k.parts);
     // by index now
     const Found f = find(n, [&](int i) -> uint64_t { return k.list[i] & (MAX_VOCAB - 1); }, [&](int i) -> uint64_t { return k.w[i]; }, 0,
-                         share(A.a.u[row], sum) + 1, k);
+                         share(u, sum) + 1, k);
     if (tid == 0) take(A, row, MAX_VOCAB - 1 - (int)f.key, f.val, sum);
 }
 
@@ -454,14 +474,15 @@ __global__ __launch_bounds__(THREADS) void k_sample_small(Args A) {
     pick_listed(A, row, r, r.n, k);
 }
 
-__global__ __launch_bounds__(THREADS) void k_sample_max(Args A) {
-    __shared__ Parts<WAVES> sh;
+template <int W>
+__global__ __launch_bounds__(64 * W) void k_sample_max(Args A) {
+    __shared__ Parts<W> sh;
     const int c = blockIdx.x, row = blockIdx.y;
     const float *x = A.a.logits + (size_t)row * A.a.stride;
     const int lo = c * A.len, hi = lo + A.len < A.a.n_vocab ? lo + A.len : A.a.n_vocab;
     uint64_t first = 0;
     float low = INFINITY;
-    each(x, lo, hi, [&](float v, int i) {
+    each<64 * W>(x, lo, hi, [&](float v, int i) {
         const uint64_t at = place_of(v, i);
         first = at > first ? at : first;
         if (v > -INFINITY) low = fminf(low, v);
@@ -470,14 +491,15 @@ __global__ __launch_bounds__(THREADS) void k_sample_max(Args A) {
     if ((threadIdx.x & 63) == 0) sh.low[threadIdx.x >> 6] = low;
     first = block_max(first, sh);
     if (threadIdx.x == 0) {
-        for (int w = 0; w < WAVES; w++) low = fminf(low, sh.low[w]);
+        for (int w = 0; w < W; w++) low = fminf(low, sh.low[w]);
         A.work[row].first[c] = first;
         A.work[row].low[c] = low;
     }
 }
 
-__global__ __launch_bounds__(THREADS) void k_sample_bins(Args A) {
-    __shared__ Parts<WAVES> sh;
+template <int W>
+__global__ __launch_bounds__(64 * W) void k_sample_bins(Args A) {
+    __shared__ Parts<W> sh;
     __shared__ unsigned count[BINS];
     __shared__ unsigned long long sum_of[BINS];
     const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
@@ -488,15 +510,15 @@ __global__ __launch_bounds__(THREADS) void k_sample_bins(Args A) {
     const int lo = c * A.len, hi = lo + A.len < r.n ? lo + A.len : r.n;
     if (!r.cut()) {
         uint64_t sum = 0;
-        each(r.x, lo, hi, [&](float v, int) { sum += r.fixed(v); });
+        each<64 * W>(r.x, lo, hi, [&](float v, int) { sum += r.fixed(v); });
         sum = block_sum(sum, sh);
         if (tid == 0) A.work[row].sums[c] = sum;
         return;
     }
     const bool sums = r.sums();
-    for (int b = tid; b < BINS; b += THREADS) count[b] = 0, sum_of[b] = 0;
+    for (int b = tid; b < BINS; b += 64 * W) count[b] = 0, sum_of[b] = 0;
     __syncthreads();
-    each(r.x, lo, hi, [&](float v, int) {
+    each<64 * W>(r.x, lo, hi, [&](float v, int) {
         if (!(v > -INFINITY)) return;
         const int b = r.bin(v);
         atomicAdd(&count[b], 1u);
@@ -504,7 +526,7 @@ __global__ __launch_bounds__(THREADS) void k_sample_bins(Args A) {
     });
     __syncthreads();
     const size_t at = ((size_t)row * A.pieces + c) * BINS;
-    for (int b = tid; b < BINS; b += THREADS) {
+    for (int b = tid; b < BINS; b += 64 * W) {
         A.count[at + b] = count[b];
         if (sums) A.sum[at + b] = sum_of[b];
     }
@@ -515,8 +537,8 @@ __global__ __launch_bounds__(BINS) void k_sample_cut(Args A) {
     constexpr int W = BINS / 64, EACH = BINS / 64;
     static_assert(W == MAX_PIECES, "a wave per piece");
     __shared__ Parts<W> sh;
-    __shared__ unsigned count_of[BINS], listed_of[MAX_PIECES];
-    __shared__ unsigned long long sum_of[BINS];
+    __shared__ unsigned count_of[BINS], before_n[BINS + 1], listed_of[MAX_PIECES];
+    __shared__ unsigned long long sum_of[BINS], before_s[BINS], part_s[W];
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, p = tid >> 6;
     Work &w = A.work[row];
     Row r;
@@ -544,25 +566,34 @@ __global__ __launch_bounds__(BINS) void k_sample_cut(Args A) {
         if (s[e]) atomicAdd(&sum_of[64 * e + lane], s[e]);
     }
     __syncthreads();
+    // the bins' running counts and sums
     const uint64_t count = count_of[tid], sum = sum_of[tid];
+    const uint64_t run_n = wave_run<false>(count), run_s = wave_run<false>(sum);
+    if (lane == 63) sh.part[p] = run_n, part_s[p] = run_s;
+    __syncthreads();
+    uint64_t n0 = run_n - count, s0 = run_s - sum, all_n = 0, all_s = 0;
+#pragma unroll
+    for (int q = 0; q < W; q++) {
+        if (q < p) n0 += sh.part[q], s0 += part_s[q];
+        all_n += sh.part[q];
+        all_s += part_s[q];
+    }
+    const uint64_t want = r.top_k ? ((uint64_t)r.top_k < all_n ? (uint64_t)r.top_k : all_n) : r.top_p < 1.0f ? wanted(r.top_p, all_s) : ~0ull;
+    before_n[tid] = (unsigned)n0;
+    before_s[tid] = s0;
+    if (r.top_k ? n0 < want && n0 + count >= want : s0 < want && s0 + sum >= want) sh.key = tid;
+    if (tid == 0) before_n[BINS] = (unsigned)all_n;
+    __syncthreads();
     int b0 = 0, b1 = BINS - 1, mode = ROW_SUM;
-    uint64_t want = ~0ull, whole;
     if (r.top_k) {
-        block_scan(count, &whole, sh);
-        reach(count, 0, (uint64_t)r.top_k < whole ? (uint64_t)r.top_k : whole, sh);
         b1 = (int)sh.key;
         mode = ROW_TOP;
-        if (block_sum(tid <= b1 ? count : 0, sh) > LIST) {
+        if (before_n[b1 + 1] > LIST) {
             b0 = b1;
             mode = sums ? ROW_COUNT : ROW_SLOW;
         }
     } else {
-        if (r.top_p < 1.0f) {
-            block_scan(sum, &whole, sh);
-            want = wanted(r.top_p, whole);
-            reach(sum, 0, want, sh);
-            b0 = b1 = (int)sh.key;
-        }
+        if (r.top_p < 1.0f) b0 = b1 = (int)sh.key;
         if (r.min_p > 0.0f) {
             // the bins that the border can be in: their arithmetic is in 32 bits
             const float far = r.min_p < 1.0f ? -logf(r.min_p) * r.temp * r.per_bin : 0.0f;
@@ -572,15 +603,14 @@ __global__ __launch_bounds__(BINS) void k_sample_cut(Args A) {
             b1 = hi < b1 ? hi : b1;
         }
     }
-    const uint64_t listed = block_sum(tid >= b0 && tid <= b1 ? count : 0, sh);
-    const uint64_t before = block_sum(tid < b0 ? (mode == ROW_COUNT ? count : sum) : 0, sh);
+    const int listed = (int)(before_n[b1 + 1] - before_n[b0]);
     if (listed > LIST) mode = ROW_SLOW;
     if (tid == 0) {
         w.mode = mode;
-        w.n_list = (int)listed;
+        w.n_list = listed;
         w.b0 = b0;
         w.b1 = b1;
-        w.before = before;
+        w.before = mode == ROW_COUNT ? before_n[b0] : before_s[b0];
         w.want = want;
     }
     // the piece's sum before the listed bins, and its listed tokens' number
@@ -609,7 +639,8 @@ __global__ __launch_bounds__(BINS) void k_sample_cut(Args A) {
     }
 }
 
-__global__ __launch_bounds__(THREADS) void k_sample_list(Args A) {
+template <int W>
+__global__ __launch_bounds__(64 * W) void k_sample_list(Args A) {
     __shared__ unsigned next;
     const int c = blockIdx.x, row = blockIdx.y;
     Work &w = A.work[row];
@@ -622,7 +653,7 @@ __global__ __launch_bounds__(THREADS) void k_sample_list(Args A) {
     if (threadIdx.x == 0) next = w.offset[c];
     __syncthreads();
     const int lo = c * A.len, hi = lo + A.len < r.n ? lo + A.len : r.n;
-    each(r.x, lo, hi, [&](float v, int i) {
+    each<64 * W>(r.x, lo, hi, [&](float v, int i) {
         if (!(v > -INFINITY)) return;
         const int b = r.bin(v);
         if (b >= b0 && b <= b1) w.list[atomicAdd(&next, 1u)] = place_of(v, i);
@@ -787,10 +818,18 @@ extern "C" int sdy_sample(const sdy_sample_args *a, sdy_stream s) {
     if (small) {
         hipLaunchKernelGGL(k_sample_small, rows, block, sizeof(Lds), st, A);
     } else {
-        hipLaunchKernelGGL(k_sample_max, grid, block, 0, st, A);
-        hipLaunchKernelGGL(k_sample_bins, grid, block, 0, st, A);
+        const bool few = a->n_rows <= FEW_ROWS;
+        const dim3 wide(1024);
+        if (few) {
+            hipLaunchKernelGGL(k_sample_max<16>, grid, wide, 0, st, A);
+            hipLaunchKernelGGL(k_sample_bins<16>, grid, wide, 0, st, A);
+        } else {
+            hipLaunchKernelGGL(k_sample_max<4>, grid, block, 0, st, A);
+            hipLaunchKernelGGL(k_sample_bins<4>, grid, block, 0, st, A);
+        }
         hipLaunchKernelGGL(k_sample_cut, rows, dim3(BINS), 0, st, A);
-        hipLaunchKernelGGL(k_sample_list, grid, block, 0, st, A);
+        if (few) hipLaunchKernelGGL(k_sample_list<16>, grid, wide, 0, st, A);
+        else hipLaunchKernelGGL(k_sample_list<4>, grid, block, 0, st, A);
         hipLaunchKernelGGL(k_sample_pick, rows, block, sizeof(Lds), st, A);
     }
     return sdy_check_launch("sample");

@@ -541,7 +541,7 @@ def test_a_step_answers_as_one_token_at_a_time():
         bp, bpar, bpast = up((past + depth).astype(np.int32)), up(np.array(parent, np.int32)), up(np.array([past], np.int32))
         slots = up(np.arange(n, dtype=np.int32))
         for l in range(n_layer):
-            bx, bq, bo = up(x @ w[l]), capi.DeviceBuffer(n * dim * 4), capi.DeviceBuffer(n * dim * 4)
+            bx, bq, bo = up(x @ w[l]), capi.DeviceBuffer(n * dim * 4), up(np.zeros((n, dim), np.float32))
             a = capi.SdyRopeAtArgs(q=bx.ptr, k=bx.ptr + 4 * dim, v=bx.ptr + 4 * (dim + nkv * hd), q_stride=width,
                                    k_stride=width, v_stride=width, q_out=bq.ptr, q_out_stride=dim,
                                    k_rows=layer(draft[0], l, n_max), v_rows=layer(draft[1], l, n_max),
