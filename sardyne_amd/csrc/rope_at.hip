@@ -42,26 +42,110 @@ SDY_DEV void sincos_f64(double x, double *sn, double *cs) {
     *cs = (quad + 1) & 2 ? -b : b;
 }
 
-// One workgroup per token and head-group: one wave per head of q, k or v, the head in LDS.
+// The token's slot, or -1 where this workgroup is to write no rows: of two tokens with one slot the later one's row stays.
+// All 256 threads.
+SDY_DEV long slot_of(const sdy_rope_at_args &a, int t) {
+    const long slot = a.slot ? a.slot[t] : a.pos[t];
+    int keep = a.k && slot >= 0 && slot < a.n_slot;
+    if (keep)
+        for (int u = t + 1 + (int)threadIdx.x; u < a.n_tok; u += 256) keep &= (a.slot ? a.slot[u] : a.pos[u]) != slot;
+    return __syncthreads_and(keep) ? slot : -1;
+}
+
+// Heads of 32, 64, 128 or 256 dims in aligned rows: HD / 4 lanes to a row of q, k or v, four dims each. A workgroup takes
+// `rows` rows of one token, 256 / (HD / 4) at a time.
+template <int HD, class KT>
+__global__ __launch_bounds__(256) void k_rope_rows(sdy_rope_at_args a, int rows) {
+    constexpr int L = HD / 4, RPP = 256 / L;
+    __shared__ __align__(16) float cs[HD / 2], sn[HD / 2];
+    const int t = blockIdx.x, tid = threadIdx.x, c = tid % L, d = 4 * c;
+    const int half = a.n_rot / 2;
+    const int n_q = a.q ? a.n_head : 0, n_k = a.k ? a.n_kv_head : 0, all = n_q + 2 * n_k;
+    const int r0 = blockIdx.y * rows + tid / L, end = (int)(blockIdx.y + 1) * rows < all ? (int)(blockIdx.y + 1) * rows : all;
+    auto load = [&](int r) {
+        if (r >= end) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const float *src = r < n_q         ? a.q + (size_t)t * a.q_stride + (size_t)r * HD
+                           : r < n_q + n_k ? a.k + (size_t)t * a.k_stride + (size_t)(r - n_q) * HD
+                                           : a.v + (size_t)t * a.v_stride + (size_t)(r - n_q - n_k) * HD;
+        return *reinterpret_cast<const float4 *>(src + d);
+    };
+    float4 x = load(r0);
+    const int pos = a.pos[t];
+    if (tid < half) {
+        double s, c2;
+        sincos_f64((double)pos * a.freq[tid], &s, &c2);
+        cs[tid] = (float)((double)a.mscale * c2);
+        sn[tid] = (float)((double)a.mscale * s);
+    }
+    long slot = -1;
+    if (end > n_q) slot = slot_of(a, t);
+    else __syncthreads();
+    for (int r = r0; r - tid / L < end; r += RPP) {
+        const float4 next = load(r + RPP);
+        const bool is_q = r < n_q, is_v = r >= n_q + n_k;
+        const float *nw = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
+        if (a.q_norm || a.k_norm) {
+            double ss = ((double)x.x * (double)x.x + (double)x.y * (double)x.y) + ((double)x.z * (double)x.z + (double)x.w * (double)x.w);
+#pragma unroll
+            for (int off = L / 2; off >= 1; off /= 2) ss += __shfl_xor(ss, off);
+            if (nw) {
+                const float sc = (float)(1.0 / sqrt(ss / (double)HD + (double)a.eps));
+                const float4 w = *reinterpret_cast<const float4 *>(nw + d);
+                x = make_float4(x.x * sc * w.x, x.y * sc * w.y, x.z * sc * w.z, x.w * sc * w.w);
+            }
+        }
+        float4 y = x;
+        if (a.interleaved) {
+            if (d < a.n_rot && !is_v) {
+                const float2 co = *reinterpret_cast<const float2 *>(cs + d / 2), si = *reinterpret_cast<const float2 *>(sn + d / 2);
+                const float ac = x.x * co.x, bs = x.y * si.x, as = x.x * si.x, bc = x.y * co.x;
+                const float ec = x.z * co.y, fs = x.w * si.y, es = x.z * si.y, fc = x.w * co.y;
+                y = make_float4(ac - bs, as + bc, ec - fs, es + fc);
+            }
+        } else {
+            const bool low = d < half;
+            const int from = (tid & 63 & ~(L - 1)) + (low ? c + half / 4 : d < a.n_rot ? c - half / 4 : c);
+            const float4 o = make_float4(__shfl(x.x, from), __shfl(x.y, from), __shfl(x.z, from), __shfl(x.w, from));
+            if (d < a.n_rot && !is_v) {
+                const int i = low ? d : d - half;
+                const float4 co = *reinterpret_cast<const float4 *>(cs + i), si = *reinterpret_cast<const float4 *>(sn + i);
+                const float4 xc = make_float4(x.x * co.x, x.y * co.y, x.z * co.z, x.w * co.w);
+                const float4 os = make_float4(o.x * si.x, o.y * si.y, o.z * si.z, o.w * si.w);
+                // a c - b s for the first of a pair, a s + b c for the second
+                y = low ? make_float4(xc.x - os.x, xc.y - os.y, xc.z - os.z, xc.w - os.w)
+                        : make_float4(os.x + xc.x, os.y + xc.y, os.z + xc.z, os.w + xc.w);
+            }
+        }
+        if (r < end) {
+            if (is_q) {
+                *reinterpret_cast<float4 *>(a.q_out + (size_t)t * a.q_out_stride + (size_t)r * HD + d) = y;
+            } else if (slot >= 0) {
+                KT *dst = (KT *)(is_v ? a.v_rows : a.k_rows) + (size_t)(r - n_q - (is_v ? n_k : 0)) * a.head_stride + (size_t)slot * HD + d;
+                if constexpr (KvElt<KT>::BYTES == 4)
+                    *reinterpret_cast<float4 *>(dst) = y;
+                else
+                    *reinterpret_cast<uint2 *>(dst) = make_uint2(sdy_f2h(y.x) | (uint32_t)sdy_f2h(y.y) << 16, sdy_f2h(y.z) | (uint32_t)sdy_f2h(y.w) << 16);
+            }
+        }
+        x = next;
+    }
+}
+
+// Any even head: one workgroup per token, one wave per head of q or k (with its v), the head in LDS.
 template <class KT>
-__global__ __launch_bounds__(256) void k_qk_rope_at(sdy_rope_at_args a) {
+__global__ __launch_bounds__(256) void k_rope_any(sdy_rope_at_args a) {
     __shared__ float cs[256], sn[256], heads[4][512];
     const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int half = a.n_rot / 2;
     const int pos = a.pos[t];
-    const long slot = a.slot ? a.slot[t] : pos;
     if (tid < half) {
         double s, c;
         sincos_f64((double)pos * a.freq[tid], &s, &c);
         cs[tid] = (float)((double)a.mscale * c);
         sn[tid] = (float)((double)a.mscale * s);
     }
-    // of two tokens with one slot the later one's row stays
-    int keep = a.k && slot >= 0 && slot < a.n_slot;
-    if (keep)
-        for (int u = t + 1 + tid; u < a.n_tok; u += 256) keep &= (a.slot ? a.slot[u] : a.pos[u]) != slot;
-    keep = __syncthreads_and(keep);
-    const int n_q = a.q ? a.n_head : 0, n_k = keep ? a.n_kv_head : 0;
+    const long slot = slot_of(a, t);
+    const int n_q = a.q ? a.n_head : 0, n_k = slot >= 0 ? a.n_kv_head : 0;
     float *buf = heads[wave];
     for (int h = wave; h < n_q + n_k; h += 4) {
         const bool is_q = h < n_q;
@@ -104,6 +188,16 @@ __global__ __launch_bounds__(256) void k_qk_rope_at(sdy_rope_at_args a) {
     }
 }
 
+// Few tokens: a workgroup for every 256 lanes' rows; from 1024 of those on, one per token.
+template <int HD, class KT>
+int launch_rows(const sdy_rope_at_args &a, hipStream_t st) {
+    constexpr int RPP = 256 / (HD / 4);
+    const int all = (a.q ? a.n_head : 0) + (a.k ? 2 * a.n_kv_head : 0), parts = (all + RPP - 1) / RPP;
+    const bool few = (long)a.n_tok * parts <= 1024 && parts <= 65535;
+    hipLaunchKernelGGL((k_rope_rows<HD, KT>), dim3(a.n_tok, few ? parts : 1), dim3(256), 0, st, a, few ? RPP : all);
+    return sdy_check_launch("qk_rope_at");
+}
+
 }  // namespace
 
 extern "C" int sdy_qk_rope_at(const sdy_rope_at_args *a, sdy_stream s) {
@@ -125,9 +219,23 @@ extern "C" int sdy_qk_rope_at(const sdy_rope_at_args *a, sdy_stream s) {
     // rows may share memory only where they are the same rows: a token's heads are written while others are read
     if (a->q && a->q_out == a->q && a->q_out_stride != a->q_stride)
         return sdy_fail(-1, "qk_rope_at: q in place needs q_out_stride %ld to be q_stride %ld", a->q_out_stride, a->q_stride);
-    if (a->kv_type == SDY_KV_F16)
-        hipLaunchKernelGGL(k_qk_rope_at<uint16_t>, dim3(a->n_tok), dim3(256), 0, (hipStream_t)s, *a);
-    else
-        hipLaunchKernelGGL(k_qk_rope_at<float>, dim3(a->n_tok), dim3(256), 0, (hipStream_t)s, *a);
+    hipStream_t st = (hipStream_t)s;
+    const bool f16 = a->kv_type == SDY_KV_F16;
+    // rows of float4 (and of 4 stored values), no four dims half turned
+    const bool wide = (a->hd == 32 || a->hd == 64 || a->hd == 128 || a->hd == 256) && a->n_rot % (a->interleaved ? 4 : 8) == 0 &&
+                      (!a->q || !(((uintptr_t)a->q | (uintptr_t)a->q_out) & 15 || (a->q_stride | a->q_out_stride) & 3)) &&
+                      (!a->k || !(((uintptr_t)a->k | (uintptr_t)a->v) & 15 || (a->k_stride | a->v_stride | a->head_stride) & 3 ||
+                                  ((uintptr_t)a->k_rows | (uintptr_t)a->v_rows) & (f16 ? 7 : 15))) &&
+                      !(((uintptr_t)a->q_norm | (uintptr_t)a->k_norm) & 15);
+    if (wide) {
+        switch (a->hd) {
+            case 32: return f16 ? launch_rows<32, uint16_t>(*a, st) : launch_rows<32, float>(*a, st);
+            case 64: return f16 ? launch_rows<64, uint16_t>(*a, st) : launch_rows<64, float>(*a, st);
+            case 128: return f16 ? launch_rows<128, uint16_t>(*a, st) : launch_rows<128, float>(*a, st);
+            default: return f16 ? launch_rows<256, uint16_t>(*a, st) : launch_rows<256, float>(*a, st);
+        }
+    }
+    if (f16) hipLaunchKernelGGL(k_rope_any<uint16_t>, dim3(a->n_tok), dim3(256), 0, st, *a);
+    else hipLaunchKernelGGL(k_rope_any<float>, dim3(a->n_tok), dim3(256), 0, st, *a);
     return sdy_check_launch("qk_rope_at");
 }
