@@ -67,11 +67,13 @@ template <int HD, class KT, int RW, int KW>
 struct Lds {
     static constexpr bool F32 = std::is_same<KT, float>::value;
     static constexpr int NP = F32 ? 2 : 1;    // f16 parts of a K or V value
-    static constexpr int RS = HD + 8;         // f16 of a row: consecutive rows start 4 banks apart
-    static constexpr int PLANE = 32 * RS;
-    static constexpr size_t tile = (size_t)2 * NP * PLANE * 2;   // bytes, K parts then V parts
-    static constexpr size_t tiles = KW * tile;
-    static constexpr size_t flags = KW * 32 * 4 + 16;            // bad, the greatest |K| and |V|
+    // f16 of a row: K's rows start 4 banks apart (eight lanes read 16 bytes of a row each), V's 8 (four rows' 32 bytes)
+    static constexpr int KS = HD + 8, VS = HD + 16;
+    static constexpr int KPLANE = 32 * KS, VPLANE = 32 * VS, TILE = NP * (KPLANE + VPLANE);
+    // two tiles where they leave room for two workgroups, so that one is written while the other is read
+    static constexpr int BUFS = KW == 1 && (size_t)2 * TILE * 2 <= 76 * 1024 ? 2 : 1;
+    static constexpr size_t tiles = (size_t)KW * BUFS * TILE * 2;
+    static constexpr size_t flags = KW * (BUFS * 32 * 4 + 4 * 8);  // bad, the greatest |K| and |V| of four tiles
     static constexpr size_t masks = MAX_NODES * (MAX_NODES / 32) * 4 + MAX_NODES * 2;
     static constexpr int OS = HD + 4;
     static constexpr size_t merge = KW > 1 ? (size_t)KW * 32 * RW * (OS + 2) * 4 : 0;
@@ -108,7 +110,7 @@ template <int HD, class KT, int RW>
 struct Stage {
     static constexpr bool F32 = std::is_same<KT, float>::value;
     static constexpr int LPR = 2 * RW;                              // lanes of a row
-    static constexpr int CE = F32 ? 4 : (HD / 8 >= LPR ? 8 : 4);    // elements of a chunk
+    static constexpr int CE = HD / 8 >= LPR ? 8 : 4;                // elements of a chunk
     static constexpr int NC = HD / CE / LPR;                        // chunks of a lane
     static constexpr int W = CE * (int)sizeof(KT) / 4;              // words of a chunk
     static_assert(NC >= 1 && HD == NC * CE * LPR, "a row's chunks divide over its lanes");
@@ -118,9 +120,12 @@ struct Stage {
 #pragma unroll
         for (int i = 0; i < NC; i++) {
             const uint32_t at = o + (uint32_t)(i * LPR * CE * sizeof(KT));
-            if constexpr (W == 4) {
-                const auto u = __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0);
-                for (int w = 0; w < 4; w++) r[i][w] = u[w];
+            if constexpr (W >= 4) {
+#pragma unroll
+                for (int x = 0; x < W; x += 4) {
+                    const auto u = __builtin_amdgcn_raw_buffer_load_b128(rs, at + 4 * x, 0, 0);
+                    for (int w = 0; w < 4; w++) r[i][x + w] = u[w];
+                }
             } else {
                 const auto u = __builtin_amdgcn_raw_buffer_load_b64(rs, at, 0, 0);
                 for (int w = 0; w < 2; w++) r[i][w] = u[w];
@@ -156,27 +161,23 @@ struct Stage {
             for (int w = 0; w < W; w += 2) m = max3_abs(m, r[i][w], r[i][w + 1]);
         return m;
     }
-    // The row's parts (f32: of the values times sc) to the planes at dst
+    // The row's parts (f32: of the values times sc) to the planes at dst, rows RS apart
+    template <int RS>
     SDY_DEV void store(uint16_t *dst, float sc, int tg) const {
-        constexpr int RS = HD + 8;
         uint16_t *d = dst + (tg / LPR) * RS + (tg % LPR) * CE;
 #pragma unroll
         for (int i = 0; i < NC; i++) {
-            if constexpr (F32) {
-                u32x2 hi, lo;
+            uint32_t out[2][CE / 2];
 #pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    uint32_t h, l;
-                    split2(__uint_as_float(r[i][2 * w]) * sc, __uint_as_float(r[i][2 * w + 1]) * sc, h, l);
-                    hi[w] = h;
-                    lo[w] = l;
-                }
-                *reinterpret_cast<u32x2 *>(d + i * LPR * CE) = hi;
-                *reinterpret_cast<u32x2 *>(d + 32 * RS + i * LPR * CE) = lo;
-            } else if constexpr (W == 4) {
-                *reinterpret_cast<u32x4 *>(d + i * LPR * CE) = u32x4{r[i][0], r[i][1], r[i][2], r[i][3]};
-            } else {
-                *reinterpret_cast<u32x2 *>(d + i * LPR * CE) = u32x2{r[i][0], r[i][1]};
+            for (int w = 0; w < CE / 2; w++) {
+                if constexpr (F32) split2(__uint_as_float(r[i][2 * w]) * sc, __uint_as_float(r[i][2 * w + 1]) * sc, out[0][w], out[1][w]);
+                else out[0][w] = r[i][w];
+            }
+#pragma unroll
+            for (int p = 0; p < (F32 ? 2 : 1); p++) {
+                uint16_t *to = d + p * 32 * RS + i * LPR * CE;
+                if constexpr (CE == 8) *reinterpret_cast<u32x4 *>(to) = u32x4{out[p][0], out[p][1], out[p][2], out[p][3]};
+                else *reinterpret_cast<u32x2 *>(to) = u32x2{out[p][0], out[p][1]};
             }
         }
     }
@@ -218,7 +219,8 @@ template <int HD, class KT, int RW, int KW>
 __global__ __launch_bounds__(64 * RW * KW) void k_tree_part(TreeArgs A) {
     using L = Lds<HD, KT, RW, KW>;
     constexpr bool F32 = L::F32;
-    constexpr int NP = L::NP, RS = L::RS, ND = HD / 32, NS = HD / 16, GROUP = 64 * RW;
+    constexpr int NP = L::NP, KS = L::KS, VS = L::VS, BUFS = L::BUFS, ND = HD / 32, NS = HD / 16, GROUP = 64 * RW;
+    using St = Stage<HD, KT, RW>;
     extern __shared__ __align__(16) unsigned char lds_bytes[];
     const sdy_attn_tree_args &a = A.a;
     const int past = *a.n_past;
@@ -244,9 +246,10 @@ __global__ __launch_bounds__(64 * RW * KW) void k_tree_part(TreeArgs A) {
     const bool live = row < A.rows;
     const int node = live ? row / rep : 0;
 
-    uint16_t *const kt = reinterpret_cast<uint16_t *>(lds_bytes + kw * L::tile), *const vt = kt + NP * L::PLANE;
-    float *const bad = reinterpret_cast<float *>(lds_bytes + L::body) + kw * 32;
-    unsigned *const greatest = reinterpret_cast<unsigned *>(lds_bytes + L::body) + KW * 32;
+    uint16_t *const tiles = reinterpret_cast<uint16_t *>(lds_bytes) + kw * BUFS * L::TILE;
+    float *const bads = reinterpret_cast<float *>(lds_bytes + L::body) + kw * BUFS * 32;
+    // the greatest |K| and |V| beyond the scale's, of four tiles in turn; for all waves, or each one's own
+    unsigned *const greatest = reinterpret_cast<unsigned *>(lds_bytes + L::body) + KW * BUFS * 32 + (RW > 1 ? 0 : 8 * kw);
 
     uint32_t sees[MAX_NODES / 32];
     if (draft) {
@@ -306,141 +309,186 @@ __global__ __launch_bounds__(64 * RW * KW) void k_tree_part(TreeArgs A) {
     const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void *)kbase, (short)0, size, 0x00020000);
     const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void *)vbase, (short)0, size, 0x00020000);
     const int rounds = (n_keys + KB * KW - 1) / (KB * KW);
-    Stage<HD, KT, RW> sk, sv;
-    sk.load(rk, (uint32_t)(kw * KB), tg);
-    sv.load(rv, (uint32_t)(kw * KB), tg);
+    St sk, sv;
     auto sync = [&]() {
         if constexpr (RW > 1) __syncthreads();
         else sdy_wave_sync();
     };
-    for (int it = 0; it < rounds; it++) {
-        const int k0 = (it * KW + kw) * KB;  // within the span
-        if (draft) {
-            // an empty place's rows are left out; rows with an infinity or a NaN are NaN for those that see them and nothing
-            // for the others
-            const int t = k0 + tg / Stage<HD, KT, RW>::LPR;
-            const bool u = sk.unfit() || sv.unfit();
-            if (u || t >= a.n_tok || a.parent[t] < -1) {
-                sk.clear();
-                sv.clear();
-            }
-            if (tg % Stage<HD, KT, RW>::LPR == 0) bad[tg / Stage<HD, KT, RW>::LPR] = u ? NAN : 0.0f;
+    const bool leader = RW > 1 ? tid == 0 : lane == 0;
+    auto at_round = [&](int it) { return (uint32_t)((it * KW + kw) * KB); };  // the group's first position in the span
+    // An empty place's drafted rows are left out; rows with an infinity or a NaN are NaN for those that see them and nothing
+    // for the others.
+    auto drafted = [&](int it) {
+        const int t = (int)at_round(it) + tg / St::LPR;
+        const bool u = sk.unfit() || sv.unfit();
+        if (u || t >= a.n_tok || a.parent[t] < -1) {
+            sk.clear();
+            sv.clear();
         }
-        if constexpr (F32) {
-            float mk = sk.most(), mv = sv.most();
-            const bool over = exp_of(mk) > xk + 2 || exp_of(mv) > xv + 2;
-            bool any;
-            if constexpr (RW > 1) any = __syncthreads_or(over);
-            else any = __ballot(over) != 0;
-            if (any) {  // new scales, the same for all that share tiles
-                for (int off = 32; off >= 1; off >>= 1) {
-                    mk = fmaxf(mk, __shfl_xor(mk, off));
-                    mv = fmaxf(mv, __shfl_xor(mv, off));
-                }
-                if constexpr (RW > 1) {
-                    if (tid < 2) greatest[tid] = 0;
-                    __syncthreads();
-                    if (lane == 0) {
-                        atomicMax(&greatest[0], __float_as_uint(mk));
-                        atomicMax(&greatest[1], __float_as_uint(mv));
-                    }
-                    __syncthreads();
-                    mk = __uint_as_float(greatest[0]);
-                    mv = __uint_as_float(greatest[1]);
-                }
-                if (exp_of(mk) > xk) xk = exp_of(mk);
-                const int x = exp_of(mv) > xv ? exp_of(mv) : xv;
-                factor = ldexpf(A.log_scale, eq + xk - TOP);
-#pragma unroll
-                for (int d = 0; d < ND; d++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) o[d][e] = ldexpf(o[d][e], xv - x);
-                xv = x;
+        if (tg % St::LPR == 0) bads[(it & (BUFS - 1)) * 32 + tg / St::LPR] = u ? NAN : 0.0f;
+    };
+    // notes the greatest values for tile `it` where they are beyond the scales
+    auto note = [&](int it, float mk, float mv) {
+        if (__ballot(exp_of(mk) > xk + 2 || exp_of(mv) > xv + 2)) {
+            for (int off = 32; off >= 1; off >>= 1) {
+                mk = fmaxf(mk, __shfl_xor(mk, off));
+                mv = fmaxf(mv, __shfl_xor(mv, off));
+            }
+            if (lane == 0) {
+                atomicMax(&greatest[2 * (it & 3)], __float_as_uint(mk));
+                atomicMax(&greatest[2 * (it & 3) + 1], __float_as_uint(mv));
             }
         }
-        sk.store(kt, exp_scale(xk), tg);
-        sv.store(vt, exp_scale(xv), tg);
+    };
+    auto store_k = [&](int it) { sk.template store<KS>(tiles + (it & (BUFS - 1)) * L::TILE, exp_scale(xk), tg); };
+    auto store_v = [&](int it) { sv.template store<VS>(tiles + (it & (BUFS - 1)) * L::TILE + NP * L::KPLANE, exp_scale(xv), tg); };
+    // new scales from what was noted for tile `it`
+    auto rescale = [&](int it) {
+        const int ek = exp_of(__uint_as_float(greatest[2 * (it & 3)])), ev = exp_of(__uint_as_float(greatest[2 * (it & 3) + 1]));
+        xk = ek > xk ? ek : xk;
+        const int x = ev > xv ? ev : xv;
+        factor = ldexpf(A.log_scale, eq + xk - TOP);
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[d][e] = ldexpf(o[d][e], xv - x);
+        xv = x;
+    };
+    if constexpr (F32) {
+        if (lane < 8) greatest[lane] = 0;
         sync();
-        if (it + 1 < rounds) {
-            sk.load(rk, (uint32_t)(k0 + KW * KB), tg);
-            sv.load(rv, (uint32_t)(k0 + KW * KB), tg);
+    }
+    sk.load(rk, at_round(0), tg);
+    sv.load(rv, at_round(0), tg);
+    if (draft) drafted(0);
+    if constexpr (F32) {
+        note(0, sk.most(), sv.most());
+        sync();
+        rescale(0);
+        sync();
+        if (leader) greatest[0] = greatest[1] = 0;
+    }
+    store_k(0);
+    store_v(0);
+    sk.load(rk, at_round(1), tg);
+    sv.load(rv, at_round(1), tg);
+    for (int it = 0; it < rounds; it++) {
+        const int k0 = (int)at_round(it);
+        sync();
+        if constexpr (F32) {
+            if (leader) greatest[2 * ((it + 2) & 3)] = greatest[2 * ((it + 2) & 3) + 1] = 0;
+            const uint2 g = *reinterpret_cast<const uint2 *>(greatest + 2 * (it & 3));
+            if (__builtin_amdgcn_readfirstlane(g.x | g.y)) {  // the tile was stored beyond its scales: once more
+                rescale(it);
+                sk.load(rk, at_round(it), tg);
+                sv.load(rv, at_round(it), tg);
+                if (draft) drafted(it);
+                sync();
+                store_k(it);
+                store_v(it);
+                sk.load(rk, at_round(it + 1), tg);
+                sv.load(rv, at_round(it + 1), tg);
+                sync();
+            }
         }
-        if (k0 < n_keys) {
-            f32x16 s = f32x16{};
-            const uint16_t *kr = kt + ql * RS + 8 * hh;
+        const uint16_t *const kt = tiles + (it & (BUFS - 1)) * L::TILE, *const vt = kt + NP * L::KPLANE;
+        const float *const bad = bads + (it & (BUFS - 1)) * 32;
+        float mk = 0.0f, mv = 0.0f;
+        // the next tile's rows into the other buffer and the one after it on its way
+        if constexpr (BUFS == 2) {
+            if (draft) drafted(it + 1);
+        }
+        f32x16 s = f32x16{};
+        {
+            const uint16_t *kr = kt + ql * KS + 8 * hh;
 #pragma unroll
             for (int i = 0; i < NS; i++) {
                 const f16x8 k = *reinterpret_cast<const f16x8 *>(kr + 16 * i);
                 s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qlo[i], s, 0, 0, 0);
                 if constexpr (F32)
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8 *>(kr + 32 * RS + 16 * i), qh[i], s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8 *>(kr + L::KPLANE + 16 * i), qh[i], s, 0, 0, 0);
                 s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[i], s, 0, 0, 0);
             }
-            // register r: position 8 (r / 4) + 4 hh + r % 4 of the tile
-            if (draft) {
-                __asm__ volatile("");  // (a branch: not worth a select per score)
-                const uint32_t bits = sees[k0 / KB] >> (4 * hh);
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int k = 8 * (r >> 2) + (r & 3);
-                    s[r] = bits >> k & 1 ? s[r] + bad[k + 4 * hh] : -INFINITY;
-                }
-            } else if (k0 + KB > n_keys) {
-                __asm__ volatile("");
-#pragma unroll
-                for (int r = 0; r < 16; r++) s[r] = k0 + 8 * (r >> 2) + 4 * hh + (r & 3) < n_keys ? s[r] : -INFINITY;
-            }
-            float mt = s[0];
-#pragma unroll
-            for (int r = 1; r < 16; r++) mt = fmaxf(mt, s[r]);
-            mt = fmaxf(mt, __shfl_xor(mt, 32));
-            const float m_new = fmaxf(m, ceilf(mt * factor));
-            const float mu = m_new == -INFINITY ? 0.0f : m_new;  // nothing seen yet: every weight is 0
-            float p[16], ls = 0.0f;
+        }
+        if constexpr (BUFS == 2) {
+            if constexpr (F32) mk = sk.most();
+            store_k(it + 1);
+            sk.load(rk, at_round(it + 2), tg);
+        }
+        // register r: position 8 (r / 4) + 4 hh + r % 4 of the tile
+        if (draft) {
+            __asm__ volatile("");  // (a branch: not worth a select per score)
+            const uint32_t bits = k0 < n_keys ? sees[k0 / KB] >> (4 * hh) : 0u;
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], factor, P_BITS - mu));
-                ls += p[r];
+                const int k = 8 * (r >> 2) + (r & 3);
+                s[r] = bits >> k & 1 ? s[r] + bad[k + 4 * hh] : -INFINITY;
             }
-            // exact: both maxima are whole
-            const int down = m == -INFINITY ? -300 : (int)fmaxf(m - mu, -300.0f);
-            l = ldexpf(l, down) + ls;
-            m = m_new;
-            if (__ballot(down != 0)) {
+        } else if (k0 + KB > n_keys) {
+            __asm__ volatile("");
 #pragma unroll
-                for (int d = 0; d < ND; d++)
+            for (int r = 0; r < 16; r++) s[r] = k0 + 8 * (r >> 2) + 4 * hh + (r & 3) < n_keys ? s[r] : -INFINITY;
+        }
+        float mt = s[0];
 #pragma unroll
-                    for (int e = 0; e < 16; e++) o[d][e] = ldexpf(o[d][e], down);
+        for (int r = 1; r < 16; r++) mt = fmaxf(mt, s[r]);
+        mt = fmaxf(mt, __shfl_xor(mt, 32));
+        const float m_new = fmaxf(m, ceilf(mt * factor));
+        const float mu = m_new == -INFINITY ? 0.0f : m_new;  // nothing seen yet: every weight is 0
+        float p[16], ls = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], factor, P_BITS - mu));
+            ls += p[r];
+        }
+        // exact: both maxima are whole
+        const int down = m == -INFINITY ? -300 : (int)fmaxf(m - mu, -300.0f);
+        l = ldexpf(l, down) + ls;
+        m = m_new;
+        if (__ballot(down != 0)) {
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[d][e] = ldexpf(o[d][e], down);
+        }
+        // step u: positions 16 u + 4 hh .. + 3 and 16 u + 8 + 4 hh .. + 3 of the tile, the scores' registers 8 u ..
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            u32x4 h, w;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t h0, l0;
+                split2(p[8 * u + 2 * j], p[8 * u + 2 * j + 1], h0, l0);
+                h[j] = h0;
+                w[j] = l0;
             }
-            // step u: positions 16 u + 4 hh .. + 3 and 16 u + 8 + 4 hh .. + 3 of the tile, the scores' registers 8 u ..
+            const f16x8 ph = __builtin_bit_cast(f16x8, h), pl = __builtin_bit_cast(f16x8, w);
+            // V^T by transposing reads: 16 lanes give the addresses of 4 rows x 16 dims (4 each) and get a dim's 4 rows
+            auto vread = [&](int plane, int d) {
+                const uint16_t *at = vt + plane * L::VPLANE + (16 * u + 4 * hh + ((lane & 15) >> 2)) * VS + 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at);
+                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(at + 8 * VS));
+                return __builtin_bit_cast(f16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                u32x4 h, w;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    uint32_t h0, l0;
-                    split2(p[8 * u + 2 * j], p[8 * u + 2 * j + 1], h0, l0);
-                    h[j] = h0;
-                    w[j] = l0;
-                }
-                const f16x8 ph = __builtin_bit_cast(f16x8, h), pl = __builtin_bit_cast(f16x8, w);
-                // V^T by transposing reads: 16 lanes give the addresses of 4 rows x 16 dims (4 each) and get a dim's 4 rows
-                auto vread = [&](int plane, int d) {
-                    uint16_t *at = vt + plane * L::PLANE + (16 * u + 4 * hh + ((lane & 15) >> 2)) * RS + 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-                    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at);
-                    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(at + 8 * RS));
-                    return __builtin_bit_cast(f16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-                };
-#pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    const f16x8 v = vread(0, d);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[d], 0, 0, 0);
-                    if constexpr (F32) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vread(1, d), ph, o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[d], 0, 0, 0);
-                }
+            for (int d = 0; d < ND; d++) {
+                const f16x8 v = vread(0, d);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[d], 0, 0, 0);
+                if constexpr (F32) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vread(1, d), ph, o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[d], 0, 0, 0);
             }
         }
-        sync();
+        if constexpr (BUFS == 1) {
+            sync();
+            if (draft) drafted(it + 1);
+            if constexpr (F32) mk = sk.most();
+            store_k(it + 1);
+            sk.load(rk, at_round(it + 2), tg);
+        }
+        if constexpr (F32) mv = sv.most();
+        store_v(it + 1);
+        sv.load(rv, at_round(it + 2), tg);
+        if constexpr (F32) note(it + 1, mk, mv);
     }
     l += __shfl_xor(l, 32);
     if constexpr (F32) {
