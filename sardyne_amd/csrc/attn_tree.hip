@@ -5,10 +5,11 @@
 // A parent outside [0, t) makes t a root; below -1 it marks a place without a node: its output row stays as it was and no
 // node attends to it.
 //
-//   k_tree_part<HD, KT, RW, KW>  one workgroup per (span of positions, kv head, block of 32 RW rows); a row is a node and one
-//   of the query heads that share the kv head, so a K/V tile is read once for all of them. Span 0 is the drafted rows. RW
-//   waves share each tile of 32 positions, KW groups of them take tiles in turn. Per tile a wave computes
-//   S^T = K Q^T (a lane holds one row's 16 scores), the running maximum and sum, and O^T += V^T P.
+//   k_tree_part<HD, KT, RB, RW, KW>  one workgroup per (span of positions, kv head, block of 32 RB RW rows); a row is a node
+//   and one of the query heads that share the kv head, so a K/V tile is read once for all of them. Span 0 is the drafted rows.
+//   RW waves of 32 RB rows share each tile of 32 positions, KW groups of them take tiles in turn. Per tile a wave computes
+//   S^T = K Q^T (a lane holds one row's 16 scores), P = exp2(S - m), and O^T += V^T P. In turn t it multiplies K of tile t + 1
+//   while it makes P of tile t, then V of tile t while it splits K of tile t + 2 and V of tile t + 1 into the other buffers.
 //   k_tree_merge<HD>  one workgroup per node and head: the spans' (m, l, O) in span order.
 //
 // Products on the f16 matrix cores at f32's precision: an f32 is the sum of two f16 (22 bits and a sign) once it is scaled by
@@ -16,8 +17,8 @@
 // taken as they are; of the split products low x low, at most 2^-22 of the whole, is left out. A row of q goes by its own
 // greatest value; a span's K and V by the greatest met so far, brought to 2^13 .. 2^16 (f16's least bit is then 2^-38 of it),
 // a power that changes with the first tile and seldom after. Powers of two go back exactly: K's and q's into the scores'
-// factor, V's into O (ldexp). The running maximum is kept as a whole number (rounded up), so that its rescales are exact too,
-// and P is 2^14 times the weight: f16's least bit is 2^-39 of the greatest weight.
+// factor, V's into O (ldexp). The running maximum m is kept as a whole number, so that its rescales are exact too, and grows
+// only when a score passes it by 2^LAG: P is 2^4 to 2^15 at the greatest weight, f16's least bit 2^-28 of it or less.
 #include <type_traits>
 
 #include "sdy_attn_dev.h"
@@ -39,7 +40,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 constexpr int MAX_NODES = 256;
 constexpr int KB = 32;         // positions per tile
 constexpr int TOP = 13;        // the greatest value is scaled to 2^TOP .. 2^(TOP + 1), later ones up to 2^(TOP + 3)
-constexpr float P_BITS = 14;   // P is 2^14 times the weight
+constexpr float P_BITS = 4;    // P is 2^P_BITS exp2(score - m), of scores up to m + LAG
+constexpr float LAG = 11;
 constexpr int MAX_PARTS = 513;
 constexpr int MAX_PAST = 1 << 28;  // 512 spans of at most 2^30 bytes hold them
 
@@ -48,7 +50,7 @@ struct TreeArgs {
     int rows;       // per kv head: n_tok * (n_head / n_kv_head)
     int n_block;    // row blocks
     int n_span;     // spans of cached positions (the grid's; those in use follow from n_past)
-    int granule;    // positions of one round of a workgroup: 32 KW
+    int granule;    // positions of one turn of a workgroup: 32 KW
     float log_scale;  // log2(e) / sqrt(head_dim)
     float *part;    // [1 + n_span][n_kv_head * rows][HD], then the (m, l) [1 + n_span][n_kv_head * rows][2]
 };
@@ -63,22 +65,22 @@ SDY_DEV int spans_used(const TreeArgs &A, int past) {
     return per ? (n + per - 1) / per : 0;
 }
 
-template <int HD, class KT, int RW, int KW>
+template <int HD, class KT, int RB, int RW, int KW>
 struct Lds {
     static constexpr bool F32 = std::is_same<KT, float>::value;
     static constexpr int NP = F32 ? 2 : 1;    // f16 parts of a K or V value
     // f16 of a row: K's rows start 4 banks apart (eight lanes read 16 bytes of a row each), V's 8 (four rows' 32 bytes)
     static constexpr int KS = HD + 8, VS = HD + 16;
     static constexpr int KPLANE = 32 * KS, VPLANE = 32 * VS, TILE = NP * (KPLANE + VPLANE);
-    // two tiles where they leave room for two workgroups, so that one is written while the other is read
-    static constexpr int BUFS = KW == 1 && (size_t)2 * TILE * 2 <= 76 * 1024 ? 2 : 1;
-    static constexpr size_t tiles = (size_t)KW * BUFS * TILE * 2;
-    static constexpr size_t flags = KW * (BUFS * 32 * 4 + 4 * 8);  // bad, the greatest |K| and |V| of four tiles
-    static constexpr size_t masks = MAX_NODES * (MAX_NODES / 32) * 4 + MAX_NODES * 2;
-    static constexpr int OS = HD + 4;
-    static constexpr size_t merge = KW > 1 ? (size_t)KW * 32 * RW * (OS + 2) * 4 : 0;
-    static constexpr size_t body = tiles > merge ? (tiles > masks ? tiles : masks) : (merge > masks ? merge : masks);
-    static constexpr size_t bytes = body + flags;
+    static constexpr size_t tiles = (size_t)KW * 2 * TILE * 2;  // two of each
+    static constexpr int ROWS = 32 * RB * RW, OS = HD + 4;
+    static constexpr size_t merge = KW > 1 ? (size_t)KW * ROWS * (OS + 2) * 4 : 0;
+    static constexpr size_t body = tiles > merge ? tiles : merge;
+    // the nodes' masks, their farthest known ancestors, and what is wrong with their rows
+    static constexpr size_t masks = MAX_NODES * (MAX_NODES / 32) * 4 + MAX_NODES * 2 + MAX_NODES * 4;
+    static constexpr size_t flags = 2 * 4 * 4;  // the greatest |K| and |V| of four tiles
+    static constexpr size_t bytes = body + masks + flags;
+    static_assert(bytes <= 160 * 1024, "fits a CU");
 };
 
 // Two f32 as two f16 pairs, hi + lo = x up to 2^-23 of x (while lo is at least f16's least normal)
@@ -184,43 +186,44 @@ struct Stage {
 };
 
 // Which nodes each node sees, as bits: mask[t] starts as t itself, then takes that of the farthest node known above it and
-// that one's farthest in turn, doubling the distance, so 8 rounds reach all of 256. In: parents. All threads of the block.
+// that one's farthest in turn, doubling the distance. All 256 threads.
 SDY_DEV void ancestor_masks(const int32_t *parent, int n, uint32_t (*mask)[MAX_NODES / 32], int16_t *up) {
-    const int tid = threadIdx.x;
-    if (tid < MAX_NODES) {
-        int p = tid < n ? parent[tid] : -2;
-        for (int w = 0; w < MAX_NODES / 32; w++) mask[tid][w] = p >= -1 && w == tid / 32 ? 1u << (tid % 32) : 0u;
-        if (p < 0 || p >= tid || parent[p] < -1) p = -1;
-        up[tid] = (int16_t)p;
-    }
+    constexpr int W = MAX_NODES / 32;
+    const int tid = threadIdx.x, words = (n + 31) / 32;
+    const int p0 = tid < n ? parent[tid] : -2;
+    up[tid] = (int16_t)(p0 < -1 ? -2 : p0 < 0 || p0 >= tid ? -1 : p0);
+#pragma unroll
+    for (int w = 0; w < W; w++) mask[tid][w] = p0 >= -1 && w == tid / 32 ? 1u << (tid % 32) : 0u;
     __syncthreads();
-    for (int round = 0; round < 8; round++) {
-        uint32_t add[MAX_NODES / 32];
+    int p = up[tid];
+    if (p >= 0 && up[p] < -1) p = -1;  // under an empty place: a root
+    __syncthreads();
+    up[tid] = (int16_t)p;
+    __syncthreads();
+    for (int reach = 1; reach < n; reach *= 2) {
+        uint32_t add[W];
         int far = -1;
-        if (tid < MAX_NODES) {
-            const int p = up[tid];
-            if (p >= 0) {
-                far = up[p];
-                for (int w = 0; w < MAX_NODES / 32; w++) add[w] = mask[p][w];
-            } else {
-                for (int w = 0; w < MAX_NODES / 32; w++) add[w] = 0;
-            }
+        if (p >= 0) {
+            far = up[p];
+            for (int w = 0; w < words; w++) add[w] = mask[p][w];
         }
         __syncthreads();
-        if (tid < MAX_NODES) {
-            for (int w = 0; w < MAX_NODES / 32; w++) mask[tid][w] |= add[w];
+        if (p >= 0) {
+            for (int w = 0; w < words; w++) mask[tid][w] |= add[w];
             up[tid] = (int16_t)far;
+            p = far;
         }
         __syncthreads();
     }
 }
 
-template <int HD, class KT, int RW, int KW>
-__global__ __launch_bounds__(64 * RW * KW) void k_tree_part(TreeArgs A) {
-    using L = Lds<HD, KT, RW, KW>;
-    constexpr bool F32 = L::F32;
-    constexpr int NP = L::NP, KS = L::KS, VS = L::VS, BUFS = L::BUFS, ND = HD / 32, NS = HD / 16, GROUP = 64 * RW;
+template <int HD, class KT, int RB, int RW, int KW>
+__global__ __launch_bounds__(256, 1) void k_tree_part(TreeArgs A) {
+    using L = Lds<HD, KT, RB, RW, KW>;
     using St = Stage<HD, KT, RW>;
+    static_assert(RW * KW == 4, "256 threads");
+    constexpr bool F32 = L::F32;
+    constexpr int NP = L::NP, KS = L::KS, VS = L::VS, ND = HD / 32, NS = HD / 16, GROUP = 64 * RW;
     extern __shared__ __align__(16) unsigned char lds_bytes[];
     const sdy_attn_tree_args &a = A.a;
     const int past = *a.n_past;
@@ -241,29 +244,37 @@ __global__ __launch_bounds__(64 * RW * KW) void k_tree_part(TreeArgs A) {
         lo = (int)l0;
         hi = h0 < past ? (int)h0 : past;
     }
+
+    const size_t elt = sizeof(KT);
+    const char *kbase = (const char *)(draft ? a.k_draft : a.k_cache) + ((size_t)g * (draft ? a.draft_stride : a.head_stride) + (size_t)lo * HD) * elt;
+    const char *vbase = (const char *)(draft ? a.v_draft : a.v_cache) + ((size_t)g * (draft ? a.draft_stride : a.head_stride) + (size_t)lo * HD) * elt;
+    const int n_keys = hi - lo, size = n_keys * (int)(HD * sizeof(KT));  // (a span's bytes fit 31 bits: the host sees to it)
+    // positions past the span's end read as zeros and are masked below
+    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void *)kbase, (short)0, size, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void *)vbase, (short)0, size, 0x00020000);
+    const int rounds = (n_keys + KB * KW - 1) / (KB * KW);
+    auto at_round = [&](int it) { return (uint32_t)((it * KW + kw) * KB); };  // the group's first position in the span
+    St sk, sv;
+    sk.load(rk, at_round(0), tg);
+    sv.load(rv, at_round(0), tg);
+
     const int rep = a.n_head / a.n_kv_head;
-    const int row = (block * RW + rw) * 32 + ql;
-    const bool live = row < A.rows;
-    const int node = live ? row / rep : 0;
-
-    uint16_t *const tiles = reinterpret_cast<uint16_t *>(lds_bytes) + kw * BUFS * L::TILE;
-    float *const bads = reinterpret_cast<float *>(lds_bytes + L::body) + kw * BUFS * 32;
-    // the greatest |K| and |V| beyond the scale's, of four tiles in turn; for all waves, or each one's own
-    unsigned *const greatest = reinterpret_cast<unsigned *>(lds_bytes + L::body) + KW * BUFS * 32 + (RW > 1 ? 0 : 8 * kw);
-
-    uint32_t sees[MAX_NODES / 32];
-    if (draft) {
-        uint32_t(*mask)[MAX_NODES / 32] = reinterpret_cast<uint32_t(*)[MAX_NODES / 32]>(lds_bytes);
-        ancestor_masks(a.parent, a.n_tok, mask, reinterpret_cast<int16_t *>(mask + MAX_NODES));
-        for (int w = 0; w < MAX_NODES / 32; w++) sees[w] = live ? mask[node][w] : 0u;
-        __syncthreads();
-    }
+    const int row0 = (block * RW + rw) * 32 * RB + ql;  // and 32 further on
+    uint16_t *const tiles = reinterpret_cast<uint16_t *>(lds_bytes) + kw * 2 * L::TILE;
+    uint32_t(*const mask)[MAX_NODES / 32] = reinterpret_cast<uint32_t(*)[MAX_NODES / 32]>(lds_bytes + L::body);
+    int16_t *const up = reinterpret_cast<int16_t *>(mask + MAX_NODES);
+    float *const wrong = reinterpret_cast<float *>(up + MAX_NODES);  // 0, NaN (an infinity or a NaN in its rows), inf (no node)
+    unsigned *const greatest = reinterpret_cast<unsigned *>(wrong + MAX_NODES);
 
     // the rows' queries: step i holds dims 16 i + 8 hh .. + 7
-    f16x8 qh[NS], qlo[NS];
-    int eq = 0;
-    {
-        const float *q = a.q + (size_t)node * a.q_stride + (size_t)(g * rep + (live ? row - node * rep : 0)) * HD + 8 * hh;
+    f16x8 qh[RB][NS], qlo[RB][NS];
+    int eq[RB], node[RB];
+#pragma unroll
+    for (int b = 0; b < RB; b++) {
+        const int row = row0 + 32 * b;
+        node[b] = row < A.rows ? row / rep : 0;
+        const float *q = a.q + (size_t)node[b] * a.q_stride + (size_t)(g * rep + (row < A.rows ? row - node[b] * rep : 0)) * HD + 8 * hh;
+        if (row >= A.rows) node[b] = -1;
         float most = 0.0f;
         float4 v[2 * NS];
 #pragma unroll
@@ -272,12 +283,14 @@ __global__ __launch_bounds__(64 * RW * KW) void k_tree_part(TreeArgs A) {
             v[2 * i + 1] = *reinterpret_cast<const float4 *>(q + 16 * i + 4);
         }
 #pragma unroll
-        for (int i = 0; i < 2 * NS; i++)
-            most = fmaxf(most, fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
+        for (int i = 0; i < 2 * NS; i++) {
+            most = max3_abs(most, __float_as_uint(v[i].x), __float_as_uint(v[i].y));
+            most = max3_abs(most, __float_as_uint(v[i].z), __float_as_uint(v[i].w));
+        }
         most = fmaxf(most, __shfl_xor(most, 32));
-        eq = exp_of(most);
-        const float sc = exp_scale(eq);
-        eq -= TOP;
+        const int e0 = exp_of(most);
+        const float sc = exp_scale(e0);
+        eq[b] = e0 - TOP;
 #pragma unroll
         for (int i = 0; i < NS; i++) {
             u32x4 h, l;
@@ -289,180 +302,233 @@ __global__ __launch_bounds__(64 * RW * KW) void k_tree_part(TreeArgs A) {
                 split2(x.z * sc, x.w * sc, h1, l1);
                 h[2 * e] = h0, h[2 * e + 1] = h1, l[2 * e] = l0, l[2 * e + 1] = l1;
             }
-            qh[i] = __builtin_bit_cast(f16x8, h);
-            qlo[i] = __builtin_bit_cast(f16x8, l);
+            qh[b][i] = __builtin_bit_cast(f16x8, h);
+            qlo[b][i] = __builtin_bit_cast(f16x8, l);
         }
     }
 
-    f32x16 o[ND];
+    f32x16 o[RB][ND];
+    float m[RB], l[RB], factor[RB];  // m whole; the factor of the next scores
 #pragma unroll
-    for (int d = 0; d < ND; d++) o[d] = f32x16{};
-    float m = -INFINITY, l = 0.0f;  // m whole
+    for (int b = 0; b < RB; b++) {
+#pragma unroll
+        for (int d = 0; d < ND; d++) o[b][d] = f32x16{};
+        m[b] = -INFINITY;
+        l[b] = 0.0f;
+        factor[b] = ldexpf(A.log_scale, eq[b]);
+    }
     int xk = F32 ? -101 : TOP, xv = xk;  // the exponents that K's and V's scales go by (none yet for f32)
-    float factor = ldexpf(A.log_scale, eq);
 
-    const size_t elt = sizeof(KT);
-    const char *kbase = (const char *)(draft ? a.k_draft : a.k_cache) + ((size_t)g * (draft ? a.draft_stride : a.head_stride) + (size_t)lo * HD) * elt;
-    const char *vbase = (const char *)(draft ? a.v_draft : a.v_cache) + ((size_t)g * (draft ? a.draft_stride : a.head_stride) + (size_t)lo * HD) * elt;
-    const int n_keys = hi - lo, size = n_keys * (int)(HD * sizeof(KT));  // (a span's bytes fit 31 bits: the host sees to it)
-    // positions past the span's end read as zeros and are masked below
-    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void *)kbase, (short)0, size, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void *)vbase, (short)0, size, 0x00020000);
-    const int rounds = (n_keys + KB * KW - 1) / (KB * KW);
-    St sk, sv;
-    auto sync = [&]() {
-        if constexpr (RW > 1) __syncthreads();
-        else sdy_wave_sync();
-    };
-    const bool leader = RW > 1 ? tid == 0 : lane == 0;
-    auto at_round = [&](int it) { return (uint32_t)((it * KW + kw) * KB); };  // the group's first position in the span
-    // An empty place's drafted rows are left out; rows with an infinity or a NaN are NaN for those that see them and nothing
-    // for the others.
-    auto drafted = [&](int it) {
+    // Drafted rows: which nodes see which, and rows that are left out (an empty place's) or would be all that a tile's other
+    // rows are read by (with an infinity or a NaN: NaN for those that see them, nothing for the others).
+    if (draft) {
+        ancestor_masks(a.parent, a.n_tok, mask, up);
+        for (int it = 0; it < rounds; it++) {
+            if (it > 0) {
+                sk.load(rk, at_round(it), tg);
+                sv.load(rv, at_round(it), tg);
+            }
+            const bool uk = sk.unfit(), u = sv.unfit() || uk;
+            const int t = (int)at_round(it) + tg / St::LPR;
+            if (t < MAX_NODES && tg % St::LPR == 0) wrong[t] = !(mask[t][t / 32] >> (t % 32) & 1) ? INFINITY : u ? NAN : 0.0f;
+        }
+        if (rounds > 1) {
+            sk.load(rk, at_round(0), tg);
+            sv.load(rv, at_round(0), tg);
+        }
+    }
+    if (F32 && tid < 8) greatest[tid] = 0;
+    __syncthreads();
+    auto drafted = [&](St &st, int it) {
         const int t = (int)at_round(it) + tg / St::LPR;
-        const bool u = sk.unfit() || sv.unfit();
-        if (u || t >= a.n_tok || a.parent[t] < -1) {
-            sk.clear();
-            sv.clear();
-        }
-        if (tg % St::LPR == 0) bads[(it & (BUFS - 1)) * 32 + tg / St::LPR] = u ? NAN : 0.0f;
+        if (t >= a.n_tok || !(wrong[t] == 0.0f)) st.clear();
     };
-    // notes the greatest values for tile `it` where they are beyond the scales
-    auto note = [&](int it, float mk, float mv) {
-        if (__ballot(exp_of(mk) > xk + 2 || exp_of(mv) > xv + 2)) {
-            for (int off = 32; off >= 1; off >>= 1) {
-                mk = fmaxf(mk, __shfl_xor(mk, off));
-                mv = fmaxf(mv, __shfl_xor(mv, off));
-            }
-            if (lane == 0) {
-                atomicMax(&greatest[2 * (it & 3)], __float_as_uint(mk));
-                atomicMax(&greatest[2 * (it & 3) + 1], __float_as_uint(mv));
-            }
+    // notes a greatest value for the K (which 0) or V (1) of turn `it` where it is beyond the scale
+    auto note = [&](int it, int which, float most, int x) {
+        if (__ballot(exp_of(most) > x + 2)) {
+            for (int off = 32; off >= 1; off >>= 1) most = fmaxf(most, __shfl_xor(most, off));
+            if (lane == 0) atomicMax(&greatest[2 * (it & 3) + which], __float_as_uint(most));
         }
     };
-    auto store_k = [&](int it) { sk.template store<KS>(tiles + (it & (BUFS - 1)) * L::TILE, exp_scale(xk), tg); };
-    auto store_v = [&](int it) { sv.template store<VS>(tiles + (it & (BUFS - 1)) * L::TILE + NP * L::KPLANE, exp_scale(xv), tg); };
-    // new scales from what was noted for tile `it`
-    auto rescale = [&](int it) {
-        const int ek = exp_of(__uint_as_float(greatest[2 * (it & 3)])), ev = exp_of(__uint_as_float(greatest[2 * (it & 3) + 1]));
-        xk = ek > xk ? ek : xk;
-        const int x = ev > xv ? ev : xv;
-        factor = ldexpf(A.log_scale, eq + xk - TOP);
+    auto store_k = [&](int it) { sk.template store<KS>(tiles + (it & 1) * NP * L::KPLANE, exp_scale(xk), tg); };
+    auto store_v = [&](int it) { sv.template store<VS>(tiles + 2 * NP * L::KPLANE + (it & 1) * NP * L::VPLANE, exp_scale(xv), tg); };
+    // a new scale from what was noted for turn `it`
+    auto rescale_k = [&](int it) {
+        const int e = exp_of(__uint_as_float(greatest[2 * (it & 3)]));
+        xk = e > xk ? e : xk;
 #pragma unroll
-        for (int d = 0; d < ND; d++)
+        for (int b = 0; b < RB; b++) factor[b] = ldexpf(A.log_scale, eq[b] + xk - TOP);
+    };
+    auto rescale_v = [&](int it) {
+        const int e = exp_of(__uint_as_float(greatest[2 * (it & 3) + 1])), x = e > xv ? e : xv;
 #pragma unroll
-            for (int e = 0; e < 16; e++) o[d][e] = ldexpf(o[d][e], xv - x);
+        for (int b = 0; b < RB; b++)
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int e2 = 0; e2 < 16; e2++) o[b][d][e2] = ldexpf(o[b][d][e2], xv - x);
         xv = x;
     };
-    if constexpr (F32) {
-        if (lane < 8) greatest[lane] = 0;
-        sync();
+    f32x16 s[RB];
+    // S^T of turn `it`
+    auto scores = [&](int it) {
+        const uint16_t *kr = tiles + (it & 1) * NP * L::KPLANE + ql * KS + 8 * hh;
+#pragma unroll
+        for (int b = 0; b < RB; b++) s[b] = f32x16{};
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+            const f16x8 k = *reinterpret_cast<const f16x8 *>(kr + 16 * i);
+#pragma unroll
+            for (int b = 0; b < RB; b++) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qlo[b][i], s[b], 0, 0, 0);
+            if constexpr (F32) {
+                const f16x8 k2 = *reinterpret_cast<const f16x8 *>(kr + L::KPLANE + 16 * i);
+#pragma unroll
+                for (int b = 0; b < RB; b++) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k2, qh[b][i], s[b], 0, 0, 0);
+            }
+#pragma unroll
+            for (int b = 0; b < RB; b++) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[b][i], s[b], 0, 0, 0);
+        }
+    };
+    // register r of the scores: position 8 (r / 4) + 4 hh + r % 4 of the tile
+    auto masked = [&](int it) {
+        const int k0 = (int)at_round(it);
+        if (draft) {
+            __asm__ volatile("");  // (a branch: not worth a select per score)
+#pragma unroll
+            for (int b = 0; b < RB; b++) {
+                const uint32_t bits = k0 < n_keys && node[b] >= 0 ? mask[node[b]][k0 / KB] >> (4 * hh) : 0u;
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int k = 8 * (r >> 2) + (r & 3);
+                    s[b][r] = bits >> k & 1 ? s[b][r] + wrong[k0 + k + 4 * hh] : -INFINITY;
+                }
+            }
+        } else if (k0 + KB > n_keys) {
+            __asm__ volatile("");
+#pragma unroll
+            for (int b = 0; b < RB; b++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[b][r] = k0 + 8 * (r >> 2) + 4 * hh + (r & 3) < n_keys ? s[b][r] : -INFINITY;
+        }
+    };
+    float mt[RB];  // the rows' greatest scores of the tile
+    auto maxima = [&]() {
+#pragma unroll
+        for (int b = 0; b < RB; b++) {
+            mt[b] = s[b][0];
+#pragma unroll
+            for (int r = 1; r < 16; r++) mt[b] = fmaxf(mt[b], s[b][r]);
+        }
+    };
+    float fs[RB];  // the factor of the scores in s
+
+    // turn 0's K and V, turn 1's K
+    if (draft) {
+        drafted(sk, 0);
+        drafted(sv, 0);
     }
-    sk.load(rk, at_round(0), tg);
-    sv.load(rv, at_round(0), tg);
-    if (draft) drafted(0);
     if constexpr (F32) {
-        note(0, sk.most(), sv.most());
-        sync();
-        rescale(0);
-        sync();
-        if (leader) greatest[0] = greatest[1] = 0;
+        note(0, 0, sk.most(), xk);
+        note(0, 1, sv.most(), xv);
+        __syncthreads();
+        rescale_k(0);
+        rescale_v(0);
     }
     store_k(0);
     store_v(0);
     sk.load(rk, at_round(1), tg);
     sv.load(rv, at_round(1), tg);
+    if (draft) drafted(sk, 1);
+    if constexpr (F32) note(1, 0, sk.most(), xk);
+    store_k(1);
+    sk.load(rk, at_round(2), tg);
+    __syncthreads();
+    if (F32 && tid < 2) greatest[tid] = 0;
+    scores(0);
+    masked(0);
+    maxima();
+#pragma unroll
+    for (int b = 0; b < RB; b++) fs[b] = factor[b];
     for (int it = 0; it < rounds; it++) {
-        const int k0 = (int)at_round(it);
-        sync();
+        __syncthreads();
         if constexpr (F32) {
-            if (leader) greatest[2 * ((it + 2) & 3)] = greatest[2 * ((it + 2) & 3) + 1] = 0;
-            const uint2 g = *reinterpret_cast<const uint2 *>(greatest + 2 * (it & 3));
-            if (__builtin_amdgcn_readfirstlane(g.x | g.y)) {  // the tile was stored beyond its scales: once more
-                rescale(it);
-                sk.load(rk, at_round(it), tg);
-                sv.load(rv, at_round(it), tg);
-                if (draft) drafted(it);
-                sync();
-                store_k(it);
-                store_v(it);
+            // noted in the last turn: K of turn it + 1, V of turn it
+            if (tid == 0) greatest[2 * ((it + 3) & 3)] = greatest[2 * ((it + 2) & 3) + 1] = 0;
+            const unsigned nk = greatest[2 * ((it + 1) & 3)], nv = greatest[2 * (it & 3) + 1];
+            if (__builtin_amdgcn_readfirstlane(nk)) {  // stored beyond its scale: once more
+                rescale_k(it + 1);
                 sk.load(rk, at_round(it + 1), tg);
+                if (draft) drafted(sk, it + 1);
+                __syncthreads();
+                store_k(it + 1);
+                sk.load(rk, at_round(it + 2), tg);
+                __syncthreads();
+            }
+            if (__builtin_amdgcn_readfirstlane(nv)) {
+                rescale_v(it);
+                sv.load(rv, at_round(it), tg);
+                if (draft) drafted(sv, it);
+                __syncthreads();
+                store_v(it);
                 sv.load(rv, at_round(it + 1), tg);
-                sync();
+                __syncthreads();
             }
         }
-        const uint16_t *const kt = tiles + (it & (BUFS - 1)) * L::TILE, *const vt = kt + NP * L::KPLANE;
-        const float *const bad = bads + (it & (BUFS - 1)) * 32;
-        float mk = 0.0f, mv = 0.0f;
-        // the next tile's rows into the other buffer and the one after it on its way
-        if constexpr (BUFS == 2) {
-            if (draft) drafted(it + 1);
-        }
-        f32x16 s = f32x16{};
-        {
-            const uint16_t *kr = kt + ql * KS + 8 * hh;
+        // a row whose scores pass its maximum too far: all that it has, down by the difference of two whole numbers
+        float mu[RB];
+        bool far = false;
 #pragma unroll
-            for (int i = 0; i < NS; i++) {
-                const f16x8 k = *reinterpret_cast<const f16x8 *>(kr + 16 * i);
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qlo[i], s, 0, 0, 0);
-                if constexpr (F32)
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8 *>(kr + L::KPLANE + 16 * i), qh[i], s, 0, 0, 0);
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[i], s, 0, 0, 0);
+        for (int b = 0; b < RB; b++) {
+            mt[b] = fmaxf(mt[b], __shfl_xor(mt[b], 32)) * fs[b];
+            far |= mt[b] > m[b] + LAG || (mt[b] > -INFINITY && m[b] == -INFINITY);
+        }
+        if (__ballot(far)) {
+#pragma unroll
+            for (int b = 0; b < RB; b++) {
+                const float up_to = mt[b] > m[b] + LAG || m[b] == -INFINITY ? ceilf(mt[b]) : m[b];
+                const int down = m[b] == -INFINITY ? -300 : (int)fmaxf(m[b] - up_to, -300.0f);
+                m[b] = up_to;
+                l[b] = ldexpf(l[b], down);
+#pragma unroll
+                for (int d = 0; d < ND; d++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[b][d][e] = ldexpf(o[b][d][e], down);
             }
         }
-        if constexpr (BUFS == 2) {
-            if constexpr (F32) mk = sk.most();
-            store_k(it + 1);
-            sk.load(rk, at_round(it + 2), tg);
-        }
-        // register r: position 8 (r / 4) + 4 hh + r % 4 of the tile
-        if (draft) {
-            __asm__ volatile("");  // (a branch: not worth a select per score)
-            const uint32_t bits = k0 < n_keys ? sees[k0 / KB] >> (4 * hh) : 0u;
+        f32x16 sc[RB];
+        float fc[RB];
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int k = 8 * (r >> 2) + (r & 3);
-                s[r] = bits >> k & 1 ? s[r] + bad[k + 4 * hh] : -INFINITY;
+        for (int b = 0; b < RB; b++) {
+            sc[b] = s[b];
+            fc[b] = fs[b];
+            fs[b] = factor[b];
+            mu[b] = P_BITS - (m[b] == -INFINITY ? 0.0f : m[b]);  // nothing seen yet: every weight is 0
+        }
+        scores(it + 1);
+        u32x4 ph[RB][2], pl[RB][2];
+#pragma unroll
+        for (int b = 0; b < RB; b++) {
+            float ls = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][2 * j], fc[b], mu[b]));
+                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][2 * j + 1], fc[b], mu[b]));
+                ls += x + y;
+                uint32_t h0, l0;
+                split2(x, y, h0, l0);
+                ph[b][j / 4][j % 4] = h0;
+                pl[b][j / 4][j % 4] = l0;
             }
-        } else if (k0 + KB > n_keys) {
-            __asm__ volatile("");
-#pragma unroll
-            for (int r = 0; r < 16; r++) s[r] = k0 + 8 * (r >> 2) + 4 * hh + (r & 3) < n_keys ? s[r] : -INFINITY;
+            l[b] += ls;
         }
-        float mt = s[0];
+        // (made here, beside the products: not after the branch)
 #pragma unroll
-        for (int r = 1; r < 16; r++) mt = fmaxf(mt, s[r]);
-        mt = fmaxf(mt, __shfl_xor(mt, 32));
-        const float m_new = fmaxf(m, ceilf(mt * factor));
-        const float mu = m_new == -INFINITY ? 0.0f : m_new;  // nothing seen yet: every weight is 0
-        float p[16], ls = 0.0f;
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-            p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], factor, P_BITS - mu));
-            ls += p[r];
-        }
-        // exact: both maxima are whole
-        const int down = m == -INFINITY ? -300 : (int)fmaxf(m - mu, -300.0f);
-        l = ldexpf(l, down) + ls;
-        m = m_new;
-        if (__ballot(down != 0)) {
-#pragma unroll
-            for (int d = 0; d < ND; d++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) o[d][e] = ldexpf(o[d][e], down);
-        }
+        for (int b = 0; b < RB; b++) __asm__ volatile("" : "+v"(ph[b][0]), "+v"(ph[b][1]), "+v"(pl[b][0]), "+v"(pl[b][1]));
+        masked(it + 1);
         // step u: positions 16 u + 4 hh .. + 3 and 16 u + 8 + 4 hh .. + 3 of the tile, the scores' registers 8 u ..
+        const uint16_t *const vt = tiles + 2 * NP * L::KPLANE + (it & 1) * NP * L::VPLANE;
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            u32x4 h, w;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                uint32_t h0, l0;
-                split2(p[8 * u + 2 * j], p[8 * u + 2 * j + 1], h0, l0);
-                h[j] = h0;
-                w[j] = l0;
-            }
-            const f16x8 ph = __builtin_bit_cast(f16x8, h), pl = __builtin_bit_cast(f16x8, w);
             // V^T by transposing reads: 16 lanes give the addresses of 4 rows x 16 dims (4 each) and get a dim's 4 rows
             auto vread = [&](int plane, int d) {
                 const uint16_t *at = vt + plane * L::VPLANE + (16 * u + 4 * hh + ((lane & 15) >> 2)) * VS + 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
@@ -473,62 +539,61 @@ __global__ __launch_bounds__(64 * RW * KW) void k_tree_part(TreeArgs A) {
 #pragma unroll
             for (int d = 0; d < ND; d++) {
                 const f16x8 v = vread(0, d);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[d], 0, 0, 0);
-                if constexpr (F32) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vread(1, d), ph, o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[d], 0, 0, 0);
+#pragma unroll
+                for (int b = 0; b < RB; b++) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(f16x8, pl[b][u]), o[b][d], 0, 0, 0);
+                if constexpr (F32) {
+                    const f16x8 v2 = vread(1, d);
+#pragma unroll
+                    for (int b = 0; b < RB; b++) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v2, __builtin_bit_cast(f16x8, ph[b][u]), o[b][d], 0, 0, 0);
+                }
+#pragma unroll
+                for (int b = 0; b < RB; b++) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(f16x8, ph[b][u]), o[b][d], 0, 0, 0);
             }
         }
-        if constexpr (BUFS == 1) {
-            sync();
-            if (draft) drafted(it + 1);
-            if constexpr (F32) mk = sk.most();
-            store_k(it + 1);
-            sk.load(rk, at_round(it + 2), tg);
+        maxima();
+        // K of turn it + 2 and V of turn it + 1 into the other buffers, the next ones on their way
+        if (draft) {
+            drafted(sk, it + 2);
+            drafted(sv, it + 1);
         }
-        if constexpr (F32) mv = sv.most();
+        float mk = 0.0f, mv = 0.0f;
+        if constexpr (F32) mk = sk.most(), mv = sv.most();
+        store_k(it + 2);
         store_v(it + 1);
+        sk.load(rk, at_round(it + 3), tg);
         sv.load(rv, at_round(it + 2), tg);
-        if constexpr (F32) note(it + 1, mk, mv);
+        if constexpr (F32) {
+            note(it + 2, 0, mk, xk);
+            note(it + 1, 1, mv, xv);
+        }
     }
-    l += __shfl_xor(l, 32);
-    if constexpr (F32) {
-#pragma unroll
-        for (int d = 0; d < ND; d++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) o[d][e] = ldexpf(o[d][e], xv - TOP);
-    }
-
     const long all = (long)a.n_kv_head * A.rows;
     float *const po = A.part + ((long)part * all + (long)g * A.rows) * HD;
     float *const pm = A.part + (long)(1 + A.n_span) * all * HD + 2 * ((long)part * all + (long)g * A.rows);
-    if constexpr (KW == 1) {
-        if (live) {
+    float *const om = reinterpret_cast<float *>(lds_bytes), *const ml = om + KW * L::ROWS * L::OS;
+    if constexpr (KW > 1) __syncthreads();  // (the tiles are read no more)
 #pragma unroll
-            for (int d = 0; d < ND; d++)
-#pragma unroll
-                for (int b = 0; b < 4; b++)
-                    *reinterpret_cast<float4 *>(po + (long)row * HD + 32 * d + 8 * b + 4 * hh) =
-                        make_float4(o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]);
-            if (hh == 0) *reinterpret_cast<float2 *>(pm + 2 * row) = make_float2(m, l);
-        }
-    } else {
-        // the groups' (m, l, O) in group order
-        constexpr int ROWS = 32 * RW, OS = L::OS;
-        float *const om = reinterpret_cast<float *>(lds_bytes), *const ml = om + KW * ROWS * OS;
-        __syncthreads();
-        const int lr = rw * 32 + ql;
+    for (int b = 0; b < RB; b++) {
+        const int row = row0 + 32 * b, lr = rw * 32 * RB + 32 * b + ql;
+        l[b] += __shfl_xor(l[b], 32);
+        float *const to = KW == 1 ? po + (long)row * HD : om + (kw * L::ROWS + lr) * L::OS;
+        float *const tm = KW == 1 ? pm + 2 * row : ml + 2 * (kw * L::ROWS + lr);
+        if (KW == 1 && row >= A.rows) continue;
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
-            for (int b = 0; b < 4; b++)
-                *reinterpret_cast<float4 *>(om + (kw * ROWS + lr) * OS + 32 * d + 8 * b + 4 * hh) =
-                    make_float4(o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]);
-        if (hh == 0) {
-            ml[2 * (kw * ROWS + lr)] = m;
-            ml[2 * (kw * ROWS + lr) + 1] = l;
-        }
+            for (int e = 0; e < 4; e++) {
+                float4 x = make_float4(o[b][d][4 * e], o[b][d][4 * e + 1], o[b][d][4 * e + 2], o[b][d][4 * e + 3]);
+                if constexpr (F32) x = make_float4(ldexpf(x.x, xv - TOP), ldexpf(x.y, xv - TOP), ldexpf(x.z, xv - TOP), ldexpf(x.w, xv - TOP));
+                *reinterpret_cast<float4 *>(to + 32 * d + 8 * e + 4 * hh) = x;
+            }
+        if (hh == 0) *reinterpret_cast<float2 *>(tm) = make_float2(m[b], l[b]);
+    }
+    if constexpr (KW > 1) {
+        // the groups' (m, l, O) in group order
+        constexpr int ROWS = L::ROWS, OS = L::OS;
         __syncthreads();
-        for (int i = tid; i < ROWS * HD / 4; i += 64 * RW * KW) {
+        for (int i = tid; i < ROWS * HD / 4; i += 256) {
             const int r = i / (HD / 4), c = 4 * (i - r * (HD / 4)), gr = block * ROWS + r;
             if (gr >= A.rows) continue;
             float M = -INFINITY, ls = 0.0f;
@@ -603,17 +668,19 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs A) {
 
 // How the work is split, from the sizes alone.
 struct Plan {
-    int rw, kw, rows, n_block, n_span;
+    int rb, rw, kw, rows, n_block, n_span;
 };
 Plan plan_of(int n_tok, int n_head, int n_kv_head, int hd, int max_past) {
     Plan p;
     p.rows = n_tok * (n_head / n_kv_head);
-    p.rw = p.rows <= 32 && hd < 256 ? 1 : p.rows <= 64 ? 2 : 4;
+    p.rb = hd < 256 && p.rows > 64 ? 2 : 1;
+    p.rw = hd == 256 || p.rows > 128 ? 4 : 2;
     p.kw = 4 / p.rw;
-    p.n_block = (p.rows + 32 * p.rw - 1) / (32 * p.rw);
+    const int block = 32 * p.rb * p.rw;
+    p.n_block = (p.rows + block - 1) / block;
     const int granule = KB * p.kw;
     const long pairs = (long)n_kv_head * p.n_block, rounds = ((long)max_past + granule - 1) / granule;
-    long n = (512 - pairs) / pairs;
+    long n = (256 - pairs) / pairs;
     if (n > rounds) n = rounds;
     if (n > MAX_PARTS - 1) n = MAX_PARTS - 1;
     // a span's bytes (at most 2^31 - 1 for a buffer resource)
@@ -623,29 +690,29 @@ Plan plan_of(int n_tok, int n_head, int n_kv_head, int hd, int max_past) {
     return p;
 }
 
-template <int HD, class KT, int RW, int KW>
+template <int HD, class KT, int RB, int RW, int KW>
 int launch_part(const TreeArgs &A, hipStream_t st) {
     static size_t granted = 0;
-    const void *fn = (const void *)k_tree_part<HD, KT, RW, KW>;
-    const int rc = sdy_lds_limit(fn, Lds<HD, KT, RW, KW>::bytes, &granted);
+    const void *fn = (const void *)k_tree_part<HD, KT, RB, RW, KW>;
+    const int rc = sdy_lds_limit(fn, Lds<HD, KT, RB, RW, KW>::bytes, &granted);
     if (rc) return rc;
-    SDY_NOTE_KERNEL((k_tree_part<HD, KT, RW, KW>));
+    SDY_NOTE_KERNEL((k_tree_part<HD, KT, RB, RW, KW>));
     const long pairs = (long)(1 + A.n_span) * A.a.n_kv_head;
-    hipLaunchKernelGGL((k_tree_part<HD, KT, RW, KW>), dim3((unsigned)((pairs + 7) / 8 * 8 * A.n_block)), dim3(64 * RW * KW),
-                       (Lds<HD, KT, RW, KW>::bytes), st, A);
+    hipLaunchKernelGGL((k_tree_part<HD, KT, RB, RW, KW>), dim3((unsigned)((pairs + 7) / 8 * 8 * A.n_block)), dim3(256),
+                       (Lds<HD, KT, RB, RW, KW>::bytes), st, A);
     return sdy_check_launch("attn_tree");
 }
 
 template <int HD, class KT>
-int launch_rows(const TreeArgs &A, int rw, hipStream_t st) {
-    if constexpr (HD < 256)
-        if (rw == 1) return launch_part<HD, KT, 1, 4>(A, st);
-    return rw == 2 ? launch_part<HD, KT, 2, 2>(A, st) : launch_part<HD, KT, 4, 1>(A, st);
+int launch_rows(const TreeArgs &A, const Plan &p, hipStream_t st) {
+    if constexpr (HD == 256) return launch_part<HD, KT, 1, 4, 1>(A, st);
+    else if (p.rw == 4) return launch_part<HD, KT, 2, 4, 1>(A, st);
+    else return p.rb == 2 ? launch_part<HD, KT, 2, 2, 2>(A, st) : launch_part<HD, KT, 1, 2, 2>(A, st);
 }
 
 template <int HD>
-int launch_tree(const TreeArgs &A, int rw, hipStream_t st) {
-    const int rc = A.a.kv_type == SDY_KV_F16 ? launch_rows<HD, uint16_t>(A, rw, st) : launch_rows<HD, float>(A, rw, st);
+int launch_tree(const TreeArgs &A, const Plan &p, hipStream_t st) {
+    const int rc = A.a.kv_type == SDY_KV_F16 ? launch_rows<HD, uint16_t>(A, p, st) : launch_rows<HD, float>(A, p, st);
     if (rc) return rc;
     hipLaunchKernelGGL(k_tree_merge<HD>, dim3(A.a.n_tok, A.a.n_head), dim3(256), 0, st, A);
     return sdy_check_launch("attn_tree merge");
@@ -696,5 +763,5 @@ extern "C" int sdy_attn_tree(const sdy_attn_tree_args *a, sdy_stream s) {
     A.log_scale = (float)(1.4426950408889634074 / sqrt((double)a->hd));
     A.part = a->part;
     hipStream_t st = (hipStream_t)s;
-    return a->hd == 64 ? launch_tree<64>(A, p.rw, st) : a->hd == 128 ? launch_tree<128>(A, p.rw, st) : launch_tree<256>(A, p.rw, st);
+    return a->hd == 64 ? launch_tree<64>(A, p, st) : a->hd == 128 ? launch_tree<128>(A, p, st) : launch_tree<256>(A, p, st);
 }
