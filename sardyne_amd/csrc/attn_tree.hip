@@ -15,9 +15,9 @@
 // Products on the f16 matrix cores at f32's precision: an f32 is the sum of two f16 (22 bits and a sign) once it is scaled by
 // a power of two that keeps it well inside f16's range. q, P and an f32 cache's K and V are split so, an f16 cache's values are
 // taken as they are; of the split products low x low, at most 2^-22 of the whole, is left out. A row of q goes by its own
-// greatest value; a span's K and V by the greatest met so far, brought to 2^13 .. 2^16 (f16's least bit is then 2^-38 of it),
-// a power that changes with the first tile and seldom after. Powers of two go back exactly: K's and q's into the scores'
-// factor, V's into O (ldexp). The running maximum m is kept as a whole number, so that its rescales are exact too, and grows
+// greatest value. A span's K and V go by fixed powers, which suit a greatest value of 2^-5 to 2^10 (K) or 2^-9 to 2^6 (V): its
+// low part's least bit is then 2^-24 of it or less; a span outside of that is computed again with its own powers. Powers of
+// two go back exactly: K's and q's into the scores' factor, V's into O (ldexp). The running maximum m is kept as a whole number, so that its rescales are exact too, and grows
 // only when a score passes it by 2^LAG: P is 2^4 to 2^15 at the greatest weight, f16's least bit 2^-28 of it or less.
 #include <type_traits>
 
@@ -39,7 +39,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int MAX_NODES = 256;
 constexpr int KB = 32;         // positions per tile
-constexpr int TOP = 13;        // the greatest value is scaled to 2^TOP .. 2^(TOP + 1), later ones up to 2^(TOP + 3)
+constexpr int TOP = 13;        // a row of q, and a span computed again, are scaled to a greatest value of 2^TOP .. 2^(TOP + 1)
+constexpr int K_SCALE = 5, V_SCALE = 9;  // the powers that K and V are scaled by at first
 constexpr float P_BITS = 4;    // P is 2^P_BITS exp2(score - m), of scores up to m + LAG
 constexpr float LAG = 11;
 constexpr int MAX_PARTS = 513;
@@ -76,9 +77,9 @@ struct Lds {
     static constexpr int ROWS = 32 * RB * RW, OS = HD + 4;
     static constexpr size_t merge = KW > 1 ? (size_t)KW * ROWS * (OS + 2) * 4 : 0;
     static constexpr size_t body = tiles > merge ? tiles : merge;
-    // the nodes' masks, their farthest known ancestors, and what is wrong with their rows
-    static constexpr size_t masks = MAX_NODES * (MAX_NODES / 32) * 4 + MAX_NODES * 2 + MAX_NODES * 4;
-    static constexpr size_t flags = 2 * 4 * 4;  // the greatest |K| and |V| of four tiles
+    // the nodes' masks and their farthest known ancestors; per 32 nodes, those with rows that hold (ok) and that do not (bad)
+    static constexpr size_t masks = MAX_NODES * (MAX_NODES / 32) * 4 + MAX_NODES * 2 + 2 * 16 * 4;
+    static constexpr size_t flags = 2 * 4;      // the greatest |K| and |V|
     static constexpr size_t bytes = body + masks + flags;
     static_assert(bytes <= 160 * 1024, "fits a CU");
 };
@@ -99,13 +100,12 @@ SDY_DEV float max3_abs(float m, uint32_t a, uint32_t b) {
     return m;
 }
 
-// The exponent of a greatest |value|, from 2^-100 on (smaller ones count as that), and the power of two that brings it to
-// 2^TOP. An infinity or a NaN stays one.
-SDY_DEV int exp_of(float most) {
+// The power of two that brings a greatest |value| (one of at least 2^-100) to 2^TOP .. 2^(TOP + 1)
+SDY_DEV int power_for(float most) {
     const int e = (int)(__float_as_uint(most) >> 23) - 127;
-    return e > -100 ? e : -100;
+    return TOP - (e > -100 ? e : -100);
 }
-SDY_DEV float exp_scale(int e) { return __uint_as_float((uint32_t)(127 + TOP - e) << 23); }
+SDY_DEV float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 // Rows of K and V on their way to LDS: thread tg of a group of 64 RW holds chunks of CE consecutive elements of one row.
 template <int HD, class KT, int RW>
@@ -134,19 +134,17 @@ struct Stage {
             }
         }
     }
-    // Whether this row (of LPR threads) has an infinity or a NaN
-    SDY_DEV bool unfit() const {
-        uint32_t any = 0;
+    // 0, or NaN where this thread's values have an infinity or a NaN
+    SDY_DEV float zeros() const {
+        float z = 0.0f;
 #pragma unroll
         for (int i = 0; i < NC; i++)
 #pragma unroll
             for (int w = 0; w < W; w++) {
-                if constexpr (F32) any |= (r[i][w] & 0x7F800000u) == 0x7F800000u;
-                else any |= (r[i][w] & 0x7C00u) == 0x7C00u || (r[i][w] & 0x7C000000u) == 0x7C000000u;
+                if constexpr (F32) z = __builtin_fmaf(__uint_as_float(r[i][w]), 0.0f, z);
+                else z = __builtin_fmaf(sdy_h2f((uint16_t)r[i][w]), 0.0f, __builtin_fmaf(sdy_h2f((uint16_t)(r[i][w] >> 16)), 0.0f, z));
             }
-#pragma unroll
-        for (int off = 1; off < LPR; off *= 2) any |= (uint32_t)__shfl_xor((int)any, off);
-        return any != 0;
+        return z;
     }
     SDY_DEV void clear() {
 #pragma unroll
@@ -154,9 +152,8 @@ struct Stage {
 #pragma unroll
             for (int w = 0; w < W; w++) r[i][w] = 0;
     }
-    // The greatest |value| of this thread's
-    SDY_DEV float most() const {
-        float m = 0.0f;
+    // The greatest |value| of this thread's, or m
+    SDY_DEV float most(float m) const {
 #pragma unroll
         for (int i = 0; i < NC; i++)
 #pragma unroll
@@ -186,11 +183,10 @@ struct Stage {
 };
 
 // Which nodes each node sees, as bits: mask[t] starts as t itself, then takes that of the farthest node known above it and
-// that one's farthest in turn, doubling the distance. All 256 threads.
-SDY_DEV void ancestor_masks(const int32_t *parent, int n, uint32_t (*mask)[MAX_NODES / 32], int16_t *up) {
+// that one's farthest in turn, doubling the distance. All 256 threads; p0 is the parent of node tid.
+SDY_DEV void ancestor_masks(int p0, int n, uint32_t (*mask)[MAX_NODES / 32], int16_t *up) {
     constexpr int W = MAX_NODES / 32;
     const int tid = threadIdx.x, words = (n + 31) / 32;
-    const int p0 = tid < n ? parent[tid] : -2;
     up[tid] = (int16_t)(p0 < -1 ? -2 : p0 < 0 || p0 >= tid ? -1 : p0);
 #pragma unroll
     for (int w = 0; w < W; w++) mask[tid][w] = p0 >= -1 && w == tid / 32 ? 1u << (tid % 32) : 0u;
@@ -226,8 +222,6 @@ __global__ __launch_bounds__(256, 1) void k_tree_part(TreeArgs A) {
     constexpr int NP = L::NP, KS = L::KS, VS = L::VS, ND = HD / 32, NS = HD / 16, GROUP = 64 * RW;
     extern __shared__ __align__(16) unsigned char lds_bytes[];
     const sdy_attn_tree_args &a = A.a;
-    const int past = *a.n_past;
-    if (past < 0 || past > a.max_past) return;
     // all row blocks of one span and kv head on one XCD (workgroups are dealt to the 8 in turn): its L2 holds the tile
     const int pairs = (1 + A.n_span) * a.n_kv_head;
     const int id = (int)blockIdx.x, pair = (id / 8 / A.n_block) * 8 + id % 8, block = id / 8 % A.n_block;
@@ -236,35 +230,9 @@ __global__ __launch_bounds__(256, 1) void k_tree_part(TreeArgs A) {
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, ql = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rw = wave % RW, kw = wave / RW, tg = tid - kw * GROUP;
     const bool draft = part == 0;
-    int lo = 0, hi = a.n_tok;
-    if (!draft) {
-        const int per = span_rounds(A, past) * A.granule;
-        const long l0 = (long)(part - 1) * per, h0 = l0 + per;
-        if (l0 >= past) return;  // the merge does not look at it
-        lo = (int)l0;
-        hi = h0 < past ? (int)h0 : past;
-    }
-
-    const size_t elt = sizeof(KT);
-    const char *kbase = (const char *)(draft ? a.k_draft : a.k_cache) + ((size_t)g * (draft ? a.draft_stride : a.head_stride) + (size_t)lo * HD) * elt;
-    const char *vbase = (const char *)(draft ? a.v_draft : a.v_cache) + ((size_t)g * (draft ? a.draft_stride : a.head_stride) + (size_t)lo * HD) * elt;
-    const int n_keys = hi - lo, size = n_keys * (int)(HD * sizeof(KT));  // (a span's bytes fit 31 bits: the host sees to it)
-    // positions past the span's end read as zeros and are masked below
-    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void *)kbase, (short)0, size, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void *)vbase, (short)0, size, 0x00020000);
-    const int rounds = (n_keys + KB * KW - 1) / (KB * KW);
-    auto at_round = [&](int it) { return (uint32_t)((it * KW + kw) * KB); };  // the group's first position in the span
-    St sk, sv;
-    sk.load(rk, at_round(0), tg);
-    sv.load(rv, at_round(0), tg);
-
     const int rep = a.n_head / a.n_kv_head;
     const int row0 = (block * RW + rw) * 32 * RB + ql;  // and 32 further on
-    uint16_t *const tiles = reinterpret_cast<uint16_t *>(lds_bytes) + kw * 2 * L::TILE;
-    uint32_t(*const mask)[MAX_NODES / 32] = reinterpret_cast<uint32_t(*)[MAX_NODES / 32]>(lds_bytes + L::body);
-    int16_t *const up = reinterpret_cast<int16_t *>(mask + MAX_NODES);
-    float *const wrong = reinterpret_cast<float *>(up + MAX_NODES);  // 0, NaN (an infinity or a NaN in its rows), inf (no node)
-    unsigned *const greatest = reinterpret_cast<unsigned *>(wrong + MAX_NODES);
+    const int p0 = draft && tid < a.n_tok ? a.parent[tid] : -2;
 
     // the rows' queries: step i holds dims 16 i + 8 hh .. + 7
     f16x8 qh[RB][NS], qlo[RB][NS];
@@ -288,9 +256,8 @@ __global__ __launch_bounds__(256, 1) void k_tree_part(TreeArgs A) {
             most = max3_abs(most, __float_as_uint(v[i].z), __float_as_uint(v[i].w));
         }
         most = fmaxf(most, __shfl_xor(most, 32));
-        const int e0 = exp_of(most);
-        const float sc = exp_scale(e0);
-        eq[b] = e0 - TOP;
+        eq[b] = power_for(most);
+        const float sc = pow2(eq[b]);
 #pragma unroll
         for (int i = 0; i < NS; i++) {
             u32x4 h, l;
@@ -307,265 +274,240 @@ __global__ __launch_bounds__(256, 1) void k_tree_part(TreeArgs A) {
         }
     }
 
-    f32x16 o[RB][ND];
-    float m[RB], l[RB], factor[RB];  // m whole; the factor of the next scores
-#pragma unroll
-    for (int b = 0; b < RB; b++) {
-#pragma unroll
-        for (int d = 0; d < ND; d++) o[b][d] = f32x16{};
-        m[b] = -INFINITY;
-        l[b] = 0.0f;
-        factor[b] = ldexpf(A.log_scale, eq[b]);
+    const int past = *a.n_past;
+    if (past < 0 || past > a.max_past) return;
+    int lo = 0, hi = a.n_tok;
+    if (!draft) {
+        const int per = span_rounds(A, past) * A.granule;
+        const long l0 = (long)(part - 1) * per, h0 = l0 + per;
+        if (l0 >= past) return;  // the merge does not look at it
+        lo = (int)l0;
+        hi = h0 < past ? (int)h0 : past;
     }
-    int xk = F32 ? -101 : TOP, xv = xk;  // the exponents that K's and V's scales go by (none yet for f32)
+    const long from = ((long)g * (draft ? a.draft_stride : a.head_stride) + (long)lo * HD) * (long)sizeof(KT);
+    const int n_keys = hi - lo, size = n_keys * (int)(HD * sizeof(KT));  // (a span's bytes fit 31 bits: the host sees to it)
+    // positions past the span's end read as zeros and are masked below
+    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void *)((const char *)(draft ? a.k_draft : a.k_cache) + from), (short)0, size, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void *)((const char *)(draft ? a.v_draft : a.v_cache) + from), (short)0, size, 0x00020000);
+    const int rounds = (n_keys + KB * KW - 1) / (KB * KW);
+    auto at_round = [&](int it) { return (uint32_t)((it * KW + kw) * KB); };  // the group's first position in the span
 
-    // Drafted rows: which nodes see which, and rows that are left out (an empty place's) or would be all that a tile's other
-    // rows are read by (with an infinity or a NaN: NaN for those that see them, nothing for the others).
+    uint16_t *const tiles = reinterpret_cast<uint16_t *>(lds_bytes) + kw * 2 * L::TILE;
+    uint32_t(*const mask)[MAX_NODES / 32] = reinterpret_cast<uint32_t(*)[MAX_NODES / 32]>(lds_bytes + L::body);
+    int16_t *const up = reinterpret_cast<int16_t *>(mask + MAX_NODES);
+    uint32_t *const ok = reinterpret_cast<uint32_t *>(up + MAX_NODES), *const bad = ok + 16;
+    unsigned *const greatest = bad + 16;
+
+    St sk, sv;
+    // Drafted rows: which nodes see which, and rows that are left out: an empty place's, and those with an infinity or a NaN
+    // (NaN for the nodes that see them, nothing for the others).
     if (draft) {
-        ancestor_masks(a.parent, a.n_tok, mask, up);
+        if (tid < 32) ok[tid] = 0;
+        ancestor_masks(p0, a.n_tok, mask, up);
+#pragma unroll 1
         for (int it = 0; it < rounds; it++) {
-            if (it > 0) {
-                sk.load(rk, at_round(it), tg);
-                sv.load(rv, at_round(it), tg);
-            }
-            const bool uk = sk.unfit(), u = sv.unfit() || uk;
+            sk.load(rk, at_round(it), tg);
+            sv.load(rv, at_round(it), tg);
+            const float z = sk.zeros() + sv.zeros();
             const int t = (int)at_round(it) + tg / St::LPR;
-            if (t < MAX_NODES && tg % St::LPR == 0) wrong[t] = !(mask[t][t / 32] >> (t % 32) & 1) ? INFINITY : u ? NAN : 0.0f;
-        }
-        if (rounds > 1) {
-            sk.load(rk, at_round(0), tg);
-            sv.load(rv, at_round(0), tg);
+            if (t < MAX_NODES && (mask[t][t / 32] >> (t % 32) & 1)) atomicOr(z == 0.0f ? &ok[t / 32] : &bad[t / 32], 1u << (t % 32));
         }
     }
-    if (F32 && tid < 8) greatest[tid] = 0;
-    __syncthreads();
     auto drafted = [&](St &st, int it) {
-        const int t = (int)at_round(it) + tg / St::LPR;
-        if (t >= a.n_tok || !(wrong[t] == 0.0f)) st.clear();
+        const uint32_t t = at_round(it) / KB;
+        if (!((ok[t] & ~bad[t]) >> (tg / St::LPR) & 1)) st.clear();
     };
-    // notes a greatest value for the K (which 0) or V (1) of turn `it` where it is beyond the scale
-    auto note = [&](int it, int which, float most, int x) {
-        if (__ballot(exp_of(most) > x + 2)) {
-            for (int off = 32; off >= 1; off >>= 1) most = fmaxf(most, __shfl_xor(most, off));
-            if (lane == 0) atomicMax(&greatest[2 * (it & 3) + which], __float_as_uint(most));
+
+    f32x16 o[RB][ND];
+    float m[RB], l[RB];  // m whole
+    int pk = F32 ? K_SCALE : 0, pv = F32 ? V_SCALE : 0;  // the powers that K and V are scaled by
+    for (;;) {
+        float factor[RB], greatest_k = 0.0f, greatest_v = 0.0f;
+#pragma unroll
+        for (int b = 0; b < RB; b++) {
+#pragma unroll
+            for (int d = 0; d < ND; d++) o[b][d] = f32x16{};
+            m[b] = -INFINITY;
+            l[b] = 0.0f;
+            factor[b] = ldexpf(A.log_scale, -eq[b] - pk);
         }
-    };
-    auto store_k = [&](int it) { sk.template store<KS>(tiles + (it & 1) * NP * L::KPLANE, exp_scale(xk), tg); };
-    auto store_v = [&](int it) { sv.template store<VS>(tiles + 2 * NP * L::KPLANE + (it & 1) * NP * L::VPLANE, exp_scale(xv), tg); };
-    // a new scale from what was noted for turn `it`
-    auto rescale_k = [&](int it) {
-        const int e = exp_of(__uint_as_float(greatest[2 * (it & 3)]));
-        xk = e > xk ? e : xk;
+        const float fk = pow2(pk), fv = pow2(pv);
+        // K of turn `it` into its buffer, the next one on its way; V
+        auto next_k = [&](int it) {
+            if (draft) drafted(sk, it);
+            if constexpr (F32) greatest_k = sk.most(greatest_k);
+            sk.template store<KS>(tiles + (it & 1) * NP * L::KPLANE, fk, tg);
+            sk.load(rk, at_round(it + 1), tg);
+        };
+        auto next_v = [&](int it) {
+            if (draft) drafted(sv, it);
+            if constexpr (F32) greatest_v = sv.most(greatest_v);
+            sv.template store<VS>(tiles + 2 * NP * L::KPLANE + (it & 1) * NP * L::VPLANE, fv, tg);
+            sv.load(rv, at_round(it + 1), tg);
+        };
+        f32x16 s[RB];
+        float mt[RB];  // the rows' greatest scores of the tile
+        // S^T of turn `it`
+        auto scores = [&](int it) {
+            const uint16_t *kr = tiles + (it & 1) * NP * L::KPLANE + ql * KS + 8 * hh;
 #pragma unroll
-        for (int b = 0; b < RB; b++) factor[b] = ldexpf(A.log_scale, eq[b] + xk - TOP);
-    };
-    auto rescale_v = [&](int it) {
-        const int e = exp_of(__uint_as_float(greatest[2 * (it & 3) + 1])), x = e > xv ? e : xv;
+            for (int b = 0; b < RB; b++) s[b] = f32x16{};
 #pragma unroll
-        for (int b = 0; b < RB; b++)
+            for (int i = 0; i < NS; i++) {
+                const f16x8 k = *reinterpret_cast<const f16x8 *>(kr + 16 * i);
 #pragma unroll
-            for (int d = 0; d < ND; d++)
+                for (int b = 0; b < RB; b++) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qlo[b][i], s[b], 0, 0, 0);
+                if constexpr (F32) {
+                    const f16x8 k2 = *reinterpret_cast<const f16x8 *>(kr + L::KPLANE + 16 * i);
 #pragma unroll
-                for (int e2 = 0; e2 < 16; e2++) o[b][d][e2] = ldexpf(o[b][d][e2], xv - x);
-        xv = x;
-    };
-    f32x16 s[RB];
-    // S^T of turn `it`
-    auto scores = [&](int it) {
-        const uint16_t *kr = tiles + (it & 1) * NP * L::KPLANE + ql * KS + 8 * hh;
+                    for (int b = 0; b < RB; b++) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k2, qh[b][i], s[b], 0, 0, 0);
+                }
 #pragma unroll
-        for (int b = 0; b < RB; b++) s[b] = f32x16{};
-#pragma unroll
-        for (int i = 0; i < NS; i++) {
-            const f16x8 k = *reinterpret_cast<const f16x8 *>(kr + 16 * i);
-#pragma unroll
-            for (int b = 0; b < RB; b++) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qlo[b][i], s[b], 0, 0, 0);
-            if constexpr (F32) {
-                const f16x8 k2 = *reinterpret_cast<const f16x8 *>(kr + L::KPLANE + 16 * i);
-#pragma unroll
-                for (int b = 0; b < RB; b++) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k2, qh[b][i], s[b], 0, 0, 0);
+                for (int b = 0; b < RB; b++) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[b][i], s[b], 0, 0, 0);
             }
-#pragma unroll
-            for (int b = 0; b < RB; b++) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[b][i], s[b], 0, 0, 0);
-        }
-    };
-    // register r of the scores: position 8 (r / 4) + 4 hh + r % 4 of the tile
-    auto masked = [&](int it) {
-        const int k0 = (int)at_round(it);
-        if (draft) {
+        };
+        // what a tile's rows do not see; register r of the scores is position 8 (r / 4) + 4 hh + r % 4 of the tile
+        auto masked = [&](int it) {
+            const int k0 = (int)at_round(it);
+            if (!draft && k0 + KB <= n_keys) return;
             __asm__ volatile("");  // (a branch: not worth a select per score)
+            const uint32_t end = k0 >= n_keys ? 0u : n_keys - k0 >= KB ? ~0u : (1u << (n_keys - k0)) - 1;
 #pragma unroll
             for (int b = 0; b < RB; b++) {
-                const uint32_t bits = k0 < n_keys && node[b] >= 0 ? mask[node[b]][k0 / KB] >> (4 * hh) : 0u;
+                uint32_t bits = end;
+                if (draft) {
+                    bits = k0 < n_keys && node[b] >= 0 ? mask[node[b]][k0 / KB] : 0u;
+                    if (bits & bad[k0 / KB]) l[b] = NAN;
+                }
+                bits >>= 4 * hh;
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    const int k = 8 * (r >> 2) + (r & 3);
-                    s[b][r] = bits >> k & 1 ? s[b][r] + wrong[k0 + k + 4 * hh] : -INFINITY;
+                    const uint32_t see = (uint32_t)__builtin_amdgcn_sbfe((int)bits, 8 * (r >> 2) + (r & 3), 1);
+                    s[b][r] = __uint_as_float((__float_as_uint(s[b][r]) & see) | (0xFF800000u & ~see));
                 }
             }
-        } else if (k0 + KB > n_keys) {
-            __asm__ volatile("");
-#pragma unroll
-            for (int b = 0; b < RB; b++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) s[b][r] = k0 + 8 * (r >> 2) + 4 * hh + (r & 3) < n_keys ? s[b][r] : -INFINITY;
-        }
-    };
-    float mt[RB];  // the rows' greatest scores of the tile
-    auto maxima = [&]() {
-#pragma unroll
-        for (int b = 0; b < RB; b++) {
-            mt[b] = s[b][0];
-#pragma unroll
-            for (int r = 1; r < 16; r++) mt[b] = fmaxf(mt[b], s[b][r]);
-        }
-    };
-    float fs[RB];  // the factor of the scores in s
-
-    // turn 0's K and V, turn 1's K
-    if (draft) {
-        drafted(sk, 0);
-        drafted(sv, 0);
-    }
-    if constexpr (F32) {
-        note(0, 0, sk.most(), xk);
-        note(0, 1, sv.most(), xv);
-        __syncthreads();
-        rescale_k(0);
-        rescale_v(0);
-    }
-    store_k(0);
-    store_v(0);
-    sk.load(rk, at_round(1), tg);
-    sv.load(rv, at_round(1), tg);
-    if (draft) drafted(sk, 1);
-    if constexpr (F32) note(1, 0, sk.most(), xk);
-    store_k(1);
-    sk.load(rk, at_round(2), tg);
-    __syncthreads();
-    if (F32 && tid < 2) greatest[tid] = 0;
-    scores(0);
-    masked(0);
-    maxima();
-#pragma unroll
-    for (int b = 0; b < RB; b++) fs[b] = factor[b];
-    for (int it = 0; it < rounds; it++) {
-        __syncthreads();
-        if constexpr (F32) {
-            // noted in the last turn: K of turn it + 1, V of turn it
-            if (tid == 0) greatest[2 * ((it + 3) & 3)] = greatest[2 * ((it + 2) & 3) + 1] = 0;
-            const unsigned nk = greatest[2 * ((it + 1) & 3)], nv = greatest[2 * (it & 3) + 1];
-            if (__builtin_amdgcn_readfirstlane(nk)) {  // stored beyond its scale: once more
-                rescale_k(it + 1);
-                sk.load(rk, at_round(it + 1), tg);
-                if (draft) drafted(sk, it + 1);
-                __syncthreads();
-                store_k(it + 1);
-                sk.load(rk, at_round(it + 2), tg);
-                __syncthreads();
-            }
-            if (__builtin_amdgcn_readfirstlane(nv)) {
-                rescale_v(it);
-                sv.load(rv, at_round(it), tg);
-                if (draft) drafted(sv, it);
-                __syncthreads();
-                store_v(it);
-                sv.load(rv, at_round(it + 1), tg);
-                __syncthreads();
-            }
-        }
-        // a row whose scores pass its maximum too far: all that it has, down by the difference of two whole numbers
-        float mu[RB];
-        bool far = false;
-#pragma unroll
-        for (int b = 0; b < RB; b++) {
-            mt[b] = fmaxf(mt[b], __shfl_xor(mt[b], 32)) * fs[b];
-            far |= mt[b] > m[b] + LAG || (mt[b] > -INFINITY && m[b] == -INFINITY);
-        }
-        if (__ballot(far)) {
+        };
+        auto maxima = [&]() {
 #pragma unroll
             for (int b = 0; b < RB; b++) {
-                const float up_to = mt[b] > m[b] + LAG || m[b] == -INFINITY ? ceilf(mt[b]) : m[b];
-                const int down = m[b] == -INFINITY ? -300 : (int)fmaxf(m[b] - up_to, -300.0f);
-                m[b] = up_to;
-                l[b] = ldexpf(l[b], down);
+                mt[b] = s[b][0];
 #pragma unroll
-                for (int d = 0; d < ND; d++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) o[b][d][e] = ldexpf(o[b][d][e], down);
+                for (int r = 1; r < 16; r++) mt[b] = fmaxf(mt[b], s[b][r]);
             }
-        }
-        f32x16 sc[RB];
-        float fc[RB];
-#pragma unroll
-        for (int b = 0; b < RB; b++) {
-            sc[b] = s[b];
-            fc[b] = fs[b];
-            fs[b] = factor[b];
-            mu[b] = P_BITS - (m[b] == -INFINITY ? 0.0f : m[b]);  // nothing seen yet: every weight is 0
-        }
-        scores(it + 1);
-        u32x4 ph[RB][2], pl[RB][2];
-#pragma unroll
-        for (int b = 0; b < RB; b++) {
-            float ls = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][2 * j], fc[b], mu[b]));
-                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][2 * j + 1], fc[b], mu[b]));
-                ls += x + y;
-                uint32_t h0, l0;
-                split2(x, y, h0, l0);
-                ph[b][j / 4][j % 4] = h0;
-                pl[b][j / 4][j % 4] = l0;
-            }
-            l[b] += ls;
-        }
-        // (made here, beside the products: not after the branch)
-#pragma unroll
-        for (int b = 0; b < RB; b++) __asm__ volatile("" : "+v"(ph[b][0]), "+v"(ph[b][1]), "+v"(pl[b][0]), "+v"(pl[b][1]));
-        masked(it + 1);
-        // step u: positions 16 u + 4 hh .. + 3 and 16 u + 8 + 4 hh .. + 3 of the tile, the scores' registers 8 u ..
-        const uint16_t *const vt = tiles + 2 * NP * L::KPLANE + (it & 1) * NP * L::VPLANE;
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            // V^T by transposing reads: 16 lanes give the addresses of 4 rows x 16 dims (4 each) and get a dim's 4 rows
-            auto vread = [&](int plane, int d) {
-                const uint16_t *at = vt + plane * L::VPLANE + (16 * u + 4 * hh + ((lane & 15) >> 2)) * VS + 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at);
-                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(at + 8 * VS));
-                return __builtin_bit_cast(f16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-            };
-#pragma unroll
-            for (int d = 0; d < ND; d++) {
-                const f16x8 v = vread(0, d);
-#pragma unroll
-                for (int b = 0; b < RB; b++) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(f16x8, pl[b][u]), o[b][d], 0, 0, 0);
-                if constexpr (F32) {
-                    const f16x8 v2 = vread(1, d);
-#pragma unroll
-                    for (int b = 0; b < RB; b++) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v2, __builtin_bit_cast(f16x8, ph[b][u]), o[b][d], 0, 0, 0);
-                }
-#pragma unroll
-                for (int b = 0; b < RB; b++) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(f16x8, ph[b][u]), o[b][d], 0, 0, 0);
-            }
-        }
+        };
+        __syncthreads();
+        sk.load(rk, at_round(0), tg);
+        sv.load(rv, at_round(0), tg);
+#pragma unroll 1
+        for (int it = 0; it < 2; it++) next_k(it);
+        next_v(0);
+        __syncthreads();
+        scores(0);
+        masked(0);
         maxima();
-        // K of turn it + 2 and V of turn it + 1 into the other buffers, the next ones on their way
-        if (draft) {
-            drafted(sk, it + 2);
-            drafted(sv, it + 1);
+#pragma unroll 1
+        for (int it = 0; it < rounds; it++) {
+            __syncthreads();
+            // a row whose scores pass its maximum too far: all that it has, down by the difference of two whole numbers
+            float mu[RB];
+            bool far = false;
+#pragma unroll
+            for (int b = 0; b < RB; b++) {
+                mt[b] = fmaxf(mt[b], __shfl_xor(mt[b], 32)) * factor[b];
+                far |= mt[b] > m[b] + LAG || (mt[b] > -INFINITY && m[b] == -INFINITY);
+            }
+            if (__ballot(far)) {
+#pragma unroll
+                for (int b = 0; b < RB; b++) {
+                    const float up_to = mt[b] > m[b] + LAG || m[b] == -INFINITY ? ceilf(mt[b]) : m[b];
+                    const int down = m[b] == -INFINITY ? -300 : (int)fmaxf(m[b] - up_to, -300.0f);
+                    m[b] = up_to;
+                    l[b] = ldexpf(l[b], down);
+                    if (it > 0) {
+#pragma unroll
+                        for (int d = 0; d < ND; d++)
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[b][d][e] = ldexpf(o[b][d][e], down);
+                    }
+                }
+            }
+            f32x16 sc[RB];
+#pragma unroll
+            for (int b = 0; b < RB; b++) {
+                sc[b] = s[b];
+                mu[b] = P_BITS - (m[b] == -INFINITY ? 0.0f : m[b]);  // nothing seen yet: every weight is 0
+            }
+            scores(it + 1);
+            u32x4 ph[RB][2], pl[RB][2];
+#pragma unroll
+            for (int b = 0; b < RB; b++) {
+                float ls = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][2 * j], factor[b], mu[b]));
+                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][2 * j + 1], factor[b], mu[b]));
+                    ls += x + y;
+                    uint32_t h0, l0;
+                    split2(x, y, h0, l0);
+                    ph[b][j / 4][j % 4] = h0;
+                    pl[b][j / 4][j % 4] = l0;
+                }
+                l[b] += ls;
+            }
+            // (made here, beside the products: not after the branch)
+#pragma unroll
+            for (int b = 0; b < RB; b++) __asm__ volatile("" : "+v"(ph[b][0]), "+v"(ph[b][1]), "+v"(pl[b][0]), "+v"(pl[b][1]));
+            masked(it + 1);
+            // step u: positions 16 u + 4 hh .. + 3 and 16 u + 8 + 4 hh .. + 3 of the tile, the scores' registers 8 u ..
+            const uint16_t *const vt = tiles + 2 * NP * L::KPLANE + (it & 1) * NP * L::VPLANE;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                // V^T by transposing reads: 16 lanes give the addresses of 4 rows x 16 dims (4 each) and get a dim's 4 rows
+                auto vread = [&](int plane, int d) {
+                    const uint16_t *at = vt + plane * L::VPLANE + (16 * u + 4 * hh + ((lane & 15) >> 2)) * VS + 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at);
+                    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(at + 8 * VS));
+                    return __builtin_bit_cast(f16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+                };
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    const f16x8 v = vread(0, d);
+#pragma unroll
+                    for (int b = 0; b < RB; b++) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(f16x8, pl[b][u]), o[b][d], 0, 0, 0);
+                    if constexpr (F32) {
+                        const f16x8 v2 = vread(1, d);
+#pragma unroll
+                        for (int b = 0; b < RB; b++) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v2, __builtin_bit_cast(f16x8, ph[b][u]), o[b][d], 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int b = 0; b < RB; b++) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(f16x8, ph[b][u]), o[b][d], 0, 0, 0);
+                }
+            }
+            maxima();
+            next_k(it + 2);
+            next_v(it + 1);
         }
-        float mk = 0.0f, mv = 0.0f;
-        if constexpr (F32) mk = sk.most(), mv = sv.most();
-        store_k(it + 2);
-        store_v(it + 1);
-        sk.load(rk, at_round(it + 3), tg);
-        sv.load(rv, at_round(it + 2), tg);
-        if constexpr (F32) {
-            note(it + 2, 0, mk, xk);
-            note(it + 1, 1, mv, xv);
+        if constexpr (!F32) break;
+        // K or V beyond their powers, or so small that the low parts lack bits: once more, with the span's own
+        if (pk != K_SCALE || pv != V_SCALE) break;
+        if (tid < 2) greatest[tid] = 0;
+        __syncthreads();
+        for (int off = 32; off >= 1; off >>= 1) {
+            greatest_k = fmaxf(greatest_k, __shfl_xor(greatest_k, off));
+            greatest_v = fmaxf(greatest_v, __shfl_xor(greatest_v, off));
         }
+        if (lane == 0) {
+            atomicMax(&greatest[0], __float_as_uint(greatest_k));
+            atomicMax(&greatest[1], __float_as_uint(greatest_v));
+        }
+        __syncthreads();
+        const float gk = __uint_as_float(greatest[0]), gv = __uint_as_float(greatest[1]);
+        const bool fits_k = gk == 0.0f || (gk >= pow2(-K_SCALE) && gk <= pow2(15 - K_SCALE));
+        const bool fits_v = gv == 0.0f || (gv >= pow2(-V_SCALE) && gv <= pow2(15 - V_SCALE));
+        if (fits_k && fits_v) break;
+        if (!fits_k) pk = power_for(gk);
+        if (!fits_v) pv = power_for(gv);
+        if (pk == K_SCALE && pv == V_SCALE) break;  // (the same again)
     }
     const long all = (long)a.n_kv_head * A.rows;
     float *const po = A.part + ((long)part * all + (long)g * A.rows) * HD;
@@ -584,7 +526,7 @@ __global__ __launch_bounds__(256, 1) void k_tree_part(TreeArgs A) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 float4 x = make_float4(o[b][d][4 * e], o[b][d][4 * e + 1], o[b][d][4 * e + 2], o[b][d][4 * e + 3]);
-                if constexpr (F32) x = make_float4(ldexpf(x.x, xv - TOP), ldexpf(x.y, xv - TOP), ldexpf(x.z, xv - TOP), ldexpf(x.w, xv - TOP));
+                if constexpr (F32) x = make_float4(ldexpf(x.x, -pv), ldexpf(x.y, -pv), ldexpf(x.z, -pv), ldexpf(x.w, -pv));
                 *reinterpret_cast<float4 *>(to + 32 * d + 8 * e + 4 * hh) = x;
             }
         if (hh == 0) *reinterpret_cast<float2 *>(tm) = make_float2(m[b], l[b]);
