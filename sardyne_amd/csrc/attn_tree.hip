@@ -5,9 +5,9 @@
 // A parent outside [0, t) makes t a root; below -1 it marks a place without a node: its output row stays as it was and no
 // node attends to it.
 //
-//   k_tree_part<HD, KT, RB, RW, KW>  one workgroup per (span of positions, kv head, block of 32 RB RW rows); a row is a node
+//   k_tree_part<HD, KT, RW, KW>  one workgroup per (span of positions, kv head, block of 32 RW rows); a row is a node
 //   and one of the query heads that share the kv head, so a K/V tile is read once for all of them. Span 0 is the drafted rows.
-//   RW waves of 32 RB rows share each tile of 32 positions, KW groups of them take tiles in turn. Per tile a wave computes
+//   RW waves of 32 rows share each tile of 32 positions, KW groups of them take tiles in turn. Per tile a wave computes
 //   S^T = K Q^T (a lane holds one row's 16 scores), P = exp2(S - m), and O^T += V^T P. In turn t it multiplies K of tile t + 1
 //   while it makes P of tile t, then V of tile t while it splits K of tile t + 2 and V of tile t + 1 into the other buffers.
 //   k_tree_merge<HD>  one workgroup per node and head: the spans' (m, l, O) in span order.
@@ -66,7 +66,7 @@ SDY_DEV int spans_used(const TreeArgs &A, int past) {
     return per ? (n + per - 1) / per : 0;
 }
 
-template <int HD, class KT, int RB, int RW, int KW>
+template <int HD, class KT, int RW, int KW>
 struct Lds {
     static constexpr bool F32 = std::is_same<KT, float>::value;
     static constexpr int NP = F32 ? 2 : 1;    // f16 parts of a K or V value
@@ -74,7 +74,7 @@ struct Lds {
     static constexpr int KS = HD + 8, VS = HD + 16;
     static constexpr int KPLANE = 32 * KS, VPLANE = 32 * VS, TILE = NP * (KPLANE + VPLANE);
     static constexpr size_t tiles = (size_t)KW * 2 * TILE * 2;  // two of each
-    static constexpr int ROWS = 32 * RB * RW, OS = HD + 4;
+    static constexpr int ROWS = 32 * RW, OS = HD + 4;
     static constexpr size_t merge = KW > 1 ? (size_t)KW * ROWS * (OS + 2) * 4 : 0;
     static constexpr size_t body = tiles > merge ? tiles : merge;
     // the nodes' masks and their farthest known ancestors; per 32 nodes, those with rows that hold (ok) and that do not (bad)
@@ -152,49 +152,51 @@ struct Stage {
 #pragma unroll
             for (int w = 0; w < W; w++) r[i][w] = 0;
     }
-    // The greatest |value| of this thread's, or m
-    SDY_DEV float most(float m) const {
+    static constexpr int PAIRS = NC * CE / 2;  // pairs of values
+    uint32_t part[F32 ? 2 : 1][PAIRS];
+    // the greatest of m and an f32 pair's |values|
+    SDY_DEV float most_of(int j, float m) const {
+        if constexpr (F32) return max3_abs(m, r[2 * j / CE][2 * j % CE], r[2 * j / CE][2 * j % CE + 1]);
+        else return m;
+    }
+    // pair j's parts (f32: of the values times sc)
+    SDY_DEV void split(int j, float sc) {
+        const int i = 2 * j / CE, w = 2 * j % CE;
+        if constexpr (F32) split2(__uint_as_float(r[i][w]) * sc, __uint_as_float(r[i][w + 1]) * sc, part[0][j], part[1][j]);
+        else part[0][j] = r[i][w / 2];
+    }
+    // all parts to the planes at dst, rows RS apart
+    template <int RS>
+    SDY_DEV void store(uint16_t *dst, int tg) const {
+        uint16_t *d = dst + (tg / LPR) * RS + (tg % LPR) * CE;
 #pragma unroll
         for (int i = 0; i < NC; i++)
 #pragma unroll
-            for (int w = 0; w < W; w += 2) m = max3_abs(m, r[i][w], r[i][w + 1]);
-        return m;
-    }
-    // The row's parts (f32: of the values times sc) to the planes at dst, rows RS apart
-    template <int RS>
-    SDY_DEV void store(uint16_t *dst, float sc, int tg) const {
-        uint16_t *d = dst + (tg / LPR) * RS + (tg % LPR) * CE;
-#pragma unroll
-        for (int i = 0; i < NC; i++) {
-            uint32_t out[2][CE / 2];
-#pragma unroll
-            for (int w = 0; w < CE / 2; w++) {
-                if constexpr (F32) split2(__uint_as_float(r[i][2 * w]) * sc, __uint_as_float(r[i][2 * w + 1]) * sc, out[0][w], out[1][w]);
-                else out[0][w] = r[i][w];
-            }
-#pragma unroll
             for (int p = 0; p < (F32 ? 2 : 1); p++) {
                 uint16_t *to = d + p * 32 * RS + i * LPR * CE;
-                if constexpr (CE == 8) *reinterpret_cast<u32x4 *>(to) = u32x4{out[p][0], out[p][1], out[p][2], out[p][3]};
-                else *reinterpret_cast<u32x2 *>(to) = u32x2{out[p][0], out[p][1]};
+                const uint32_t *x = part[p] + i * CE / 2;
+                if constexpr (CE == 8) *reinterpret_cast<u32x4 *>(to) = u32x4{x[0], x[1], x[2], x[3]};
+                else *reinterpret_cast<u32x2 *>(to) = u32x2{x[0], x[1]};
             }
-        }
     }
 };
 
 // Which nodes each node sees, as bits: mask[t] starts as t itself, then takes that of the farthest node known above it and
-// that one's farthest in turn, doubling the distance. All 256 threads; p0 is the parent of node tid.
+// that one's farthest in turn, doubling the distance. The first 256 threads do; p0 is the parent of node tid.
 SDY_DEV void ancestor_masks(int p0, int n, uint32_t (*mask)[MAX_NODES / 32], int16_t *up) {
     constexpr int W = MAX_NODES / 32;
     const int tid = threadIdx.x, words = (n + 31) / 32;
-    up[tid] = (int16_t)(p0 < -1 ? -2 : p0 < 0 || p0 >= tid ? -1 : p0);
+    const bool mine = tid < MAX_NODES;
+    if (mine) {
+        up[tid] = (int16_t)(p0 < -1 ? -2 : p0 < 0 || p0 >= tid ? -1 : p0);
 #pragma unroll
-    for (int w = 0; w < W; w++) mask[tid][w] = p0 >= -1 && w == tid / 32 ? 1u << (tid % 32) : 0u;
+        for (int w = 0; w < W; w++) mask[tid][w] = p0 >= -1 && w == tid / 32 ? 1u << (tid % 32) : 0u;
+    }
     __syncthreads();
-    int p = up[tid];
+    int p = mine ? up[tid] : -1;
     if (p >= 0 && up[p] < -1) p = -1;  // under an empty place: a root
     __syncthreads();
-    up[tid] = (int16_t)p;
+    if (mine) up[tid] = (int16_t)p;
     __syncthreads();
     for (int reach = 1; reach < n; reach *= 2) {
         uint32_t add[W];
@@ -213,13 +215,262 @@ SDY_DEV void ancestor_masks(int p0, int n, uint32_t (*mask)[MAX_NODES / 32], int
     }
 }
 
-template <int HD, class KT, int RB, int RW, int KW>
-__global__ __launch_bounds__(256, 1) void k_tree_part(TreeArgs A) {
-    using L = Lds<HD, KT, RB, RW, KW>;
+// The work of one span: all of its tiles, (m, l, O) in registers.
+template <int HD, class KT, int RW, int KW, bool DRAFT>
+struct Span {
+    using L = Lds<HD, KT, RW, KW>;
     using St = Stage<HD, KT, RW>;
-    static_assert(RW * KW == 4, "256 threads");
+    static constexpr bool F32 = L::F32;
+    static constexpr int NP = L::NP, KS = L::KS, VS = L::VS, ND = HD / 32, NS = HD / 16;
+    // given
+    uint16_t *tiles;
+    const uint32_t *sees;        // DRAFT: this row's nodes
+    const uint32_t *ok, *bad;    // DRAFT: rows that hold and that do not, per 32 nodes
+    unsigned *greatest;
+    __amdgpu_buffer_rsrc_t rk, rv;
+    int n_keys, rounds, kw, tg, tid, lane, hh, ql;
+    float log_scale;             // log2(e) / sqrt(HD), over the power that q is scaled by
+    f16x8 qh[NS], qlo[NS];
+    // made
+    f32x16 o[ND];
+    float m, l;  // m whole
+    int pk, pv;  // the powers that K and V are scaled by
+
+    SDY_DEV uint32_t at_round(int it) const { return (uint32_t)((it * KW + kw) * KB); }  // the group's first position in the span
+    SDY_DEV void drafted(St &st, int it) const {
+        if constexpr (DRAFT) {
+            const uint32_t t = at_round(it) / KB;
+            if (!((ok[t] & ~bad[t]) >> (tg / St::LPR) & 1)) st.clear();
+        }
+    }
+    SDY_DEV const uint16_t *k_row(int it) const { return tiles + (it & 1) * NP * L::KPLANE + ql * KS + 8 * hh; }
+    SDY_DEV static f16x8 frag(const uint16_t *p) { return *reinterpret_cast<const f16x8 *>(p); }
+    SDY_DEV static f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    // nothing moves across: products and other work stay side by side as they are written
+    SDY_DEV static void fix() { __builtin_amdgcn_sched_barrier(0); }
+    // what a tile's row does not see; register r of the scores is position 8 (r / 4) + 4 hh + r % 4 of the tile
+    SDY_DEV void masked(f32x16 &s, int it) {
+        const int k0 = (int)at_round(it);
+        if (!DRAFT && k0 + KB <= n_keys) return;
+        __asm__ volatile("");  // (a branch: not worth a select per score)
+        uint32_t bits = k0 >= n_keys ? 0u : n_keys - k0 >= KB ? ~0u : (1u << (n_keys - k0)) - 1;
+        if constexpr (DRAFT) {
+            bits = k0 < n_keys && sees ? sees[k0 / KB] : 0u;
+            if (bits & bad[k0 / KB]) l = NAN;
+        }
+        bits >>= 4 * hh;
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const uint32_t see = (uint32_t)__builtin_amdgcn_sbfe((int)bits, 8 * (r >> 2) + (r & 3), 1);
+            s[r] = __uint_as_float((__float_as_uint(s[r]) & see) | (0xFF800000u & ~see));
+        }
+    }
+    // One pass; the greatest |K| and |V| that this thread met.
+    SDY_DEV void pass(float &greatest_k, float &greatest_v) {
+        St sk, sv;
+#pragma unroll
+        for (int d = 0; d < ND; d++) o[d] = f32x16{};
+        m = -INFINITY;
+        l = 0.0f;
+        greatest_k = greatest_v = 0.0f;
+        const float factor = ldexpf(log_scale, -pk), fk = pow2(pk), fv = pow2(pv);
+        // K and V of turn `it` into their buffers, the next ones on their way
+        auto put_k = [&](int it) {
+            sk.template store<KS>(tiles + (it & 1) * NP * L::KPLANE, tg);
+            sk.load(rk, at_round(it + 1), tg);
+        };
+        auto put_v = [&](int it) {
+            sv.template store<VS>(tiles + 2 * NP * L::KPLANE + (it & 1) * NP * L::VPLANE, tg);
+            sv.load(rv, at_round(it + 1), tg);
+        };
+        constexpr int PAIRS = St::PAIRS;
+        __syncthreads();
+        sk.load(rk, at_round(0), tg);
+        sv.load(rv, at_round(0), tg);
+#pragma unroll 1
+        for (int it = 0; it < 2; it++) {
+            drafted(sk, it);
+#pragma unroll
+            for (int j = 0; j < PAIRS; j++) greatest_k = sk.most_of(j, greatest_k), sk.split(j, fk);
+            put_k(it);
+        }
+        drafted(sv, 0);
+#pragma unroll
+        for (int j = 0; j < PAIRS; j++) greatest_v = sv.most_of(j, greatest_v), sv.split(j, fv);
+        put_v(0);
+        __syncthreads();
+        f32x16 s = f32x16{};
+        {
+            const uint16_t *kr = k_row(0);
+#pragma unroll
+            for (int i = 0; i < NS; i++) {
+                const f16x8 k = frag(kr + 16 * i);
+                s = mfma(k, qlo[i], s);
+                if constexpr (F32) s = mfma(frag(kr + L::KPLANE + 16 * i), qh[i], s);
+                s = mfma(k, qh[i], s);
+            }
+        }
+        masked(s, 0);
+        float mt = s[0];  // the row's greatest score of the tile
+#pragma unroll
+        for (int r = 1; r < 16; r++) mt = fmaxf(mt, s[r]);
+#pragma unroll 1
+        for (int it = 0; it < rounds; it++) {
+            __syncthreads();
+            // a row whose scores pass its maximum too far: all that it has, down by the difference of two whole numbers
+            mt = fmaxf(mt, __shfl_xor(mt, 32)) * factor;
+            if (__ballot(mt > m + LAG || (mt > -INFINITY && m == -INFINITY))) {
+                const float up_to = mt > m + LAG || m == -INFINITY ? ceilf(mt) : m;
+                const int down = m == -INFINITY ? -300 : (int)fmaxf(m - up_to, -300.0f);
+                m = up_to;
+                l = ldexpf(l, down);
+                if (it > 0) {
+#pragma unroll
+                    for (int d = 0; d < ND; d++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) o[d][e] = ldexpf(o[d][e], down);
+                }
+            }
+            const float mu = P_BITS - (m == -INFINITY ? 0.0f : m);  // nothing seen yet: every weight is 0
+            // S of turn it + 1, a step of 16 dims at a time; beside it P of turn `it`, in 8 pairs
+            f32x16 next = f32x16{};
+            u32x4 ph[2], pl[2];
+            {
+                const uint16_t *kr = k_row(it + 1);
+                f16x8 k = frag(kr), k2 = frag(kr + (NP - 1) * L::KPLANE);
+                constexpr int EACH = NS < 8 ? 8 / NS : 1, EVERY = NS > 8 ? NS / 8 : 1;
+                float x[EACH], y[EACH];
+                fix();
+#pragma unroll
+                for (int i = 0; i < NS; i++) {
+                    const int i1 = i + 1 < NS ? i + 1 : i;
+                    const f16x8 kn = frag(kr + 16 * i1), kn2 = frag(kr + (NP - 1) * L::KPLANE + 16 * i1);
+                    const bool on = i % EVERY == 0;
+                    const int j0 = i / EVERY * EACH;
+                    next = mfma(k, qlo[i], next);
+                    fix();
+                    if (on)
+#pragma unroll
+                        for (int e = 0; e < EACH; e++) {
+                            x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * (j0 + e)], factor, mu));
+                            y[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * (j0 + e) + 1], factor, mu));
+                            __asm__ volatile("" : "+v"(x[e]), "+v"(y[e]));  // (made here, not where it is used)
+                        }
+                    fix();
+                    if constexpr (F32) next = mfma(k2, qh[i], next);
+                    fix();
+                    if (on)
+#pragma unroll
+                        for (int e = 0; e < EACH; e++) {
+                            l += x[e] + y[e];
+                            uint32_t h0, l0;
+                            split2(x[e], y[e], h0, l0);
+                            __asm__ volatile("" : "+v"(h0), "+v"(l0));
+                            ph[(j0 + e) / 4][(j0 + e) % 4] = h0;
+                            pl[(j0 + e) / 4][(j0 + e) % 4] = l0;
+                        }
+                    fix();
+                    next = mfma(k, qh[i], next);
+                    k = kn;
+                    k2 = kn2;
+                }
+                fix();
+            }
+            masked(next, it + 1);
+            drafted(sk, it + 2);
+            drafted(sv, it + 1);
+            // O, 32 dims and 16 positions a step: u: positions 16 u + 4 hh .. + 3 and 16 u + 8 + 4 hh .. + 3 of the tile, the
+            // scores' registers 8 u ..; beside it the greatest of the next scores, K of turn it + 2 and V of turn it + 1
+            {
+                const uint16_t *const vt = tiles + 2 * NP * L::KPLANE + (it & 1) * NP * L::VPLANE + (4 * hh + ((lane & 15) >> 2)) * VS +
+                                           16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                // V^T by transposing reads: 16 lanes give the addresses of 4 rows x 16 dims (4 each) and get a dim's 4 rows
+                auto vread = [&](int plane, int step) {
+                    const uint16_t *at = vt + plane * L::VPLANE + 16 * (step / ND) * VS + 32 * (step % ND);
+                    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at);
+                    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(at + 8 * VS));
+                    return __builtin_bit_cast(f16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+                };
+                constexpr int STEPS = 2 * ND, EACH = (2 * PAIRS + STEPS - 1) / STEPS, MORE = 16 / STEPS;
+                f16x8 v = vread(0, 0), v2 = vread(NP - 1, 0);
+                mt = next[0];
+                fix();
+#pragma unroll
+                for (int step = 0; step < STEPS; step++) {
+                    const int u = step / ND, d = step % ND, s1 = step + 1 < STEPS ? step + 1 : step;
+                    const f16x8 vn = vread(0, s1), vn2 = vread(NP - 1, s1);
+                    o[d] = mfma(v, __builtin_bit_cast(f16x8, pl[u]), o[d]);
+                    fix();
+                    auto work = [&](int e) {
+                        const int j = EACH * step + e;
+                        if (j < PAIRS) {
+                            greatest_k = sk.most_of(j, greatest_k);
+                            sk.split(j, fk);
+                        } else if (j < 2 * PAIRS) {
+                            const int i = j - PAIRS;
+                            greatest_v = sv.most_of(i, greatest_v);
+                            sv.split(i, fv);
+                        }
+                    };
+#pragma unroll
+                    for (int e = 0; e < EACH / 2; e++) work(e);
+                    fix();
+                    if constexpr (F32) o[d] = mfma(v2, __builtin_bit_cast(f16x8, ph[u]), o[d]);
+                    fix();
+#pragma unroll
+                    for (int e = EACH / 2; e < EACH; e++) work(e);
+#pragma unroll
+                    for (int r = 0; r < MORE; r++) mt = fmaxf(mt, next[MORE * step + r]);
+                    fix();
+                    o[d] = mfma(v, __builtin_bit_cast(f16x8, ph[u]), o[d]);
+                    v = vn;
+                    v2 = vn2;
+                }
+                fix();
+            }
+            s = next;
+            put_k(it + 2);
+            put_v(it + 1);
+        }
+    }
+    SDY_DEV void run() {
+        pk = F32 ? K_SCALE : 0;
+        pv = F32 ? V_SCALE : 0;
+        for (;;) {
+            float gk, gv;
+            pass(gk, gv);
+            if constexpr (!F32) return;
+            // K or V beyond their powers, or so small that the low parts lack bits: once more, with the span's own
+            if (pk != K_SCALE || pv != V_SCALE) return;
+            if (tid < 2) greatest[tid] = 0;
+            __syncthreads();
+            for (int off = 32; off >= 1; off >>= 1) {
+                gk = fmaxf(gk, __shfl_xor(gk, off));
+                gv = fmaxf(gv, __shfl_xor(gv, off));
+            }
+            if (lane == 0) {
+                atomicMax(&greatest[0], __float_as_uint(gk));
+                atomicMax(&greatest[1], __float_as_uint(gv));
+            }
+            __syncthreads();
+            gk = __uint_as_float(greatest[0]);
+            gv = __uint_as_float(greatest[1]);
+            const bool fits_k = gk == 0.0f || (gk >= pow2(-K_SCALE) && gk <= pow2(15 - K_SCALE));
+            const bool fits_v = gv == 0.0f || (gv >= pow2(-V_SCALE) && gv <= pow2(15 - V_SCALE));
+            if (fits_k && fits_v) return;
+            if (!fits_k) pk = power_for(gk);
+            if (!fits_v) pv = power_for(gv);
+        }
+    }
+};
+
+template <int HD, class KT, int RW, int KW>
+__global__ __launch_bounds__(64 * RW * KW, 1) void k_tree_part(TreeArgs A) {
+    using L = Lds<HD, KT, RW, KW>;
+    using St = Stage<HD, KT, RW>;
     constexpr bool F32 = L::F32;
-    constexpr int NP = L::NP, KS = L::KS, VS = L::VS, ND = HD / 32, NS = HD / 16, GROUP = 64 * RW;
+    constexpr int ND = HD / 32, NS = HD / 16, GROUP = 64 * RW, THREADS = GROUP * KW;
+    static_assert(THREADS >= MAX_NODES, "a thread per node");
     extern __shared__ __align__(16) unsigned char lds_bytes[];
     const sdy_attn_tree_args &a = A.a;
     // all row blocks of one span and kv head on one XCD (workgroups are dealt to the 8 in turn): its L2 holds the tile
@@ -231,18 +482,15 @@ __global__ __launch_bounds__(256, 1) void k_tree_part(TreeArgs A) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rw = wave % RW, kw = wave / RW, tg = tid - kw * GROUP;
     const bool draft = part == 0;
     const int rep = a.n_head / a.n_kv_head;
-    const int row0 = (block * RW + rw) * 32 * RB + ql;  // and 32 further on
+    const int row = (block * RW + rw) * 32 + ql;
+    const int node = row < A.rows ? row / rep : 0;
     const int p0 = draft && tid < a.n_tok ? a.parent[tid] : -2;
 
-    // the rows' queries: step i holds dims 16 i + 8 hh .. + 7
-    f16x8 qh[RB][NS], qlo[RB][NS];
-    int eq[RB], node[RB];
-#pragma unroll
-    for (int b = 0; b < RB; b++) {
-        const int row = row0 + 32 * b;
-        node[b] = row < A.rows ? row / rep : 0;
-        const float *q = a.q + (size_t)node[b] * a.q_stride + (size_t)(g * rep + (row < A.rows ? row - node[b] * rep : 0)) * HD + 8 * hh;
-        if (row >= A.rows) node[b] = -1;
+    // the row's queries: step i holds dims 16 i + 8 hh .. + 7
+    f16x8 qh[NS], qlo[NS];
+    float log_scale;
+    {
+        const float *q = a.q + (size_t)node * a.q_stride + (size_t)(g * rep + (row < A.rows ? row - node * rep : 0)) * HD + 8 * hh;
         float most = 0.0f;
         float4 v[2 * NS];
 #pragma unroll
@@ -256,8 +504,9 @@ __global__ __launch_bounds__(256, 1) void k_tree_part(TreeArgs A) {
             most = max3_abs(most, __float_as_uint(v[i].z), __float_as_uint(v[i].w));
         }
         most = fmaxf(most, __shfl_xor(most, 32));
-        eq[b] = power_for(most);
-        const float sc = pow2(eq[b]);
+        const int eq = power_for(most);
+        const float sc = pow2(eq);
+        log_scale = ldexpf(A.log_scale, -eq);
 #pragma unroll
         for (int i = 0; i < NS; i++) {
             u32x4 h, l;
@@ -269,8 +518,8 @@ __global__ __launch_bounds__(256, 1) void k_tree_part(TreeArgs A) {
                 split2(x.z * sc, x.w * sc, h1, l1);
                 h[2 * e] = h0, h[2 * e + 1] = h1, l[2 * e] = l0, l[2 * e + 1] = l1;
             }
-            qh[b][i] = __builtin_bit_cast(f16x8, h);
-            qlo[b][i] = __builtin_bit_cast(f16x8, l);
+            qh[i] = __builtin_bit_cast(f16x8, h);
+            qlo[i] = __builtin_bit_cast(f16x8, l);
         }
     }
 
@@ -286,256 +535,86 @@ __global__ __launch_bounds__(256, 1) void k_tree_part(TreeArgs A) {
     }
     const long from = ((long)g * (draft ? a.draft_stride : a.head_stride) + (long)lo * HD) * (long)sizeof(KT);
     const int n_keys = hi - lo, size = n_keys * (int)(HD * sizeof(KT));  // (a span's bytes fit 31 bits: the host sees to it)
-    // positions past the span's end read as zeros and are masked below
+    // positions past the span's end read as zeros and are masked
     const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void *)((const char *)(draft ? a.k_draft : a.k_cache) + from), (short)0, size, 0x00020000);
     const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void *)((const char *)(draft ? a.v_draft : a.v_cache) + from), (short)0, size, 0x00020000);
     const int rounds = (n_keys + KB * KW - 1) / (KB * KW);
-    auto at_round = [&](int it) { return (uint32_t)((it * KW + kw) * KB); };  // the group's first position in the span
 
-    uint16_t *const tiles = reinterpret_cast<uint16_t *>(lds_bytes) + kw * 2 * L::TILE;
     uint32_t(*const mask)[MAX_NODES / 32] = reinterpret_cast<uint32_t(*)[MAX_NODES / 32]>(lds_bytes + L::body);
     int16_t *const up = reinterpret_cast<int16_t *>(mask + MAX_NODES);
     uint32_t *const ok = reinterpret_cast<uint32_t *>(up + MAX_NODES), *const bad = ok + 16;
-    unsigned *const greatest = bad + 16;
 
-    St sk, sv;
-    // Drafted rows: which nodes see which, and rows that are left out: an empty place's, and those with an infinity or a NaN
-    // (NaN for the nodes that see them, nothing for the others).
+    f32x16 o[ND];
+    float m, l;
+    int pv;
+    auto span = [&](auto w) {
+        w.tiles = reinterpret_cast<uint16_t *>(lds_bytes) + kw * 2 * L::TILE;
+        w.sees = row < A.rows ? mask[node] : nullptr;
+        w.ok = ok;
+        w.bad = bad;
+        w.greatest = bad + 16;
+        w.rk = rk;
+        w.rv = rv;
+        w.n_keys = n_keys;
+        w.rounds = rounds;
+        w.kw = kw;
+        w.tg = tg;
+        w.tid = tid;
+        w.lane = lane;
+        w.hh = hh;
+        w.ql = ql;
+        w.log_scale = log_scale;
+#pragma unroll
+        for (int i = 0; i < NS; i++) w.qh[i] = qh[i], w.qlo[i] = qlo[i];
+        w.run();
+#pragma unroll
+        for (int d = 0; d < ND; d++) o[d] = w.o[d];
+        m = w.m;
+        l = w.l;
+        pv = w.pv;
+    };
     if (draft) {
+        // which nodes see which, and rows that are left out: an empty place's, and those with an infinity or a NaN (NaN for
+        // the nodes that see them, nothing for the others)
         if (tid < 32) ok[tid] = 0;
         ancestor_masks(p0, a.n_tok, mask, up);
 #pragma unroll 1
         for (int it = 0; it < rounds; it++) {
-            sk.load(rk, at_round(it), tg);
-            sv.load(rv, at_round(it), tg);
+            St sk, sv;
+            sk.load(rk, (uint32_t)((it * KW + kw) * KB), tg);
+            sv.load(rv, (uint32_t)((it * KW + kw) * KB), tg);
             const float z = sk.zeros() + sv.zeros();
-            const int t = (int)at_round(it) + tg / St::LPR;
+            const int t = (it * KW + kw) * KB + tg / St::LPR;
             if (t < MAX_NODES && (mask[t][t / 32] >> (t % 32) & 1)) atomicOr(z == 0.0f ? &ok[t / 32] : &bad[t / 32], 1u << (t % 32));
         }
+        span(Span<HD, KT, RW, KW, true>());
+    } else {
+        span(Span<HD, KT, RW, KW, false>());
     }
-    auto drafted = [&](St &st, int it) {
-        const uint32_t t = at_round(it) / KB;
-        if (!((ok[t] & ~bad[t]) >> (tg / St::LPR) & 1)) st.clear();
-    };
 
-    f32x16 o[RB][ND];
-    float m[RB], l[RB];  // m whole
-    int pk = F32 ? K_SCALE : 0, pv = F32 ? V_SCALE : 0;  // the powers that K and V are scaled by
-    for (;;) {
-        float factor[RB], greatest_k = 0.0f, greatest_v = 0.0f;
-#pragma unroll
-        for (int b = 0; b < RB; b++) {
-#pragma unroll
-            for (int d = 0; d < ND; d++) o[b][d] = f32x16{};
-            m[b] = -INFINITY;
-            l[b] = 0.0f;
-            factor[b] = ldexpf(A.log_scale, -eq[b] - pk);
-        }
-        const float fk = pow2(pk), fv = pow2(pv);
-        // K of turn `it` into its buffer, the next one on its way; V
-        auto next_k = [&](int it) {
-            if (draft) drafted(sk, it);
-            if constexpr (F32) greatest_k = sk.most(greatest_k);
-            sk.template store<KS>(tiles + (it & 1) * NP * L::KPLANE, fk, tg);
-            sk.load(rk, at_round(it + 1), tg);
-        };
-        auto next_v = [&](int it) {
-            if (draft) drafted(sv, it);
-            if constexpr (F32) greatest_v = sv.most(greatest_v);
-            sv.template store<VS>(tiles + 2 * NP * L::KPLANE + (it & 1) * NP * L::VPLANE, fv, tg);
-            sv.load(rv, at_round(it + 1), tg);
-        };
-        f32x16 s[RB];
-        float mt[RB];  // the rows' greatest scores of the tile
-        // S^T of turn `it`
-        auto scores = [&](int it) {
-            const uint16_t *kr = tiles + (it & 1) * NP * L::KPLANE + ql * KS + 8 * hh;
-#pragma unroll
-            for (int b = 0; b < RB; b++) s[b] = f32x16{};
-#pragma unroll
-            for (int i = 0; i < NS; i++) {
-                const f16x8 k = *reinterpret_cast<const f16x8 *>(kr + 16 * i);
-#pragma unroll
-                for (int b = 0; b < RB; b++) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qlo[b][i], s[b], 0, 0, 0);
-                if constexpr (F32) {
-                    const f16x8 k2 = *reinterpret_cast<const f16x8 *>(kr + L::KPLANE + 16 * i);
-#pragma unroll
-                    for (int b = 0; b < RB; b++) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k2, qh[b][i], s[b], 0, 0, 0);
-                }
-#pragma unroll
-                for (int b = 0; b < RB; b++) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[b][i], s[b], 0, 0, 0);
-            }
-        };
-        // what a tile's rows do not see; register r of the scores is position 8 (r / 4) + 4 hh + r % 4 of the tile
-        auto masked = [&](int it) {
-            const int k0 = (int)at_round(it);
-            if (!draft && k0 + KB <= n_keys) return;
-            __asm__ volatile("");  // (a branch: not worth a select per score)
-            const uint32_t end = k0 >= n_keys ? 0u : n_keys - k0 >= KB ? ~0u : (1u << (n_keys - k0)) - 1;
-#pragma unroll
-            for (int b = 0; b < RB; b++) {
-                uint32_t bits = end;
-                if (draft) {
-                    bits = k0 < n_keys && node[b] >= 0 ? mask[node[b]][k0 / KB] : 0u;
-                    if (bits & bad[k0 / KB]) l[b] = NAN;
-                }
-                bits >>= 4 * hh;
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const uint32_t see = (uint32_t)__builtin_amdgcn_sbfe((int)bits, 8 * (r >> 2) + (r & 3), 1);
-                    s[b][r] = __uint_as_float((__float_as_uint(s[b][r]) & see) | (0xFF800000u & ~see));
-                }
-            }
-        };
-        auto maxima = [&]() {
-#pragma unroll
-            for (int b = 0; b < RB; b++) {
-                mt[b] = s[b][0];
-#pragma unroll
-                for (int r = 1; r < 16; r++) mt[b] = fmaxf(mt[b], s[b][r]);
-            }
-        };
-        __syncthreads();
-        sk.load(rk, at_round(0), tg);
-        sv.load(rv, at_round(0), tg);
-#pragma unroll 1
-        for (int it = 0; it < 2; it++) next_k(it);
-        next_v(0);
-        __syncthreads();
-        scores(0);
-        masked(0);
-        maxima();
-#pragma unroll 1
-        for (int it = 0; it < rounds; it++) {
-            __syncthreads();
-            // a row whose scores pass its maximum too far: all that it has, down by the difference of two whole numbers
-            float mu[RB];
-            bool far = false;
-#pragma unroll
-            for (int b = 0; b < RB; b++) {
-                mt[b] = fmaxf(mt[b], __shfl_xor(mt[b], 32)) * factor[b];
-                far |= mt[b] > m[b] + LAG || (mt[b] > -INFINITY && m[b] == -INFINITY);
-            }
-            if (__ballot(far)) {
-#pragma unroll
-                for (int b = 0; b < RB; b++) {
-                    const float up_to = mt[b] > m[b] + LAG || m[b] == -INFINITY ? ceilf(mt[b]) : m[b];
-                    const int down = m[b] == -INFINITY ? -300 : (int)fmaxf(m[b] - up_to, -300.0f);
-                    m[b] = up_to;
-                    l[b] = ldexpf(l[b], down);
-                    if (it > 0) {
-#pragma unroll
-                        for (int d = 0; d < ND; d++)
-#pragma unroll
-                            for (int e = 0; e < 16; e++) o[b][d][e] = ldexpf(o[b][d][e], down);
-                    }
-                }
-            }
-            f32x16 sc[RB];
-#pragma unroll
-            for (int b = 0; b < RB; b++) {
-                sc[b] = s[b];
-                mu[b] = P_BITS - (m[b] == -INFINITY ? 0.0f : m[b]);  // nothing seen yet: every weight is 0
-            }
-            scores(it + 1);
-            u32x4 ph[RB][2], pl[RB][2];
-#pragma unroll
-            for (int b = 0; b < RB; b++) {
-                float ls = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][2 * j], factor[b], mu[b]));
-                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][2 * j + 1], factor[b], mu[b]));
-                    ls += x + y;
-                    uint32_t h0, l0;
-                    split2(x, y, h0, l0);
-                    ph[b][j / 4][j % 4] = h0;
-                    pl[b][j / 4][j % 4] = l0;
-                }
-                l[b] += ls;
-            }
-            // (made here, beside the products: not after the branch)
-#pragma unroll
-            for (int b = 0; b < RB; b++) __asm__ volatile("" : "+v"(ph[b][0]), "+v"(ph[b][1]), "+v"(pl[b][0]), "+v"(pl[b][1]));
-            masked(it + 1);
-            // step u: positions 16 u + 4 hh .. + 3 and 16 u + 8 + 4 hh .. + 3 of the tile, the scores' registers 8 u ..
-            const uint16_t *const vt = tiles + 2 * NP * L::KPLANE + (it & 1) * NP * L::VPLANE;
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                // V^T by transposing reads: 16 lanes give the addresses of 4 rows x 16 dims (4 each) and get a dim's 4 rows
-                auto vread = [&](int plane, int d) {
-                    const uint16_t *at = vt + plane * L::VPLANE + (16 * u + 4 * hh + ((lane & 15) >> 2)) * VS + 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-                    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at);
-                    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(at + 8 * VS));
-                    return __builtin_bit_cast(f16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-                };
-#pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    const f16x8 v = vread(0, d);
-#pragma unroll
-                    for (int b = 0; b < RB; b++) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(f16x8, pl[b][u]), o[b][d], 0, 0, 0);
-                    if constexpr (F32) {
-                        const f16x8 v2 = vread(1, d);
-#pragma unroll
-                        for (int b = 0; b < RB; b++) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v2, __builtin_bit_cast(f16x8, ph[b][u]), o[b][d], 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int b = 0; b < RB; b++) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(f16x8, ph[b][u]), o[b][d], 0, 0, 0);
-                }
-            }
-            maxima();
-            next_k(it + 2);
-            next_v(it + 1);
-        }
-        if constexpr (!F32) break;
-        // K or V beyond their powers, or so small that the low parts lack bits: once more, with the span's own
-        if (pk != K_SCALE || pv != V_SCALE) break;
-        if (tid < 2) greatest[tid] = 0;
-        __syncthreads();
-        for (int off = 32; off >= 1; off >>= 1) {
-            greatest_k = fmaxf(greatest_k, __shfl_xor(greatest_k, off));
-            greatest_v = fmaxf(greatest_v, __shfl_xor(greatest_v, off));
-        }
-        if (lane == 0) {
-            atomicMax(&greatest[0], __float_as_uint(greatest_k));
-            atomicMax(&greatest[1], __float_as_uint(greatest_v));
-        }
-        __syncthreads();
-        const float gk = __uint_as_float(greatest[0]), gv = __uint_as_float(greatest[1]);
-        const bool fits_k = gk == 0.0f || (gk >= pow2(-K_SCALE) && gk <= pow2(15 - K_SCALE));
-        const bool fits_v = gv == 0.0f || (gv >= pow2(-V_SCALE) && gv <= pow2(15 - V_SCALE));
-        if (fits_k && fits_v) break;
-        if (!fits_k) pk = power_for(gk);
-        if (!fits_v) pv = power_for(gv);
-        if (pk == K_SCALE && pv == V_SCALE) break;  // (the same again)
-    }
     const long all = (long)a.n_kv_head * A.rows;
     float *const po = A.part + ((long)part * all + (long)g * A.rows) * HD;
     float *const pm = A.part + (long)(1 + A.n_span) * all * HD + 2 * ((long)part * all + (long)g * A.rows);
     float *const om = reinterpret_cast<float *>(lds_bytes), *const ml = om + KW * L::ROWS * L::OS;
     if constexpr (KW > 1) __syncthreads();  // (the tiles are read no more)
-#pragma unroll
-    for (int b = 0; b < RB; b++) {
-        const int row = row0 + 32 * b, lr = rw * 32 * RB + 32 * b + ql;
-        l[b] += __shfl_xor(l[b], 32);
-        float *const to = KW == 1 ? po + (long)row * HD : om + (kw * L::ROWS + lr) * L::OS;
-        float *const tm = KW == 1 ? pm + 2 * row : ml + 2 * (kw * L::ROWS + lr);
-        if (KW == 1 && row >= A.rows) continue;
+    l += __shfl_xor(l, 32);
+    const int lr = rw * 32 + ql;
+    float *const to = KW == 1 ? po + (long)row * HD : om + (kw * L::ROWS + lr) * L::OS;
+    if (KW > 1 || row < A.rows) {
+        const float back = F32 ? pow2(-pv) : 1.0f;
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                float4 x = make_float4(o[b][d][4 * e], o[b][d][4 * e + 1], o[b][d][4 * e + 2], o[b][d][4 * e + 3]);
-                if constexpr (F32) x = make_float4(ldexpf(x.x, -pv), ldexpf(x.y, -pv), ldexpf(x.z, -pv), ldexpf(x.w, -pv));
-                *reinterpret_cast<float4 *>(to + 32 * d + 8 * e + 4 * hh) = x;
-            }
-        if (hh == 0) *reinterpret_cast<float2 *>(tm) = make_float2(m[b], l[b]);
+            for (int e = 0; e < 4; e++)
+                *reinterpret_cast<float4 *>(to + 32 * d + 8 * e + 4 * hh) =
+                    make_float4(o[d][4 * e] * back, o[d][4 * e + 1] * back, o[d][4 * e + 2] * back, o[d][4 * e + 3] * back);
+        if (hh == 0) *reinterpret_cast<float2 *>(KW == 1 ? pm + 2 * row : ml + 2 * (kw * L::ROWS + lr)) = make_float2(m, l);
     }
     if constexpr (KW > 1) {
         // the groups' (m, l, O) in group order
         constexpr int ROWS = L::ROWS, OS = L::OS;
         __syncthreads();
-        for (int i = tid; i < ROWS * HD / 4; i += 256) {
+        for (int i = tid; i < ROWS * HD / 4; i += THREADS) {
             const int r = i / (HD / 4), c = 4 * (i - r * (HD / 4)), gr = block * ROWS + r;
             if (gr >= A.rows) continue;
             float M = -INFINITY, ls = 0.0f;
@@ -610,15 +689,14 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs A) {
 
 // How the work is split, from the sizes alone.
 struct Plan {
-    int rb, rw, kw, rows, n_block, n_span;
+    int rw, kw, rows, n_block, n_span;
 };
 Plan plan_of(int n_tok, int n_head, int n_kv_head, int hd, int max_past) {
     Plan p;
     p.rows = n_tok * (n_head / n_kv_head);
-    p.rb = hd < 256 && p.rows > 64 ? 2 : 1;
-    p.rw = hd == 256 || p.rows > 128 ? 4 : 2;
-    p.kw = 4 / p.rw;
-    const int block = 32 * p.rb * p.rw;
+    p.rw = hd < 256 && p.rows > 128 ? 8 : 4;
+    p.kw = hd == 256 ? 1 : 8 / p.rw;
+    const int block = 32 * p.rw;
     p.n_block = (p.rows + block - 1) / block;
     const int granule = KB * p.kw;
     const long pairs = (long)n_kv_head * p.n_block, rounds = ((long)max_past + granule - 1) / granule;
@@ -632,24 +710,23 @@ Plan plan_of(int n_tok, int n_head, int n_kv_head, int hd, int max_past) {
     return p;
 }
 
-template <int HD, class KT, int RB, int RW, int KW>
+template <int HD, class KT, int RW, int KW>
 int launch_part(const TreeArgs &A, hipStream_t st) {
     static size_t granted = 0;
-    const void *fn = (const void *)k_tree_part<HD, KT, RB, RW, KW>;
-    const int rc = sdy_lds_limit(fn, Lds<HD, KT, RB, RW, KW>::bytes, &granted);
+    const void *fn = (const void *)k_tree_part<HD, KT, RW, KW>;
+    const int rc = sdy_lds_limit(fn, Lds<HD, KT, RW, KW>::bytes, &granted);
     if (rc) return rc;
-    SDY_NOTE_KERNEL((k_tree_part<HD, KT, RB, RW, KW>));
+    SDY_NOTE_KERNEL((k_tree_part<HD, KT, RW, KW>));
     const long pairs = (long)(1 + A.n_span) * A.a.n_kv_head;
-    hipLaunchKernelGGL((k_tree_part<HD, KT, RB, RW, KW>), dim3((unsigned)((pairs + 7) / 8 * 8 * A.n_block)), dim3(256),
-                       (Lds<HD, KT, RB, RW, KW>::bytes), st, A);
+    hipLaunchKernelGGL((k_tree_part<HD, KT, RW, KW>), dim3((unsigned)((pairs + 7) / 8 * 8 * A.n_block)), dim3(64 * RW * KW),
+                       (Lds<HD, KT, RW, KW>::bytes), st, A);
     return sdy_check_launch("attn_tree");
 }
 
 template <int HD, class KT>
 int launch_rows(const TreeArgs &A, const Plan &p, hipStream_t st) {
-    if constexpr (HD == 256) return launch_part<HD, KT, 1, 4, 1>(A, st);
-    else if (p.rw == 4) return launch_part<HD, KT, 2, 4, 1>(A, st);
-    else return p.rb == 2 ? launch_part<HD, KT, 2, 2, 2>(A, st) : launch_part<HD, KT, 1, 2, 2>(A, st);
+    if constexpr (HD == 256) return launch_part<HD, KT, 4, 1>(A, st);
+    else return p.rw == 8 ? launch_part<HD, KT, 8, 1>(A, st) : launch_part<HD, KT, 4, 2>(A, st);
 }
 
 template <int HD>
