@@ -6,7 +6,8 @@
 // node attends to it.
 //
 //   k_tree_part<HD, KT, RW, KW>  one workgroup per (span of positions, kv head, block of 32 RW rows); a row is a node
-//   and one of the query heads that share the kv head, so a K/V tile is read once for all of them. Span 0 is the drafted rows.
+//   and one of the query heads that share the kv head, so a K/V tile is read once for all of them. The first spans are the
+//   drafted rows, a turn each.
 //   RW waves of 32 rows share each tile of 32 positions, KW groups of them take tiles in turn. Per tile a wave computes
 //   S^T = K Q^T (a lane holds one row's 16 scores), P = exp2(S - m), and O^T += V^T P. In turn t it multiplies K of tile t + 1
 //   while it makes P of tile t, then V of tile t while it splits K of tile t + 2 and V of tile t + 1 into the other buffers.
@@ -43,27 +44,29 @@ constexpr int TOP = 13;        // a row of q, and a span computed again, are sca
 constexpr int K_SCALE = 5, V_SCALE = 9;  // the powers that K and V are scaled by at first
 constexpr float P_BITS = 4;    // P is 2^P_BITS exp2(score - m), of scores up to m + LAG
 constexpr float LAG = 11;
-constexpr int MAX_PARTS = 513;
+constexpr int MAX_PARTS = 512 + MAX_NODES / KB;
 constexpr int MAX_PAST = 1 << 28;  // 512 spans of at most 2^30 bytes hold them
 
 struct TreeArgs {
     sdy_attn_tree_args a;
     int rows;       // per kv head: n_tok * (n_head / n_kv_head)
     int n_block;    // row blocks
+    int n_draft;    // spans of drafted rows
     int n_span;     // spans of cached positions (the grid's; those in use follow from n_past)
+    int least;      // turns of such a span, at least
     int granule;    // positions of one turn of a workgroup: 32 KW
     float log_scale;  // log2(e) / sqrt(head_dim)
-    float *part;    // [1 + n_span][n_kv_head * rows][HD], then the (m, l) [1 + n_span][n_kv_head * rows][2]
+    float *part;    // [n_draft + n_span][n_kv_head * rows][HD], then the (m, l) [n_draft + n_span][n_kv_head * rows][2]
 };
 
 // The rounds (granules) per span and the spans in use for so many positions.
 SDY_DEV int span_rounds(const TreeArgs &A, int past) {
-    const int n = (past + A.granule - 1) / A.granule;
-    return (n + A.n_span - 1) / A.n_span;
+    const int n = (past + A.granule - 1) / A.granule, per = (n + A.n_span - 1) / A.n_span;
+    return per > A.least ? per : A.least;
 }
 SDY_DEV int spans_used(const TreeArgs &A, int past) {
     const int per = span_rounds(A, past), n = (past + A.granule - 1) / A.granule;
-    return per ? (n + per - 1) / per : 0;
+    return (n + per - 1) / per;
 }
 
 template <int HD, class KT, int RW, int KW>
@@ -492,13 +495,13 @@ __global__ __launch_bounds__(64 * RW * KW, 1) void k_tree_part(TreeArgs A) {
     extern __shared__ __align__(16) unsigned char lds_bytes[];
     const sdy_attn_tree_args &a = A.a;
     // all row blocks of one span and kv head on one XCD (workgroups are dealt to the 8 in turn): its L2 holds the tile
-    const int pairs = (1 + A.n_span) * a.n_kv_head;
+    const int pairs = (A.n_draft + A.n_span) * a.n_kv_head;
     const int id = (int)blockIdx.x, pair = (id / 8 / A.n_block) * 8 + id % 8, block = id / 8 % A.n_block;
     if (pair >= pairs) return;
     const int part = pair / a.n_kv_head, g = pair - part * a.n_kv_head;
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, ql = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rw = wave / KW, kw = wave % KW, tg = rw * 64 + lane;
-    const bool draft = part == 0;
+    const bool draft = part < A.n_draft;
     const int rep = a.n_head / a.n_kv_head;
     const int row = (block * RW + rw) * 32 + ql;
     const int past = *a.n_past;
@@ -543,10 +546,13 @@ __global__ __launch_bounds__(64 * RW * KW, 1) void k_tree_part(TreeArgs A) {
     }
 
     if (past < 0 || past > a.max_past) return;
-    int lo = 0, hi = a.n_tok;
-    if (!draft) {
+    int lo = part * A.granule, hi = lo + A.granule < a.n_tok ? lo + A.granule : a.n_tok;
+    if (draft) {
+        const int last = (block + 1) * 32 * RW < A.rows ? (block + 1) * 32 * RW - 1 : A.rows - 1;
+        if (lo > last / rep) return;  // none of the block's nodes sees a later one, nor does the merge look
+    } else {
         const int per = span_rounds(A, past) * A.granule;
-        const long l0 = (long)(part - 1) * per, h0 = l0 + per;
+        const long l0 = (long)(part - A.n_draft) * per, h0 = l0 + per;
         if (l0 >= past) return;  // the merge does not look at it
         lo = (int)l0;
         hi = h0 < past ? (int)h0 : past;
@@ -567,9 +573,10 @@ __global__ __launch_bounds__(64 * RW * KW, 1) void k_tree_part(TreeArgs A) {
     int pv;
     auto span = [&](auto w) {
         w.tiles = reinterpret_cast<uint16_t *>(lds_bytes) + kw * 2 * L::TILE;
-        w.sees = row < A.rows ? mask[node] : nullptr;
-        w.ok = ok;
-        w.bad = bad;
+        const int tile = draft ? lo / KB : 0;
+        w.sees = row < A.rows ? mask[node] + tile : nullptr;
+        w.ok = ok + tile;
+        w.bad = bad + tile;
         w.greatest = bad + 16;
         w.rk = rk;
         w.rv = rv;
@@ -600,14 +607,9 @@ __global__ __launch_bounds__(64 * RW * KW, 1) void k_tree_part(TreeArgs A) {
         sv.load(rv, (uint32_t)(kw * KB), tg);
         if (tid < 32) ok[tid] = 0;
         ancestor_masks(p0, a.n_tok, mask, up);
-#pragma unroll 1
-        for (int it = 0; it < rounds; it++) {
-            const float z = sk.zeros() + sv.zeros();
-            sk.load(rk, (uint32_t)(((it + 1) * KW + kw) * KB), tg);
-            sv.load(rv, (uint32_t)(((it + 1) * KW + kw) * KB), tg);
-            const int t = (it * KW + kw) * KB + tg / St::LPR;
-            if (t < a.n_tok && (mask[t][t / 32] >> (t % 32) & 1)) atomicOr(z == 0.0f ? &ok[t / 32] : &bad[t / 32], 1u << (t % 32));
-        }
+        const float z = sk.zeros() + sv.zeros();
+        const int t = lo + kw * KB + tg / St::LPR;
+        if (t < a.n_tok && (mask[t][t / 32] >> (t % 32) & 1)) atomicOr(z == 0.0f ? &ok[t / 32] : &bad[t / 32], 1u << (t % 32));
         span(Span<HD, KT, RW, KW, true>());
     } else {
         span(Span<HD, KT, RW, KW, false>());
@@ -615,7 +617,7 @@ __global__ __launch_bounds__(64 * RW * KW, 1) void k_tree_part(TreeArgs A) {
 
     const long all = (long)a.n_kv_head * A.rows;
     float *const po = A.part + ((long)part * all + (long)g * A.rows) * HD;
-    float *const pm = A.part + (long)(1 + A.n_span) * all * HD + 2 * ((long)part * all + (long)g * A.rows);
+    float *const pm = A.part + (long)(A.n_draft + A.n_span) * all * HD + 2 * ((long)part * all + (long)g * A.rows);
     float *const om = reinterpret_cast<float *>(lds_bytes), *const ml = om + KW * L::ROWS * L::OS;
     if constexpr (KW > 1) __syncthreads();  // (the tiles are read no more)
     l += __shfl_xor(l, 32);
@@ -668,12 +670,14 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs A) {
     const int past = *a.n_past, tid = threadIdx.x;
     const int t = blockIdx.x, h = blockIdx.y;
     if (past < 0 || past > a.max_past || a.parent[t] < -1) return;
-    const int n = 1 + spans_used(A, past), rep = a.n_head / a.n_kv_head, g = h / rep;
+    // the drafted spans up to the node's own, and those of the cache
+    const int nd = t / A.granule + 1, n = nd + spans_used(A, past), rep = a.n_head / a.n_kv_head, g = h / rep;
+    auto at = [&](int p) { return (long)(p < nd ? p : p - nd + A.n_draft); };
     const long all = (long)a.n_kv_head * A.rows, row = (long)g * A.rows + (long)t * rep + (h - g * rep);
-    const float2 *pm = reinterpret_cast<const float2 *>(A.part + (long)(1 + A.n_span) * all * HD) + row;
+    const float2 *pm = reinterpret_cast<const float2 *>(A.part + (long)(A.n_draft + A.n_span) * all * HD) + row;
     float M = -INFINITY;
     for (int p = tid; p < n; p += 256) {
-        ml[p] = pm[p * all];
+        ml[p] = pm[at(p) * all];
         M = fmaxf(M, ml[p].x);
     }
     for (int off = 32; off >= 1; off >>= 1) M = fmaxf(M, __shfl_xor(M, off));
@@ -686,7 +690,7 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs A) {
     float lsum = 0.0f;
 #pragma unroll 4
     for (int p = grp; p < n; p += NG) {
-        const float4 y = po[p * all * LN];
+        const float4 y = po[at(p) * all * LN];
         const float x = __builtin_amdgcn_exp2f(ml[p].x - M);
         lsum += ml[p].y * x;
         sum.x += y.x * x, sum.y += y.y * x, sum.z += y.z * x, sum.w += y.w * x;
@@ -710,7 +714,7 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs A) {
 
 // How the work is split, from the sizes alone.
 struct Plan {
-    int rw, kw, rows, n_block, n_span;
+    int rw, kw, rows, n_block, n_draft, n_span;
 };
 Plan plan_of(int n_tok, int n_head, int n_kv_head, int hd, int max_past) {
     Plan p;
@@ -720,10 +724,12 @@ Plan plan_of(int n_tok, int n_head, int n_kv_head, int hd, int max_past) {
     const int block = 32 * p.rw;
     p.n_block = (p.rows + block - 1) / block;
     const int granule = KB * p.kw;
+    p.n_draft = (n_tok + granule - 1) / granule;
     const long pairs = (long)n_kv_head * p.n_block, rounds = ((long)max_past + granule - 1) / granule;
-    long n = (256 - pairs) / pairs;
+    long n = (256 - pairs * p.n_draft) / pairs;
+    if (n < 128 / pairs) n = 128 / pairs;
     if (n > rounds) n = rounds;
-    if (n > MAX_PARTS - 1) n = MAX_PARTS - 1;
+    if (n > 512) n = 512;
     // a span's bytes (at most 2^31 - 1 for a buffer resource)
     const long least = (rounds * granule * hd * 4 + (1l << 30) - 1) >> 30;
     if (n < least) n = least;
@@ -738,7 +744,7 @@ int launch_part(const TreeArgs &A, hipStream_t st) {
     const int rc = sdy_lds_limit(fn, Lds<HD, KT, RW, KW>::bytes, &granted);
     if (rc) return rc;
     SDY_NOTE_KERNEL((k_tree_part<HD, KT, RW, KW>));
-    const long pairs = (long)(1 + A.n_span) * A.a.n_kv_head;
+    const long pairs = (long)(A.n_draft + A.n_span) * A.a.n_kv_head;
     hipLaunchKernelGGL((k_tree_part<HD, KT, RW, KW>), dim3((unsigned)((pairs + 7) / 8 * 8 * A.n_block)), dim3(64 * RW * KW),
                        (Lds<HD, KT, RW, KW>::bytes), st, A);
     return sdy_check_launch("attn_tree");
@@ -768,7 +774,7 @@ extern "C" int sdy_attn_tree_ok(int n_tok, int n_head, int n_kv_head, int hd) {
 extern "C" size_t sdy_attn_tree_floats(int n_tok, int n_head, int n_kv_head, int hd, int max_past) {
     if (!sdy_attn_tree_ok(n_tok, n_head, n_kv_head, hd) || max_past < 0 || max_past > MAX_PAST) return 0;
     const Plan p = plan_of(n_tok, n_head, n_kv_head, hd, max_past);
-    return (size_t)(1 + p.n_span) * n_kv_head * p.rows * (hd + 2);
+    return (size_t)(p.n_draft + p.n_span) * n_kv_head * p.rows * (hd + 2);
 }
 
 extern "C" int sdy_attn_tree(const sdy_attn_tree_args *a, sdy_stream s) {
@@ -800,6 +806,9 @@ extern "C" int sdy_attn_tree(const sdy_attn_tree_args *a, sdy_stream s) {
     A.n_block = p.n_block;
     A.n_span = p.n_span;
     A.granule = KB * p.kw;
+    A.n_draft = p.n_draft;
+    // two turns where they are of 32 positions: half the parts to merge (24 nodes of 16 heads over 2500: 22.2 -> 19.7 us)
+    A.least = p.kw == 1 ? 2 : 1;
     A.log_scale = (float)(1.4426950408889634074 / sqrt((double)a->hd));
     A.part = a->part;
     hipStream_t st = (hipStream_t)s;
