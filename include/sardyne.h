@@ -197,6 +197,27 @@ int sdy_grid_barrier_probe(int n_wg, int rounds, int mode, int stream_mb, sdy_ba
  * the mean microseconds per kernel of each. */
 int sdy_kernel_boundary_us(int n, float *us_graph, float *us_eager);
 
+/* ------------------------------------------------------------------ speculative step
+ * No counterpart in the reference. How a token is taken from its logits: of the greatest top_k (<= 0: all), the fewest whose
+ * probabilities at temperature temp reach top_p (>= 1: all), of these the ones with at least min_p times the greatest's; the
+ * first by id at which their running sum exceeds u of their whole. temp <= 0: the greatest logit, the lowest id of equal ones. */
+typedef struct {
+    float temp;
+    int32_t top_k;
+    float top_p, min_p;
+} sdy_sampling;
+/* Evaluates a tree of n drafted tokens in one pass and keeps the path that the model's own tokens take. tokens[0] is the
+ * context's next token; parents[0] = -1 and 0 <= parents[i] < i. A token is taken from every node's logits by `how` (NULL:
+ * temp 0) and u[i] in [0, 1) (NULL: 0); the path goes from node 0 to the lowest child whose token is its parent's taken one,
+ * until there is none or the context is full. The path's nodes become the context's last positions (engine_n_past grows by
+ * *n_path; path has room for n), *next is the token taken after them, the next call's first. With one way of taking tokens
+ * and one u per position, the tokens kept are those of one call per token, within the rounding of other sums. n at most
+ * min(n_batch, 256), head_dim 64, 128 or 256. The logits are not copied to the host (engine_n_logits 0). The first call
+ * allocates its device memory, freed with the context. 0, or -1 with the reason in engine_last_error and the context
+ * unchanged. */
+int sdy_engine_speculate(engine_ctx *c, const int32_t *tokens, const int32_t *parents, int32_t n,
+                         const sdy_sampling *how, const float *u, int32_t *path, int32_t *n_path, int32_t *next);
+
 /* ------------------------------------------------------------------ device-level, no allocation
  * No counterpart in the reference. For callers that cannot allocate device memory: code recorded
  * under graph capture, tight serving loops, harnesses that forbid hipMalloc. The one-token decode

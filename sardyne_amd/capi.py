@@ -152,6 +152,11 @@ class SdySampleArgs(ctypes.Structure):
                 ("top_k", _vp), ("top_p", _vp), ("min_p", _vp), ("u", _vp), ("token", _vp), ("prob", _vp), ("ws", _vp)]
 
 
+class SdySampling(ctypes.Structure):
+    """sdy_sampling (include/sardyne.h)."""
+    _fields_ = [("temp", _float), ("top_k", _i32), ("top_p", _float), ("min_p", _float)]
+
+
 class SdyTreeCommitArgs(ctypes.Structure):
     """sdy_tree_commit_args (sardyne_amd/csrc/sdy_ops.h)."""
     _fields_ = [("token", _vp), ("parent", _vp), ("sampled", _vp), ("n_tok", _int), ("n_past", _vp), ("k_draft", _vp),
@@ -277,6 +282,8 @@ _DEVICE_SIGNATURES = {
     "sdy_sample_ws_bytes": (_sz, [_int, _int]),
     "sdy_sample": (_int, [ctypes.POINTER(SdySampleArgs), _vp]),
     "sdy_tree_commit": (_int, [ctypes.POINTER(SdyTreeCommitArgs), _vp]),
+    "sdy_engine_speculate": (_int, [_vp, _vp, _vp, _i32, ctypes.POINTER(SdySampling), _vp, _vp, ctypes.POINTER(_i32),
+                                    ctypes.POINTER(_i32)]),
 }
 
 EPI_NONE, EPI_SWIGLU = 0, 1

@@ -854,6 +854,60 @@ int engine_eval(engine_ctx *c, const int32_t *tokens, int32_t n) {
     return 0;
 }
 
+/* ------------------------------------------------------------------ speculative steps */
+
+/* The reason a tree cannot be evaluated now (written into c->err), or 0. */
+static int refuse_tree(engine_ctx *c, const int32_t *tokens, const int32_t *parents, int32_t n) {
+    const engine_model_info *in = &c->m->info;
+    const int most = c->n_batch < 256 ? c->n_batch : 256;
+    if (!sdy_attn_tree_ok(1, in->n_head, in->n_kv_head, in->head_dim))
+        return say(c->err, sizeof c->err, "speculative steps need head_dim 64, 128 or 256 (%d)", in->head_dim);
+    if (n > most) return say(c->err, sizeof c->err, "n=%d non valido (1..%d)", n, most);
+    if (c->n_past >= c->max_seq)
+        return say(c->err, sizeof c->err, "contesto pieno: %d + %d > max_seq=%d", c->n_past, 1, c->max_seq);
+    for (int32_t i = 0; i < n; i++) {
+        if ((uint32_t)tokens[i] >= (uint32_t)in->n_vocab)
+            return say(c->err, sizeof c->err, "token %d fuori dal vocabolario [0, %d)", tokens[i], in->n_vocab);
+        if (i ? parents[i] < 0 || parents[i] >= i : parents[i] != -1)
+            return say(c->err, sizeof c->err, "parents[%d]=%d non valido", i, parents[i]);
+    }
+    return 0;
+}
+
+int sdy_engine_speculate(engine_ctx *c, const int32_t *tokens, const int32_t *parents, int32_t n,
+                         const sdy_sampling *how, const float *u, int32_t *path, int32_t *n_path, int32_t *next) {
+    if (!c) return -1;
+    c->err[0] = '\0';
+    if (!tokens || !parents || n < 1) return say(c->err, sizeof c->err, "nessun token in ingresso");
+    if (!path || !n_path || !next) return say(c->err, sizeof c->err, "path, n_path and next are needed");
+    if (refuse_tree(c, tokens, parents, n)) return -1;
+    if (sdy_engine_spec_alloc(c)) return say(c->err, sizeof c->err, "errore GPU: %s", sdy_last_error());
+    const sdy_sampling greedy = {0.0f, 0, 1.0f, 0.0f};
+    if (!how) how = &greedy;
+    const int R = c->spec_rows;
+    int32_t *w = c->spec_host;
+    float *f = (float *)c->spec_host;
+    for (int32_t i = 0; i < n; i++) {
+        w[SPEC_TOKEN * R + i] = tokens[i];
+        w[SPEC_PARENT * R + i] = parents[i];
+        w[SPEC_POS * R + i] = i ? w[SPEC_POS * R + parents[i]] + 1 : c->n_past;
+        w[SPEC_NODE * R + i] = i;
+        w[SPEC_TOP_K * R + i] = how->top_k;
+        f[SPEC_TEMP * R + i] = how->temp;
+        f[SPEC_TOP_P * R + i] = how->top_p;
+        f[SPEC_MIN_P * R + i] = how->min_p;
+        f[SPEC_U * R + i] = u ? u[i] : 0.0f;
+    }
+    w[SPEC_PAST * R] = c->n_past;
+    if (sdy_engine_spec_step(c, n)) return say(c->err, sizeof c->err, "errore GPU: %s", sdy_last_error());
+    *n_path = w[SPEC_COUNT * R];
+    for (int32_t i = 0; i < *n_path; i++) path[i] = w[SPEC_PATH * R + i];
+    *next = w[SPEC_STEP * R];
+    c->n_past += *n_path;
+    c->n_logits = 0;
+    return 0;
+}
+
 const float *engine_logits(const engine_ctx *c) { return c && c->n_logits ? c->logits : NULL; }
 int32_t engine_n_logits(const engine_ctx *c) { return c ? c->n_logits : 0; }
 int32_t engine_n_past(const engine_ctx *c) { return c ? c->n_past : 0; }

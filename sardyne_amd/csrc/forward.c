@@ -127,10 +127,38 @@ void sdy_engine_release(engine_ctx *c) {
                    c->hb2, c->logits_dev, c->part, c->xq[0], c->xq[1], c->tok_dev, c->moe_probs, c->moe_w,
                    c->moe_top, c->moe_x, c->moe_y, c->moe_sum, c->moe_gidx, c->moe_gw, c->qkv, c->step_dev,
                    c->gemm_ws, c->attn_part, c->attn_count, c->moe_grp_tok, c->moe_grp_tile, c->moe_src,
-                   c->moe_orow};
+                   c->moe_orow, c->spec_k, c->spec_v, c->spec_logits, c->spec_part, c->spec_ws, c->spec_freq, c->spec_dev};
     for (size_t i = 0; i < sizeof dev / sizeof *dev; i++) sdy_free(dev[i]);
-    void *host[] = {c->tok_host, c->moe_top_host, c->moe_w_host, c->moe_gidx_host, c->moe_gw_host, c->step_host};
+    void *host[] = {c->tok_host, c->moe_top_host, c->moe_w_host, c->moe_gidx_host, c->moe_gw_host, c->step_host,
+                    c->spec_host};
     for (size_t i = 0; i < sizeof host / sizeof *host; i++) sdy_host_free(host[i]);
+}
+
+/* Memory of speculative steps, at the first one. A failure leaves what there is for the next try or the release. */
+int sdy_engine_spec_alloc(engine_ctx *c) {
+    const engine_model_info *in = &c->m->info;
+    if (c->spec_rows) return 0;
+    const int rows = c->n_batch < 256 ? c->n_batch : 256, hd = in->head_dim;
+    const size_t kv = (size_t)in->n_layer * in->n_kv_head * rows * hd * sdy_kv_elt_bytes(c->kv_type);
+    size_t part = 0;
+    for (int n = 1; n <= rows; n++) {
+        const size_t f = sdy_attn_tree_floats(n, in->n_head, in->n_kv_head, hd, c->max_seq);
+        part = f > part ? f : part;
+    }
+    double freq[256];
+    TRY(sdy_rope_freqs(freq, &c->spec_mscale, hd, in->rope_theta, NULL));
+    if (!c->spec_k) TRY(dalloc(&c->spec_k, kv));
+    if (!c->spec_v) TRY(dalloc(&c->spec_v, kv));
+    if (!c->spec_logits) TRY(dalloc((void **)&c->spec_logits, (size_t)rows * in->n_vocab * 4));
+    if (!c->spec_part) TRY(dalloc((void **)&c->spec_part, part * 4));
+    if (!c->spec_ws) TRY(dalloc(&c->spec_ws, sdy_sample_ws_bytes(rows, in->n_vocab)));
+    if (!c->spec_freq) TRY(dalloc((void **)&c->spec_freq, sizeof freq));
+    if (!c->spec_dev) TRY(dalloc((void **)&c->spec_dev, (size_t)SPEC_ALL * rows * 4));
+    if (!c->spec_host) TRY(sdy_host_alloc((void **)&c->spec_host, (size_t)SPEC_ALL * rows * 4));
+    TRY(sdy_h2d(c->spec_freq, freq, sizeof freq, c->st));
+    TRY(sdy_sync(c->st));
+    c->spec_rows = rows;
+    return 0;
 }
 
 /* Every write of c->xq[] comes with this call: the quantisation cache forgets its sources, and the GEMM
@@ -542,14 +570,18 @@ int sdy_engine_decode_fused_ok(const engine_ctx *c) {
 
 /* The layers and the head for n tokens at positions n_past.. (kernels only: no host copies or
  * synchronisation, so that the one-token step can be recorded as a graph). decode: the fused
- * one-token kernels, with the token and its position read from step_dev. */
-static int layers(engine_ctx *c, int n, int out_rows, int decode) {
+ * one-token kernels, with the token and its position read from step_dev. tree: the n nodes of a speculative step (spec_dev),
+ * whose K/V rows go to spec_k / spec_v and whose logits to spec_logits. */
+static int layers(engine_ctx *c, int n, int out_rows, int decode, int tree) {
     const engine_model *m = c->m;
     const engine_model_info *in = &m->info;
     const int dim = in->dim, hd = in->head_dim, q_dim = in->n_head * hd, kv_dim = in->n_kv_head * hd;
     const int pos0 = c->n_past;
     const long head_stride = (long)c->max_seq * hd, layer_stride = (long)in->n_kv_head * head_stride;
-    TRY(sdy_dequant_gather(&m->tok_embd.m, decode ? c->step_dev : c->tok_dev, n, c->x, c->st));
+    const int32_t *const spec = c->spec_dev;
+    const int R = c->spec_rows;
+    float *const logits = tree ? c->spec_logits : c->logits_dev;
+    TRY(sdy_dequant_gather(&m->tok_embd.m, tree ? spec + SPEC_TOKEN * R : decode ? c->step_dev : c->tok_dev, n, c->x, c->st));
     for (int l = 0; l < in->n_layer; l++) {
         const dlayer *L = &m->layers[l];
         const size_t kv_off = (size_t)l * layer_stride * sdy_kv_elt_bytes(c->kv_type);
@@ -645,15 +677,36 @@ static int layers(engine_ctx *c, int n, int out_rows, int decode) {
                 TRY(mm(c, c->k, c->xb, &L->wk, n, L->bk, NULL, 0));
                 TRY(mm(c, c->v, c->xb, &L->wv, n, L->bv, NULL, 0));
             }
-            TRY(sdy_qk_rope_kv_strided(q, k, v, qs, ks, vs, L->q_norm, L->k_norm, in->norm_eps, c->rope_cos,
-                                       c->rope_sin, pos0, n, in->n_head, in->n_kv_head, hd, in->rope_interleaved, kc,
-                                       vc, c->kv_type, head_stride, c->st));
-            if (c->prefill_flash && (qs & 3) == 0)
-                TRY(sdy_attention_flash(q, kc, vc, c->kv_type, n, in->n_head, in->n_kv_head, hd, pos0 + 1, head_stride,
-                                        qs, c->att, q_dim, c->st));
-            else
-                TRY(sdy_attention(q, kc, vc, c->kv_type, n, in->n_head, in->n_kv_head, hd, pos0 + 1, head_stride, qs,
-                                  c->part, c->att, q_dim, c->st));
+            if (tree) {
+                const size_t off = (size_t)l * in->n_kv_head * R * hd * sdy_kv_elt_bytes(c->kv_type);
+                const sdy_rope_at_args r = {.q = q, .k = k, .v = v, .q_stride = qs, .k_stride = ks, .v_stride = vs,
+                                            .q_out = c->q, .q_out_stride = q_dim, .k_rows = (char *)c->spec_k + off,
+                                            .v_rows = (char *)c->spec_v + off, .head_stride = (long)R * hd,
+                                            .kv_type = c->kv_type, .n_slot = R, .pos = spec + SPEC_POS * R,
+                                            .slot = spec + SPEC_NODE * R, .freq = c->spec_freq, .mscale = c->spec_mscale,
+                                            .n_rot = hd, .interleaved = in->rope_interleaved, .q_norm = L->q_norm,
+                                            .k_norm = L->k_norm, .eps = in->norm_eps, .n_tok = n, .n_head = in->n_head,
+                                            .n_kv_head = in->n_kv_head, .hd = hd};
+                TRY(sdy_qk_rope_at(&r, c->st));
+                const sdy_attn_tree_args t = {.q = c->q, .q_stride = q_dim, .k_cache = kc, .v_cache = vc,
+                                              .head_stride = head_stride, .k_draft = r.k_rows, .v_draft = r.v_rows,
+                                              .draft_stride = (long)R * hd, .kv_type = c->kv_type,
+                                              .parent = spec + SPEC_PARENT * R, .n_past = spec + SPEC_PAST * R,
+                                              .max_past = c->max_seq, .n_tok = n, .n_head = in->n_head,
+                                              .n_kv_head = in->n_kv_head, .hd = hd, .out = c->att, .out_stride = q_dim,
+                                              .part = c->spec_part};
+                TRY(sdy_attn_tree(&t, c->st));
+            } else {
+                TRY(sdy_qk_rope_kv_strided(q, k, v, qs, ks, vs, L->q_norm, L->k_norm, in->norm_eps, c->rope_cos,
+                                           c->rope_sin, pos0, n, in->n_head, in->n_kv_head, hd, in->rope_interleaved,
+                                           kc, vc, c->kv_type, head_stride, c->st));
+                if (c->prefill_flash && (qs & 3) == 0)
+                    TRY(sdy_attention_flash(q, kc, vc, c->kv_type, n, in->n_head, in->n_kv_head, hd, pos0 + 1,
+                                            head_stride, qs, c->att, q_dim, c->st));
+                else
+                    TRY(sdy_attention(q, kc, vc, c->kv_type, n, in->n_head, in->n_kv_head, hd, pos0 + 1, head_stride,
+                                      qs, c->part, c->att, q_dim, c->st));
+            }
             TRY(mm(c, c->x, c->att, &L->wo, n, NULL, c->x, 1));
         }
         if (in->n_expert && decode && c->moe_device) {
@@ -687,13 +740,13 @@ static int layers(engine_ctx *c, int n, int out_rows, int decode) {
         const float *xs = c->x + (size_t)(n - out_rows) * dim;
         /* one row of logits: the head's workgroups normalise and quantise the row themselves (the
            persistent ring matvec with its norm prologue, the bits of the norm launch + matvec) */
-        const int hrc = out_rows == 1 ? mm1_fused(c, c->logits_dev, xs, m->output_norm, &m->output, NULL, NULL,
+        const int hrc = out_rows == 1 ? mm1_fused(c, logits, xs, m->output_norm, &m->output, NULL, NULL,
                                                   SDY_EPI_NONE)
                                       : 1;
         if (hrc < 0) return hrc;
         if (hrc) {
             TRY(norm_for(c, xs, m->output_norm, &m->output, out_rows));
-            TRY(mm(c, c->logits_dev, c->xb, &m->output, out_rows, NULL, NULL, 0));
+            TRY(mm(c, logits, c->xb, &m->output, out_rows, NULL, NULL, 0));
         }
     }
     return 0;
@@ -710,7 +763,7 @@ int sdy_engine_forward(engine_ctx *c, const int32_t *tokens, int n, int out_rows
            second is recorded as a graph that later steps replay */
         if (c->graph_ok == 0 && c->use_graph && c->n_decode >= 1) {
             TRY(sdy_graph_begin(c->st));
-            int rc = layers(c, 1, out_rows, 1);
+            int rc = layers(c, 1, out_rows, 1, 0);
             if (rc) {
                 sdy_graph_abort(c->st);
                 c->graph_ok = -1;
@@ -724,15 +777,39 @@ int sdy_engine_forward(engine_ctx *c, const int32_t *tokens, int n, int out_rows
             }
         }
         if (c->graph_ok == 1 && out_rows == 1) TRY(sdy_graph_launch(c->graph, c->st));
-        else TRY(layers(c, 1, out_rows, 1));
+        else TRY(layers(c, 1, out_rows, 1, 0));
         c->n_decode++;
     } else {
         memcpy(c->tok_host, tokens, (size_t)n * 4);
         TRY(sdy_h2d(c->tok_dev, c->tok_host, (size_t)n * 4, c->st));
-        TRY(layers(c, n, out_rows, 0));
+        TRY(layers(c, n, out_rows, 0, 0));
     }
     if (out_rows > 0) TRY(sdy_d2h(c->logits, c->logits_dev, (size_t)out_rows * in->n_vocab * 4, c->st));
     TRY(sdy_sync(c->st));
     c->n_past += n;
     return 0;
+}
+
+int sdy_engine_spec_step(engine_ctx *c, int n) {
+    const engine_model_info *in = &c->m->info;
+    const int R = c->spec_rows, hd = in->head_dim;
+    int32_t *const w = c->spec_dev;
+    float *const f = (float *)c->spec_dev;
+    TRY(sdy_h2d(w, c->spec_host, (size_t)SPEC_IN * R * 4, c->st));
+    TRY(layers(c, n, n, 0, 1));
+    const sdy_sample_args s = {.logits = c->spec_logits, .stride = in->n_vocab, .n_rows = n, .n_vocab = in->n_vocab,
+                               .temp = f + SPEC_TEMP * R, .top_k = w + SPEC_TOP_K * R, .top_p = f + SPEC_TOP_P * R,
+                               .min_p = f + SPEC_MIN_P * R, .u = f + SPEC_U * R, .token = w + SPEC_SAMPLED * R,
+                               .ws = c->spec_ws};
+    TRY(sdy_sample(&s, c->st));
+    const sdy_tree_commit_args t = {.token = w + SPEC_TOKEN * R, .parent = w + SPEC_PARENT * R, .sampled = w + SPEC_SAMPLED * R,
+                                    .n_tok = n, .n_past = w + SPEC_PAST * R, .k_draft = c->spec_k, .v_draft = c->spec_v,
+                                    .draft_stride = (long)R * hd, .draft_layer_stride = (long)in->n_kv_head * R * hd,
+                                    .k_cache = c->k_cache, .v_cache = c->v_cache, .head_stride = (long)c->max_seq * hd,
+                                    .layer_stride = (long)in->n_kv_head * c->max_seq * hd, .kv_type = c->kv_type,
+                                    .max_seq = c->max_seq, .n_layer = in->n_layer, .n_kv_head = in->n_kv_head, .hd = hd,
+                                    .path = w + SPEC_PATH * R, .n_acc = w + SPEC_COUNT * R, .step = w + SPEC_STEP * R};
+    TRY(sdy_tree_commit(&t, c->st));
+    TRY(sdy_d2h(c->spec_host + SPEC_IN * R, w + SPEC_IN * R, (size_t)(SPEC_ALL - SPEC_IN) * R * 4, c->st));
+    return sdy_sync(c->st);
 }

@@ -88,12 +88,28 @@ struct engine_ctx {
     int32_t *moe_src, *moe_orow;
     int moe_grouped_ok;         /* every MoE layer's experts take the grouped GEMM */
     float *moe_w_host, *moe_gw_host;
+    /* speculative steps (sdy_engine_speculate; allocated by the first one) for up to spec_rows nodes */
+    int spec_rows;
+    void *spec_k, *spec_v;      /* the nodes' K/V rows, [n_layer][n_kv_head][spec_rows][head_dim] of kv_type */
+    float *spec_logits;         /* [spec_rows][n_vocab] */
+    float *spec_part;           /* sdy_attn_tree's scratch */
+    void *spec_ws;              /* sdy_sample's */
+    double *spec_freq;          /* the rotary frequencies */
+    float spec_mscale;
+    int32_t *spec_dev, *spec_host; /* one step's words (SPEC_*), each of spec_rows */
     char err[256];
 };
+
+/* The words of a speculative step, in rows of spec_rows: what goes to the device, then what comes back */
+enum { SPEC_TOKEN, SPEC_PARENT, SPEC_POS, SPEC_NODE, SPEC_TOP_K, SPEC_TEMP, SPEC_TOP_P, SPEC_MIN_P, SPEC_U, SPEC_PAST, SPEC_IN,
+       SPEC_SAMPLED = SPEC_IN, SPEC_PATH, SPEC_COUNT, SPEC_STEP, SPEC_ALL = SPEC_STEP + 2 };
 
 int sdy_engine_alloc(engine_ctx *c);
 void sdy_engine_release(engine_ctx *c);
 int sdy_engine_forward(engine_ctx *c, const int32_t *tokens, int n, int out_rows);
+int sdy_engine_spec_alloc(engine_ctx *c);
+/* one speculative step of the n nodes in spec_host; its SPEC_PATH, SPEC_COUNT and SPEC_STEP come back there */
+int sdy_engine_spec_step(engine_ctx *c, int n);
 int sdy_engine_decode_fused_ok(const engine_ctx *c);
 int sdy_engine_moe_device_ok(const engine_ctx *c);
 #endif

@@ -124,6 +124,25 @@ class Session:
         out = self.feed([int(token)])
         return out[-1] if self.logits_all else out
 
+    def speculate(self, tokens, parents, u=None, temp=0.0, top_k=0, top_p=1.0, min_p=0.0) -> tuple[list[int], int]:
+        """One speculative step (sdy_engine_speculate): the drafted tree's tokens (the first is the context's next token)
+        with each one's parent, and the uniform numbers that tokens are taken with. Returns the accepted nodes, now the
+        context's last positions, and the token after them."""
+        ids, par = (np.ascontiguousarray(x, dtype=np.int32).reshape(-1) for x in (tokens, parents))
+        if ids.size != par.size:
+            raise ValueError(f"{ids.size} tokens and {par.size} parents")
+        uu = None if u is None else np.ascontiguousarray(u, dtype=np.float32).reshape(-1)
+        if uu is not None and uu.size != ids.size:
+            raise ValueError(f"{ids.size} tokens and {uu.size} uniform numbers")
+        path = np.empty(max(ids.size, 1), np.int32)
+        n, nxt = ctypes.c_int32(), ctypes.c_int32()
+        how = capi.SdySampling(temp, top_k, top_p, min_p)
+        if self._lib.sdy_engine_speculate(self._h, ids.ctypes.data, par.ctypes.data, int(ids.size), ctypes.byref(how),
+                                          uu.ctypes.data if uu is not None else None, path.ctypes.data, ctypes.byref(n),
+                                          ctypes.byref(nxt)) != 0:
+            self._raise()
+        return path[:n.value].tolist(), nxt.value
+
     def rewind(self, n: int):
         """Keeps the first n cached positions (engine_truncate)."""
         if self._lib.engine_truncate(self._h, int(n)) != 0:

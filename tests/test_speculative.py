@@ -110,6 +110,12 @@ def test_no_arguments():
         assert fn(None, None) == -1
 
 
+def test_speculate_without_a_context():
+    one = (ctypes.c_int32 * 1)()
+    n = ctypes.c_int32()
+    assert capi.lib().sdy_engine_speculate(None, one, one, 1, None, None, one, ctypes.byref(n), ctypes.byref(n)) == -1
+
+
 def test_empty_calls_do_nothing():
     lib = capi.lib()
     assert lib.sdy_qk_rope_at(ctypes.byref(rope_args(n_tok=0)), None) == 0
