@@ -105,7 +105,8 @@ struct Row {
         alone = none || !(temp > 0.0f);
         inv_t = 1.0 / (double)temp;
         // over the whole of the finite logits, or as far down as a w counts (2^-62 is exp(-43))
-        const float range = fminf(best - low, 43.0f * temp);
+        // (at most f32's greatest value: two logits can be farther apart, and are in the last bin then)
+        const float range = fminf(fminf(best - low, 43.0f * temp), 0x1.fffffep127f);
         per_bin = range > 0.0f ? (float)BINS / range : 0.0f;
     }
     // from the pieces' maxima, by each wave for itself
@@ -598,7 +599,8 @@ __global__ __launch_bounds__(BINS) void k_sample_cut(Args A) {
             // the bins that the border can be in: their arithmetic is in 32 bits
             const float far = r.min_p < 1.0f ? -logf(r.min_p) * r.temp * r.per_bin : 0.0f;
             const int lo = (int)fminf(far * (1.0f - 1e-5f), (float)(BINS - 1));
-            const int hi = (int)fminf(far * (1.0f + 1e-5f) + 1e-5f, (float)(BINS - 1));
+            // (with min_p 1 all those whose w rounds to 1: 2^-53 T down)
+            const int hi = (int)fminf(far * (1.0f + 1e-5f) + 1e-5f + 0x1p-52f * r.temp * r.per_bin, (float)(BINS - 1));
             b0 = r.top_p < 1.0f && b0 < lo ? b0 : lo;
             b1 = hi < b1 ? hi : b1;
         }

@@ -167,7 +167,8 @@ typedef struct {
     const float *logits;         /* rows stride floats apart */
     long stride;
     int n_rows, n_vocab;         /* at most 65535, 2^22 */
-    const float *temp;           /* [n_rows] each, or NULL: temperature 1, no top-k, no top-p, no min-p */
+    const float *temp;           /* [n_rows] each, or NULL: temperature 1, no top-k, no top-p, no min-p (NaN: temp as 0,
+                                    the others as if not given) */
     const int32_t *top_k;
     const float *top_p, *min_p;
     const float *u;              /* [n_rows] uniform numbers */

@@ -449,6 +449,32 @@ def test_sample_special_logits(v):
         assert np.array_equal(run_sample(x, u=u)[0], run_sample(x, u=np.float32(1) - np.float32(2.0 ** -24))[0])
 
 
+@pytest.mark.parametrize("v", [4099, 40003])
+def test_sample_special_long_rows(v):
+    """As above in rows that are cut into pieces: what decides is where the bins of distance from the greatest logit end."""
+    nan, inf, big = np.nan, np.inf, np.float32(3e38)
+    rng = np.random.default_rng(v)
+    x = rng.standard_normal((10, v)).astype(np.float32)
+    x[1] = -inf
+    x[1, 7::9] = nan
+    x[2, 5::1000] = inf
+    x[3] *= big / 8
+    x[4] = np.where(rng.random(v) < 0.5, big, -big)
+    x[5, :] = -inf
+    x[5, v - 1] = np.finfo(np.float32).min
+    x[6] = -0.0
+    x[6, 3] = 0.0
+    x[7] = 1e-45 * (np.arange(v) % 5)
+    x[8, rng.random(v) < 0.5] = nan
+    x[9] = inf
+    for temp in (0.0, 1e-45, 1.0, 1e19, 1e38, inf, nan):
+        for top_p, top_k, min_p in ((1.0, 0, 0.0), (0.9, 0, 0.0), (1.0, 0, 1.0), (1.0, 0, 0.03), (0.6, 0, 0.5), (1.0, 2000, 0.03),
+                                    (0.5, 300, 0.0), (0.0, 0, 2.0)):
+            check_sample(x, temp, top_k, top_p, min_p, rng.random(10))
+    u = rng.random(10)  # no numbers: as if not given
+    assert np.array_equal(run_sample(x, 2.0, 0, nan, nan, u)[0], run_sample(x, 2.0, u=u)[0])
+
+
 def test_sample_follows_the_probabilities():
     """Every token of a small row is taken by just the u of its share."""
     x = np.log(np.array([[0.1, 0.0, 0.35, 0.05, 0.5]], np.float32) + 1e-45).astype(np.float32)
