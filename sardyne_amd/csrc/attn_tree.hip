@@ -294,7 +294,8 @@ struct Span {
         m = -INFINITY;
         l = 0.0f;
         greatest_k = greatest_v = 0.0f;
-        const float factor = ldexpf(log_scale, -pk), fk = pow2(pk), fv = pow2(pv);
+        // (never 0, which would make a masked score NaN: with q and K below 2^-100 every score is 0 all the same)
+        const float factor = fmaxf(ldexpf(log_scale, -pk), 0x1p-126f), fk = pow2(pk), fv = pow2(pv);
         // K and V of turn `it` into their buffers, the next ones on their way
         auto put_k = [&](int it) {
             sk.template store<KS>(tiles + (it & 1) * NP * L::KPLANE, tg);

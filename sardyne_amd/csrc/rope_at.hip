@@ -219,6 +219,8 @@ extern "C" int sdy_qk_rope_at(const sdy_rope_at_args *a, sdy_stream s) {
     // rows may share memory only where they are the same rows: a token's heads are written while others are read
     if (a->q && a->q_out == a->q && a->q_out_stride != a->q_stride)
         return sdy_fail(-1, "qk_rope_at: q in place needs q_out_stride %ld to be q_stride %ld", a->q_out_stride, a->q_stride);
+    if (a->q && a->n_tok > 1 && a->q_out_stride < (long)a->n_head * a->hd)
+        return sdy_fail(-1, "qk_rope_at: rows of %d heads %ld apart in q_out", a->n_head, a->q_out_stride);
     hipStream_t st = (hipStream_t)s;
     const bool f16 = a->kv_type == SDY_KV_F16;
     // rows of float4 (and of 4 stored values), no four dims half turned

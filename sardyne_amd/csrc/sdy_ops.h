@@ -135,8 +135,9 @@ int sdy_qk_rope_at(const sdy_rope_at_args *a, sdy_stream s);
 
 /* Attention of the nodes: node t sees every cached position below *n_past, itself and the nodes above it. K/V rows of the
  * nodes are in memory of their own (as sdy_qk_rope_at writes them with slot = node), so the cache holds accepted
- * positions only. Within tolerance (f32 sums in the kernel's order), the same on every call. An unused place's output row,
- * and with *n_past outside [0, max_past] every row, is left as it was. */
+ * positions only. Within tolerance (f32 sums in the kernel's order), the same on every call. An infinity or NaN in a K or V
+ * row makes the outputs of the nodes that see it NaN, and of no others. An unused place's output row, and with *n_past
+ * outside [0, max_past] every row, is left as it was. */
 typedef struct {
     const float *q;              /* rotated queries, rows q_stride floats apart */
     long q_stride;
@@ -186,14 +187,15 @@ typedef struct {
     const int32_t *token, *parent, *sampled; /* [n_tok] the drafted tokens, their parents, the token sampled at each node */
     int n_tok;                   /* at most 256 */
     const int32_t *n_past;       /* device int */
-    const void *k_draft, *v_draft; /* [n_layer][n_kv_head][..][hd] of kv_type, strides in elements */
+    const void *k_draft, *v_draft; /* [n_layer][n_kv_head][..][hd] of kv_type, strides in elements; not in the cache */
     long draft_stride, draft_layer_stride;
     void *k_cache, *v_cache;     /* [n_layer][n_kv_head][max_seq][hd] */
     long head_stride, layer_stride;
     int kv_type, max_seq, n_layer, n_kv_head, hd;
     int32_t *path;               /* [n_tok] the accepted nodes in order, then -1 */
     int32_t *n_acc;              /* [1] */
-    int32_t *step;               /* [2] the next token and its position, as the one-token steps read them; not n_past's memory */
+    int32_t *step;               /* [2] the next token and its position, as the one-token steps read them; path, n_acc and step
+                                    share memory with nothing else */
 } sdy_tree_commit_args;
 int sdy_tree_commit(const sdy_tree_commit_args *a, sdy_stream s);
 #ifdef __cplusplus

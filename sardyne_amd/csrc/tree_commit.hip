@@ -80,8 +80,16 @@ extern "C" int sdy_tree_commit(const sdy_tree_commit_args *a, sdy_stream s) {
         for (int o = 0; o < 3; o++)
             if (in[i] < out[o] + out_n[o] && out[o] < in[i] + in_n[i])
                 return sdy_fail(-1, "tree_commit: path, n_acc and step must not overlap token, parent, sampled or n_past");
-    if (a->k_draft == a->k_cache || a->v_draft == a->v_cache)
-        return sdy_fail(-1, "tree_commit: the drafted rows must not be the cache's own");
+    for (int o = 0; o < 3; o++)
+        if (out[o] < out[(o + 1) % 3] + out_n[(o + 1) % 3] && out[(o + 1) % 3] < out[o] + out_n[o])
+            return sdy_fail(-1, "tree_commit: path, n_acc and step must not overlap each other");
+    // (the first head's: the others lie as these do)
+    const void *const draft[2] = {a->k_draft, a->v_draft}, *const cache[2] = {a->k_cache, a->v_cache};
+    for (int i = 0; i < 2; i++) {
+        const char *const d = (const char *)draft[i], *const c = (const char *)cache[i];
+        if (d < c + (size_t)a->max_seq * a->hd * elt && c < d + (size_t)a->n_tok * a->hd * elt)
+            return sdy_fail(-1, "tree_commit: the drafted rows must not be the cache's own");
+    }
     const uintptr_t all = (uintptr_t)a->k_draft | (uintptr_t)a->v_draft | (uintptr_t)a->k_cache | (uintptr_t)a->v_cache |
                           (uintptr_t)((a->draft_stride | a->draft_layer_stride | a->head_stride | a->layer_stride | a->hd) * (long)elt);
     const dim3 grid(a->n_kv_head, 2, a->n_layer);

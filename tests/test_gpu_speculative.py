@@ -269,7 +269,7 @@ def test_attn_tree_position_outside_leaves_out(past):
 
 
 @pytest.mark.parametrize("kv", [0, 1], ids=["f32", "f16"])
-@pytest.mark.parametrize("what", ["peaks", "large", "tiny", "mixed_rows", "equal"])
+@pytest.mark.parametrize("what", ["peaks", "large", "tiny", "vanishing", "mixed_rows", "equal"])
 def test_attn_tree_values(what, kv):
     def spike(q, cache, draft):
         if what == "peaks":  # weights that leave one position
@@ -281,6 +281,11 @@ def test_attn_tree_values(what, kv):
             q *= 1e-6
             for x in cache + draft:
                 x *= 1e-3
+        if what == "vanishing":  # scores of 0 from K and q that are not, and from a q that is
+            q[:] *= np.float32(1e-38)
+            q[::3] = 0
+            for x in cache[:1] + draft[:1]:
+                x *= x.dtype.type(1e-35 if x.dtype == np.float32 else 1e-7)
         if what == "mixed_rows":  # rows of very different sizes, and dims within a row
             q *= np.exp2(np.arange(-10, 10))[None, None, np.arange(q.shape[2]) % 20].astype(q.dtype) / 8
             cache[0][:, ::3] /= 256
@@ -290,6 +295,28 @@ def test_attn_tree_values(what, kv):
             for x in cache + draft:
                 x[:] = 1
     Tree(37, 333, 8, 2, 128, kv, 6, spike=spike).run().check()
+
+
+@pytest.mark.parametrize("kv", [0, 1], ids=["f32", "f16"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("n,nh", [(12, 8), (90, 8)])
+def test_attn_tree_bad_drafted_rows(bad, kv, n, nh):
+    """A drafted row with a value that is no number: NaN for the nodes that see it, nothing for the others."""
+    t = Tree(n, 100, nh, 2, 64, kv, 21)
+    node = n // 3
+    for side in (0, 1):
+        rows = t.draft[side].copy()
+        rows[1, node, 5] = bad
+        b = up(rows)
+        args = type(t.args).from_buffer_copy(t.args)
+        setattr(args, ("k_draft", "v_draft")[side], b.ptr)
+        capi.check(lib().sdy_attn_tree(ctypes.byref(args), None))
+        got = t.got()
+        sees = S.ancestors(t.parent)[:, node]
+        assert sees.any() and not sees.all()
+        assert np.isnan(got[sees][:, nh // 2:]).all()
+        t.want[sees, nh // 2:] = got[sees, nh // 2:] = 0
+        t.check(got)
 
 
 def test_attn_tree_strided_rows():

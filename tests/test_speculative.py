@@ -29,7 +29,7 @@ def rope_args(**kw):
     (dict(freq=None), "freq"), (dict(q_out=None), "q_out"), (dict(n_head=0), "n_head"), (dict(v=None), "v,"),
     (dict(k_rows=None), "k_rows"), (dict(v_rows=None), "v_rows"), (dict(n_kv_head=0), "n_kv_head"),
     (dict(head_stride=64 * 9 - 1), "stride"), (dict(n_slot=-1), "slots"), (dict(n_tok=-1), "n_tok"),
-    (dict(q_out=P, q_out_stride=516), "in place")])
+    (dict(q_out=P, q_out_stride=516), "in place"), (dict(q_out_stride=511), "apart")])
 def test_rope_at_refusals(kw, word):
     refused(capi.lib().sdy_qk_rope_at, rope_args(**kw), word)
 
@@ -98,6 +98,8 @@ def commit_args(**kw):
                                     "path", "n_acc", "step")] + [
     (dict(step=4 * P - 4), "overlap"), (dict(path=P), "overlap"), (dict(n_acc=2 * P + 12), "overlap"),
     (dict(path=3 * P - 12), "overlap"), (dict(k_draft=3 * P), "own"), (dict(v_draft=4 * P), "own"),
+    (dict(k_draft=3 * P + 10 * 256 - 16), "own"), (dict(v_draft=4 * P - 4 * 256 + 16), "own"),
+    (dict(n_acc=5 * P + 12), "overlap"), (dict(step=6 * P - 4), "overlap"), (dict(step=5 * P - 4), "overlap"),
     (dict(head_stride=639), "reach"), (dict(draft_stride=255), "reach"), (dict(layer_stride=1279), "reach"),
     (dict(draft_layer_stride=511), "reach")])
 def test_tree_commit_refusals(kw, word):
