@@ -568,6 +568,212 @@ def test_tree_commit_no_node():
 
 # ----------------------------------------------------------------------------------- a step of them
 
+class Step:
+    """The four operators of one step over one layer, from inputs that the host writes: rotary positions, attention, tokens
+    from given logits, the commit. Sizes that take every kernel's longer path."""
+    N, NH, NKV, HD, VOCAB, MAX = 20, 8, 2, 64, 4133, 400
+
+    def __init__(self, scratch=None):
+        n, nh, nkv, hd, vocab, mx = self.N, self.NH, self.NKV, self.HD, self.VOCAB, self.MAX
+        L = lib()
+        self.width = (nh + 2 * nkv) * hd
+        self.b = {k: up(np.zeros(v, t)) for k, (v, t) in dict(
+            x=((n, self.width), np.float32), pos=(n, np.int32), node=(n, np.int32), parent=(n, np.int32), past=(1, np.int32),
+            logits=((n, vocab), np.float32), temp=(n, np.float32), top_k=(n, np.int32), top_p=(n, np.float32),
+            u=(n, np.float32), token=(n, np.int32), cache=((2, nkv, mx, hd), np.float16)).items()}
+        self.o = {k: up(np.zeros(v, t)) for k, (v, t) in dict(
+            q=((n, nh * hd), np.float32), draft=((2, nkv, n, hd), np.float16), out=((n, nh * hd), np.float32),
+            sampled=(n, np.int32), prob=(n, np.float32), path=(n, np.int32), n_acc=(1, np.int32), step=(2, np.int32)).items()}
+        self.like = {"q": np.float32, "draft": np.uint16, "out": np.float32, "sampled": np.int32, "prob": np.float32,
+                     "path": np.int32, "n_acc": np.int32, "step": np.int32}
+        floats, ws = L.sdy_attn_tree_floats(n, nh, nkv, hd, mx), L.sdy_sample_ws_bytes(n, vocab)
+        self.scratch = scratch or (capi.DeviceBuffer(4 * floats), capi.DeviceBuffer(ws))
+        self.freq = up(rope_freq(hd)[0])
+        b, o = {k: v.ptr for k, v in self.b.items()}, {k: v.ptr for k, v in self.o.items()}
+        half, dhalf = nkv * mx * hd * 2, nkv * n * hd * 2
+        self.calls = [
+            (L.sdy_qk_rope_at, capi.SdyRopeAtArgs(
+                q=b["x"], k=b["x"] + 4 * nh * hd, v=b["x"] + 4 * (nh + nkv) * hd, q_stride=self.width, k_stride=self.width,
+                v_stride=self.width, q_out=o["q"], q_out_stride=nh * hd, k_rows=o["draft"], v_rows=o["draft"] + dhalf,
+                head_stride=n * hd, kv_type=1, n_slot=n, pos=b["pos"], slot=b["node"], freq=self.freq.ptr, mscale=1.0, n_rot=hd,
+                n_tok=n, n_head=nh, n_kv_head=nkv, hd=hd)),
+            (L.sdy_attn_tree, capi.SdyAttnTreeArgs(
+                q=o["q"], q_stride=nh * hd, k_cache=b["cache"], v_cache=b["cache"] + half, head_stride=mx * hd,
+                k_draft=o["draft"], v_draft=o["draft"] + dhalf, draft_stride=n * hd, kv_type=1, parent=b["parent"],
+                n_past=b["past"], max_past=mx, n_tok=n, n_head=nh, n_kv_head=nkv, hd=hd, out=o["out"], out_stride=nh * hd,
+                part=self.scratch[0].ptr)),
+            (L.sdy_sample, capi.SdySampleArgs(
+                logits=b["logits"], stride=vocab, n_rows=n, n_vocab=vocab, temp=b["temp"], top_k=b["top_k"], top_p=b["top_p"],
+                u=b["u"], token=o["sampled"], prob=o["prob"], ws=self.scratch[1].ptr)),
+            (L.sdy_tree_commit, capi.SdyTreeCommitArgs(
+                token=b["token"], parent=b["parent"], sampled=o["sampled"], n_tok=n, n_past=b["past"], k_draft=o["draft"],
+                v_draft=o["draft"] + dhalf, draft_stride=n * hd, draft_layer_stride=nkv * n * hd, k_cache=b["cache"],
+                v_cache=b["cache"] + half, head_stride=mx * hd, layer_stride=nkv * mx * hd, kv_type=1, max_seq=mx, n_layer=1,
+                n_kv_head=nkv, hd=hd, path=o["path"], n_acc=o["n_acc"], step=o["step"]))]
+
+    def fill(self, seed, stream=None):
+        rng = np.random.default_rng(seed)
+        n = self.N
+        parent = S.random_tree(n, rng, unused=int(rng.integers(0, 5)))
+        past = int(rng.integers(0, self.MAX))
+        logits = np.round(rng.standard_normal((n, self.VOCAB)) * 4).astype(np.float32)
+        new = dict(x=rng.standard_normal((n, self.width)), pos=past + S.ancestors(parent).sum(1), node=np.arange(n),
+                   parent=parent, past=[past], logits=logits, temp=rng.choice([0, 0.7, 2], n), top_k=rng.choice([0, 40], n),
+                   top_p=rng.choice([1, 0.9], n), u=rng.random(n), token=np.argmax(logits, 1)[np.maximum(parent, 0)],
+                   cache=rng.standard_normal((2, self.NKV, self.MAX, self.HD)))
+        types = dict(x=np.float32, pos=np.int32, node=np.int32, parent=np.int32, past=np.int32, logits=np.float32,
+                     temp=np.float32, top_k=np.int32, top_p=np.float32, u=np.float32, token=np.int32, cache=np.float16)
+        self.sent = {k: np.ascontiguousarray(v, types[k]) for k, v in new.items()}
+        for k, v in self.sent.items():
+            assert v.nbytes == self.b[k].nbytes
+            capi.check(lib().sdy_h2d(self.b[k].ptr, v.ctypes.data, v.nbytes, stream))
+        for v in self.o.values():  # (an empty place's output row stays as it was)
+            capi.check(lib().sdy_memset(v.ptr, 0, v.nbytes, stream))
+        return self
+
+    def run(self, stream=None):
+        for fn, a in self.calls:
+            capi.check(fn(ctypes.byref(a), stream))
+
+    def got(self, stream=None):
+        got = {k: v.to_array(self.like[k], v.nbytes // np.dtype(self.like[k]).itemsize, stream) for k, v in self.o.items()}
+        got["cache"] = self.b["cache"].to_array(np.uint16, self.b["cache"].nbytes // 2, stream)
+        return got
+
+
+def same(a, b):
+    return all(np.array_equal(a[k].view(np.uint16), b[k].view(np.uint16)) for k in a)
+
+
+def test_a_recorded_step_replays_for_other_trees():
+    """Two recorded steps on one scratch, replayed in turn with new inputs, eager steps between: the eager step's bits."""
+    L = lib()
+    st = ctypes.c_void_p()
+    capi.check(L.sdy_stream_new(ctypes.byref(st)))
+    eager = Step()
+    steps = [Step()]
+    steps.append(Step(steps[0].scratch))
+    graphs = []
+    for x in steps:
+        x.fill(0).run()  # (what a first launch sets up is not recorded)
+        capi.check(L.sdy_sync(None))
+        capi.check(L.sdy_graph_begin(st))
+        x.run(st)
+        g = ctypes.c_void_p()
+        capi.check(L.sdy_graph_end(st, ctypes.byref(g)))
+        graphs.append(g)
+    taken = set()
+    for k in range(12):
+        x, g = steps[k % 2], graphs[k % 2]
+        x.fill(100 + k, st)
+        capi.check(L.sdy_graph_launch(g, st))
+        eager.fill(100 + k).run()
+        want = eager.got()
+        assert same(x.got(st), want), k
+        taken.add(int(want["n_acc"][0]))
+    assert len(taken) > 1
+    for g in graphs:
+        capi.check(L.sdy_graph_free(g))
+    capi.check(L.sdy_stream_free(st))
+
+
+def test_steps_on_two_streams_at_once():
+    """Each with its own scratch."""
+    L = lib()
+    sts = [ctypes.c_void_p() for _ in range(2)]
+    for st in sts:
+        capi.check(L.sdy_stream_new(ctypes.byref(st)))
+    steps, eager = [Step(), Step()], Step()
+    for k in range(4):
+        for i, (x, st) in enumerate(zip(steps, sts)):
+            x.fill(10 * k + i, st)
+        for x, st in zip(steps, sts):
+            x.run(st)
+        for i, (x, st) in enumerate(zip(steps, sts)):
+            got = x.got(st)
+            eager.fill(10 * k + i).run()
+            assert same(got, eager.got()), (k, i)
+    for st in sts:
+        capi.check(L.sdy_stream_free(st))
+
+
+def test_rows_beyond_32_bit_offsets():
+    """Heads 2^31 elements apart: rotated rows written there, attended to, and moved there by the commit."""
+    n, past, hd, far, rng = 6, 45, 128, (1 << 31) + 128, np.random.default_rng(8)
+    big = [capi.DeviceBuffer(2 * (far + 64 * hd)) for _ in range(2)]  # f16
+    t = Tree(n, past, 4, 2, hd, 1, 5)
+    for buf, rows in zip(big, t.cache):
+        for g in range(2):
+            r = np.ascontiguousarray(rows[g, :past])
+            capi.check(lib().sdy_h2d(buf.ptr + 2 * g * far, r.ctypes.data, r.nbytes, None))
+    capi.check(lib().sdy_sync(None))
+    t.args.k_cache, t.args.v_cache, t.args.head_stride, t.args.max_past = big[0].ptr, big[1].ptr, far, past
+    t.part = capi.DeviceBuffer(4 * lib().sdy_attn_tree_floats(n, 4, 2, hd, past))
+    t.args.part = t.part.ptr
+    t.run().check()
+    # the commit of the first two nodes behind them
+    ints = [up(np.array(x, np.int32)) for x in ([3] * n, [-1, 0] + [-2] * (n - 2), [3] * n, [past], [0] * n, [0], [0, 0])]
+    p = [b.ptr for b in ints]
+    c = capi.SdyTreeCommitArgs(token=p[0], parent=p[1], sampled=p[2], n_tok=n, n_past=p[3], k_draft=t.args.k_draft,
+                               v_draft=t.args.v_draft, draft_stride=n * hd, draft_layer_stride=2 * n * hd, k_cache=big[0].ptr,
+                               v_cache=big[1].ptr, head_stride=far, layer_stride=2 * far, kv_type=1, max_seq=64, n_layer=1,
+                               n_kv_head=2, hd=hd, path=p[4], n_acc=p[5], step=p[6])
+    capi.check(lib().sdy_tree_commit(ctypes.byref(c), None))
+    # and rotary rows to the next position
+    x, freq = rng.standard_normal((1, 3 * 2 * hd)).astype(np.float32), rope_freq(hd)[0]
+    bx, bf, bp, bq = up(x), up(freq), up(np.array([past + 2], np.int32)), capi.DeviceBuffer(4 * 2 * hd)
+    a = capi.SdyRopeAtArgs(q=bx.ptr, k=bx.ptr + 8 * hd, v=bx.ptr + 16 * hd, q_stride=6 * hd, k_stride=6 * hd, v_stride=6 * hd,
+                           q_out=bq.ptr, q_out_stride=2 * hd, k_rows=big[0].ptr, v_rows=big[1].ptr, head_stride=far, kv_type=1,
+                           n_slot=64, pos=bp.ptr, freq=bf.ptr, mscale=1.0, n_rot=hd, n_tok=1, n_head=2, n_kv_head=2, hd=hd)
+    capi.check(lib().sdy_qk_rope_at(ctypes.byref(a), None))
+    for i, buf in enumerate(big):
+        for g in range(2):
+            got = np.empty((3, hd), np.float16)
+            capi.check(lib().sdy_d2h(got.ctypes.data, buf.ptr + 2 * (g * far + past * hd), got.nbytes, None))
+            capi.check(lib().sdy_sync(None))
+            assert np.array_equal(got[:2].view(np.uint16), t.draft[i][g, :2].view(np.uint16))
+            if i:
+                assert np.array_equal(got[2], x[0, (4 + g) * hd:(5 + g) * hd].astype(np.float16))
+            else:
+                want, tol = S.rope(x[:, (2 + g) * hd:(3 + g) * hd][:, None], np.array([past + 2]), freq, 1.0, hd, 0)
+                assert (np.abs(got[2] - want[0, 0]) <= tol[0, 0] + S.U16 * np.abs(want[0, 0]) * 1.01 + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("kv", [0, 1], ids=["f32", "f16"])
+def test_attn_tree_very_long_cache(kv):
+    """18 million positions: 2.3 or 4.6 GB of K. All K rows are 0 but the last one, whose weight is about that of all others."""
+    past, hd, elt = 18_000_001, 64, (np.float32, np.float16)[kv]
+    L = lib()
+    nbytes = past * hd * np.dtype(elt).itemsize
+    cache = [capi.DeviceBuffer(nbytes) for _ in range(2)]
+    for c in cache:
+        capi.check(L.sdy_memset(c.ptr, 0, nbytes, None))
+    q = np.zeros((1, 1, hd), np.float32)
+    q[0, 0, 0] = 8.0
+    last = np.zeros((2, hd), elt)
+    last[0, 0] = 16.75  # the score 8 * 16.75 / sqrt(64)
+    last[1] = 1 + np.arange(hd)
+    first = np.full(hd, 512, elt)
+    at = nbytes - hd * last.itemsize
+    for c, x in zip(cache, last):
+        capi.check(L.sdy_h2d(c.ptr + at, x.ctypes.data, x.nbytes, None))
+    capi.check(L.sdy_h2d(cache[1].ptr, first.ctypes.data, first.nbytes, None))
+    capi.check(L.sdy_sync(None))
+    b = [up(x) for x in (q, np.zeros((1, hd), elt), np.zeros((1, hd), elt), np.array([-1], np.int32), np.array([past], np.int32),
+                         np.zeros(hd, np.float32))]
+    part = capi.DeviceBuffer(4 * L.sdy_attn_tree_floats(1, 1, 1, hd, past))
+    a = capi.SdyAttnTreeArgs(q=b[0].ptr, q_stride=hd, k_cache=cache[0].ptr, v_cache=cache[1].ptr, head_stride=past * hd,
+                             k_draft=b[1].ptr, v_draft=b[2].ptr, draft_stride=hd, kv_type=kv, parent=b[3].ptr, n_past=b[4].ptr,
+                             max_past=past, n_tok=1, n_head=1, n_kv_head=1, hd=hd, out=b[5].ptr, out_stride=hd, part=part.ptr)
+    capi.check(L.sdy_attn_tree(ctypes.byref(a), None))
+    w = np.exp(16.75)
+    want = (w * last[1].astype(np.float64) + 512) / (past + w)  # (past - 1 zeros, the drafted row's and the last one)
+    # the exponent's argument (24.2 in base 2, rounded twice, times ln 2) and exponential, the sums' parts (at most 600 of
+    # them, a span's own sum of 16s is exact), the quotient
+    tol = (2 * 24.2 * 0.7 + 2 + 600 + 2) * S.U32 * want
+    assert (np.abs(b[5].to_array(np.float32, hd) - want) <= tol).all()
+
+
 def test_a_step_answers_as_one_token_at_a_time():
     """Two attention layers' worth of a toy model, greedy: drafted trees checked by the four operators on the device give
     the tokens that one token at a time gives, whatever is drafted."""
