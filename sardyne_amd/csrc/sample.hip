@@ -10,7 +10,7 @@
 // vocabulary, is never chosen.
 //
 // Every kept set is a prefix of the order, so what is looked for is where it ends, without sorting the row. Rows of up to
-// 4096 tokens are a workgroup's work in LDS (k_sample_small). A longer row is cut into pieces, a workgroup each, and read
+// 2560 tokens are a workgroup's work in LDS (k_sample_small). A longer row is cut into pieces, a workgroup each, and read
 // three times, the second and third from the caches:
 //   k_sample_max   each piece's greatest and lowest logit;
 //   k_sample_bins  each piece's tokens counted, and their w added, by distance from the greatest logit in 1024 bins;
@@ -28,9 +28,18 @@ constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int MAX_VOCAB = 1 << 22;  // a token's place in the order fits 32 + 22 bits
 constexpr int BINS = 1024;
 constexpr int LIST = 4096;          // tokens that one workgroup holds
-constexpr int SMALL_K = 1024;       // up to here the bins' sums are not made: the first top_k tokens are listed themselves
+// Rows that one workgroup does alone, in one launch (top-k 40 and top-p; alone against in pieces): 2048 tokens 20.7 against
+// 22.8 us, 64 such rows 21.6 against 26.1, 1000 rows 47 against 56; 3000 tokens 26.1 against 23.1, 27.1 against 26.5, 60
+// against 58.
+constexpr int SMALL = 2560;
+// Up to so large a top_k the bins' sums are not made: the first top_k tokens are listed themselves (without against with
+// sums, 61 rows of 151936: top-k 40 47 against 63 us, 1000 57 against 71).
+constexpr int SMALL_K = 1024;
+// Pieces of a row (4, 8, 16: one row of 151936 38.8, 33.3, 31.0 us, 61 rows 65, 51, 47, 250 rows 98, 103, 103).
 constexpr int MAX_PIECES = 16;
-constexpr int FEW_ROWS = 16;        // up to here 1024 threads to a piece
+// Up to so many rows 1024 threads to a piece instead of 256 (1 row 27.7 against 31.3 us, 16 32.2 against 35.8, 32 36.7
+// against 38.8; 40 43.0 against 41.0, 64 51.9 against 48.3).
+constexpr int FEW_ROWS = 32;
 
 // A logit's place in the order: 32 bits that grow with x (-0 as 0, NaN as -inf), then 22 that fall with the index.
 SDY_DEV float value_at(uint64_t place) {
@@ -55,6 +64,8 @@ struct Work {
     unsigned long long before;             // count or sum before them
     unsigned long long want;               // the sum that the prefix has to reach
     unsigned long long list[LIST];
+    unsigned long long sum_of[BINS];       // ROW_COUNT: the bins' sums and counts over the row
+    unsigned count_of[BINS];
 };
 // after them: per row and piece, BINS sums; then BINS counts
 
@@ -635,9 +646,9 @@ __global__ __launch_bounds__(BINS) void k_sample_cut(Args A) {
         for (int q = 0; q < tid; q++) o += listed_of[q];
         w.offset[tid] = o;
     }
-    if (mode == ROW_COUNT) {  // the pick looks at the row's bins again: in the first piece's place
-        A.count[(size_t)row * A.pieces * BINS + tid] = (unsigned)count;
-        A.sum[(size_t)row * A.pieces * BINS + tid] = sum;
+    if (mode == ROW_COUNT) {  // the pick looks at the bins again
+        w.count_of[tid] = (unsigned)count;
+        w.sum_of[tid] = sum;
     }
 }
 
@@ -690,6 +701,7 @@ __global__ __launch_bounds__(THREADS) void k_sample_pick(Args A) {
     };
     auto place = [&](int i) -> uint64_t { return k.list[i]; };
     auto w_of = [&](int i) -> uint64_t { return k.w[i]; };
+    bool summed = false;  // k.sums: the pieces' sums before the listed tokens, k.w: these tokens' w
     if (mode == ROW_SUM || mode == ROW_ALL) {
         if (tid < A.pieces) k.sums[tid] = w.sums[tid];
         if (mode == ROW_SUM) {
@@ -702,22 +714,13 @@ __global__ __launch_bounds__(THREADS) void k_sample_pick(Args A) {
             sum = block_sum(sum, k.parts);
             if (r.top_p < 1.0f && w.before + sum >= w.want) least = find(n, place, w_of, w.before, w.want, k).key;
             else if (n) least = ~block_max(~last, k.parts);
-            for (int i = tid; i < n; i += THREADS) {
-                const uint64_t v = k.list[i] < least ? 0 : r.min_p > 0.0f ? r.fixed_kept(k.list[i]) : k.w[i];
-                if (v) atomicAdd(&k.sums[index_at(k.list[i]) / A.len], (unsigned long long)v);
-            }
+        } else {
+            n = 0;
         }
         __syncthreads();
-        uint64_t whole = 0;
-        for (int p = 0; p < A.pieces; p++) whole += k.sums[p];
-        uint64_t left = share(u, whole);
-        int p = 0;
-        while (p < A.pieces - 1 && k.sums[p] <= left) left -= k.sums[p++];
-        const int lo = p * A.len, i = narrow(lo, lo + A.len < r.n ? lo + A.len : r.n, left, kept, k);
-        if (tid == 0) take(A, row, i, kept(i), whole);
-        return;
-    }
-    if (mode == ROW_COUNT) {  // many tokens by count: the end of the first top_k is known now, and with it their sum
+        summed = true;
+    } else if (mode == ROW_COUNT) {  // many tokens by count: the end of the first top_k is known now, and with it their sum
+        int end = w.b0;  // the bin that the prefix ends in, whose tokens are listed
         __syncthreads();
         for (int i = tid; i < n; i += THREADS) k.w[i] = r.fixed(value_at(k.list[i]));
         const uint64_t rest = (uint64_t)r.top_k - w.before;
@@ -728,27 +731,26 @@ __global__ __launch_bounds__(THREADS) void k_sample_pick(Args A) {
             least = ~block_max(~last, k.parts);
         }
         if (r.top_p < 1.0f) {
-            const size_t at = (size_t)row * A.pieces * BINS;
             uint64_t sum = 0, ahead = 0;
             __syncthreads();
             for (int i = tid; i < n; i += THREADS) sum += k.list[i] < least ? (k.w[i] = 0) : k.w[i];
             sum = block_sum(sum, k.parts);
-            for (int b = tid; b < w.b0; b += THREADS) ahead += A.sum[at + b];
+            for (int b = tid; b < w.b0; b += THREADS) ahead += w.sum_of[b];
             ahead = block_sum(ahead, k.parts);
             const uint64_t want = wanted(r.top_p, ahead + sum);
             if (ahead < want) {
                 least = find(n, place, w_of, ahead, want, k).key;
             } else {  // the sum ends in an earlier bin, whose tokens nobody has listed
-                const Found b = find(w.b0, [](int i) -> uint64_t { return (uint64_t)(BINS - i); }, [&](int i) -> uint64_t { return A.sum[at + i]; }, 0, want, k);
-                const int bin = BINS - (int)b.key;
-                n = (int)A.count[at + bin];
+                const Found b = find(w.b0, [](int i) -> uint64_t { return (uint64_t)(BINS - i); }, [&](int i) -> uint64_t { return w.sum_of[i]; }, 0, want, k);
+                end = BINS - (int)b.key;
+                n = (int)w.count_of[end];
                 if (n > LIST) {
                     mode = ROW_SLOW;
                 } else {
                     if (tid == 0) k.n = 0;
                     __syncthreads();
                     each(r.x, 0, r.n, [&](float x, int i) {
-                        if (x > -INFINITY && r.bin(x) == bin) {
+                        if (x > -INFINITY && r.bin(x) == end) {
                             const int to = atomicAdd(&k.n, 1);
                             k.list[to] = place_of(x, i);
                             k.w[to] = r.fixed(x);
@@ -759,6 +761,35 @@ __global__ __launch_bounds__(THREADS) void k_sample_pick(Args A) {
                 }
             }
         }
+        // (a min-p can end before the listed bin)
+        if (mode == ROW_COUNT && !(r.min_p > 0.0f)) {
+            __syncthreads();
+            for (int p = tid >> 6; p < A.pieces; p += WAVES) {
+                const unsigned long long *of = A.sum + ((size_t)row * A.pieces + p) * BINS;
+                uint64_t sum = 0;
+#pragma unroll 4
+                for (int b = tid & 63; b < end; b += 64) sum += of[b];
+                sum = wave_sum(sum);
+                if ((tid & 63) == 0) k.sums[p] = sum;
+            }
+            __syncthreads();
+            summed = true;
+        }
+    }
+    if (summed) {
+        for (int i = tid; i < n; i += THREADS) {
+            const uint64_t v = k.list[i] < least ? 0 : r.min_p > 0.0f ? r.fixed_kept(k.list[i]) : k.w[i];
+            if (v) atomicAdd(&k.sums[index_at(k.list[i]) / A.len], (unsigned long long)v);
+        }
+        __syncthreads();
+        uint64_t whole = 0;
+        for (int p = 0; p < A.pieces; p++) whole += k.sums[p];
+        uint64_t left = share(u, whole);
+        int p = 0;
+        while (p < A.pieces - 1 && k.sums[p] <= left) left -= k.sums[p++];
+        const int lo = p * A.len, i = narrow(lo, lo + A.len < r.n ? lo + A.len : r.n, left, kept, k);
+        if (tid == 0) take(A, row, i, kept(i), whole);
+        return;
     }
     if (mode == ROW_SLOW) {
         least = 0;
@@ -788,7 +819,7 @@ int pieces_of(int n_vocab) {
 
 extern "C" size_t sdy_sample_ws_bytes(int n_rows, int n_vocab) {
     if (n_rows < 1 || n_rows > 65535 || n_vocab < 1 || n_vocab > MAX_VOCAB) return 0;
-    if (n_vocab <= LIST) return 16;
+    if (n_vocab <= SMALL) return 16;
     return (size_t)n_rows * (sizeof(Work) + (size_t)pieces_of(n_vocab) * BINS * 12);
 }
 
@@ -812,7 +843,7 @@ extern "C" int sdy_sample(const sdy_sample_args *a, sdy_stream s) {
     A.sum = (unsigned long long *)(A.work + a->n_rows);
     A.count = (unsigned *)(A.sum + (size_t)a->n_rows * A.pieces * BINS);
     static size_t granted[2];
-    const bool small = a->n_vocab <= LIST;
+    const bool small = a->n_vocab <= SMALL;
     const int rc = sdy_lds_limit(small ? (const void *)k_sample_small : (const void *)k_sample_pick, sizeof(Lds), &granted[small]);
     if (rc) return rc;
     const dim3 rows(a->n_rows), grid(A.pieces, a->n_rows), block(THREADS);

@@ -230,7 +230,8 @@ class Tree:
     (1, 0, 1, 1, 64), (1, 1, 2, 1, 128), (1, 700, 16, 2, 128), (2, 31, 4, 4, 64), (3, 32, 8, 1, 128), (5, 33, 7, 1, 64),
     (4, 63, 8, 2, 128), (8, 64, 4, 1, 256), (9, 65, 16, 2, 128), (16, 127, 8, 1, 128), (17, 128, 32, 4, 64),
     (31, 0, 4, 2, 128), (33, 129, 14, 2, 64), (61, 500, 8, 1, 128), (64, 1023, 16, 2, 128), (65, 1024, 4, 1, 64),
-    (100, 40, 16, 1, 128), (128, 301, 4, 2, 256), (255, 77, 8, 2, 64), (256, 256, 4, 4, 128), (24, 5000, 8, 1, 128)])
+    (100, 40, 16, 1, 128), (128, 301, 4, 2, 256), (255, 77, 8, 2, 64), (256, 256, 4, 4, 128), (24, 5000, 8, 1, 128),
+    (2, 24700, 8, 8, 128), (3, 6000, 16, 16, 64), (50, 3000, 4, 1, 64)])
 @pytest.mark.parametrize("kv", [0, 1], ids=["f32", "f16"])
 def test_attn_tree(n, past, nh, nkv, hd, kv):
     Tree(n, past, nh, nkv, hd, kv, n + past, unused=3 if n > 8 else 0).run().check()
@@ -405,7 +406,7 @@ def check_sample(x, temp=None, top_k=None, top_p=None, min_p=None, u=None, **kw)
         assert abs(prob[r] - p) <= S.U32 * p * 1.01 + 1e-30 + 2.0 ** -39, (r, prob[r], p)
 
 
-@pytest.mark.parametrize("n,v", [(1, 1), (3, 2), (5, 17), (4, 63), (3, 64), (7, 257), (2, 1023), (3, 1025), (40, 4099),
+@pytest.mark.parametrize("n,v", [(1, 1), (3, 2), (5, 17), (4, 63), (3, 64), (7, 257), (2, 1023), (3, 1025), (4, 2560), (4, 2561), (40, 4099),
                                  (9, 32000), (300, 1500), (2, 151936), (70, 5003), (1, 262147)])
 @pytest.mark.parametrize("kind", ["float", "coarse", "masked", "flat", "steep"])
 def test_sample(n, v, kind):
@@ -476,7 +477,7 @@ def test_sample_special_logits(v):
         assert np.array_equal(run_sample(x, u=u)[0], run_sample(x, u=np.float32(1) - np.float32(2.0 ** -24))[0])
 
 
-@pytest.mark.parametrize("v", [4099, 40003])
+@pytest.mark.parametrize("v", [2561, 4099, 40003])
 def test_sample_special_long_rows(v):
     """As above in rows that are cut into pieces: what decides is where the bins of distance from the greatest logit end."""
     nan, inf, big = np.nan, np.inf, np.float32(3e38)
