@@ -185,8 +185,8 @@ struct Stage {
 };
 
 // Which nodes each node sees, as bits: mask[t] starts as t itself, then takes that of the farthest node known above it and
-// that one's farthest in turn, doubling the distance. The first 256 threads do (up to 64 nodes, in the first wave's registers:
-// 1.7 us -> 0.8 of the drafted rows' workgroup); p0 is the parent of node tid.
+// that one's farthest in turn, doubling the distance. The first 256 threads do (up to 64 nodes, in the first wave's registers: 5
+// nodes over 700 positions 13.7 -> 12.9 us, 24 16.6 -> 16.4, 61 20.8 -> 20.6); p0 is the parent of node tid.
 SDY_DEV void ancestor_masks(int p0, int n, uint32_t (*mask)[MAX_NODES / 32], int16_t *up) {
     constexpr int W = MAX_NODES / 32;
     const int tid = threadIdx.x, words = (n + 31) / 32;
@@ -717,10 +717,21 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs A) {
 struct Plan {
     int rw, kw, rows, n_block, n_draft, n_span;
 };
-Plan plan_of(int n_tok, int n_head, int n_kv_head, int hd, int max_past) {
+Plan plan_of(int n_tok, int n_head, int n_kv_head, int hd, int max_past, bool f16) {
     Plan p;
     p.rows = n_tok * (n_head / n_kv_head);
-    p.rw = hd < 256 && p.rows > 128 ? 8 : 4;
+    // Eight waves as one group of 256 rows or as two of 128 that take tiles in turn. The one group brings a tile in half the
+    // time, and needs no merge: it wins where a workgroup has few tiles, and with f32's longer products. The two have work
+    // for waves that would have no rows, and products of one group beside the other work of the other. `work`: tiles of a
+    // workgroup, in blocks of 128 rows. us, one group against two, 2 or 4 kv heads of 128 dims:
+    //   f16   40 rows over 700 11.6 : 12.9, over 33001 22.8 : 20.8; 128 rows over 700 15.2 : 17.1, over 4099 20.8 : 21.2, over
+    //         33001 38.3 : 35.9; 256 rows over 700 20.4 : 19.0, over 4099 29.7 : 24.7, over 33001 54.3 : 50.0
+    //   f32   40 rows over 700 13.9 : 16.0, over 33001 29.4 : 31.9; 128 rows over 4099 23.9 : 26.3; 512 rows over 4099 37.4 :
+    //         36.2, over 33001 116 : 128; 32 rows of 8 kv heads over 33001 62 : 57
+    //   64 dims  32 rows of 8 kv heads over 33001 f32 42 : 30, f16 34 : 23; 488 rows over 700 16.3 : 15.3, 14.7 : 13.7
+    const long work = ((long)max_past + KB - 1) / KB * n_kv_head * ((p.rows + 127) / 128) / 256;
+    const bool two = f16 || hd == 64 ? p.rows > 192 || work >= 2 : p.rows <= 64 && work >= 24;
+    p.rw = hd == 256 || two ? 4 : 8;
     p.kw = hd == 256 ? 1 : 8 / p.rw;
     const int block = 32 * p.rw;
     p.n_block = (p.rows + block - 1) / block;
@@ -774,8 +785,13 @@ extern "C" int sdy_attn_tree_ok(int n_tok, int n_head, int n_kv_head, int hd) {
 
 extern "C" size_t sdy_attn_tree_floats(int n_tok, int n_head, int n_kv_head, int hd, int max_past) {
     if (!sdy_attn_tree_ok(n_tok, n_head, n_kv_head, hd) || max_past < 0 || max_past > MAX_PAST) return 0;
-    const Plan p = plan_of(n_tok, n_head, n_kv_head, hd, max_past);
-    return (size_t)(p.n_draft + p.n_span) * n_kv_head * p.rows * (hd + 2);
+    size_t most = 0;  // of the two types
+    for (int f16 = 0; f16 < 2; f16++) {
+        const Plan p = plan_of(n_tok, n_head, n_kv_head, hd, max_past, f16);
+        const size_t n = (size_t)(p.n_draft + p.n_span) * n_kv_head * p.rows * (hd + 2);
+        most = n > most ? n : most;
+    }
+    return most;
 }
 
 extern "C" int sdy_attn_tree(const sdy_attn_tree_args *a, sdy_stream s) {
@@ -800,7 +816,7 @@ extern "C" int sdy_attn_tree(const sdy_attn_tree_args *a, sdy_stream s) {
     if (a->q_stride < (long)a->n_head * a->hd || a->out_stride < (long)a->n_head * a->hd)
         return sdy_fail(-1, "attn_tree: q and out rows of %d x %d floats (strides %ld, %ld)", a->n_head, a->hd, a->q_stride,
                         a->out_stride);
-    const Plan p = plan_of(a->n_tok, a->n_head, a->n_kv_head, a->hd, a->max_past);
+    const Plan p = plan_of(a->n_tok, a->n_head, a->n_kv_head, a->hd, a->max_past, elt == 2);
     TreeArgs A;
     A.a = *a;
     A.rows = p.rows;
