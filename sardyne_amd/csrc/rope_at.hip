@@ -53,7 +53,10 @@ SDY_DEV long slot_of(const sdy_rope_at_args &a, int t) {
 }
 
 // Heads of 32, 64, 128 or 256 dims in aligned rows: HD / 4 lanes to a row of q, k or v, four dims each. A workgroup takes
-// `rows` rows of one token, 256 / (HD / 4) at a time.
+// `rows` rows of one token, 256 / (HD / 4) at a time, the next ones' loads in flight. Bound by memory: 2048 tokens of 32 + 8
+// heads of 128 dims with f16 rows, 92 MB, 17.9 us, 5.2 TB/s (k_rope_any: 20.7; heads of 32 dims 17.8 against 42.9, of 64 18.0
+// against 25.7, of 256 18.1 against 20.1). One token takes 3.6 us (9.1), of which a launch is 1.5 and two dependent loads and
+// the sine most of the rest.
 template <int HD, class KT>
 __global__ __launch_bounds__(256) void k_rope_rows(sdy_rope_at_args a, int rows) {
     constexpr int L = HD / 4, RPP = 256 / L;
@@ -188,12 +191,14 @@ __global__ __launch_bounds__(256) void k_rope_any(sdy_rope_at_args a) {
     }
 }
 
-// Few tokens: a workgroup for every 256 lanes' rows; from 1024 of those on, one per token.
+// Few tokens: a workgroup for every 256 lanes' rows; where that would be more than 2048 of them, one per token, which makes
+// a token's sines once (against split, 32 + 8 heads of 128 dims: 1 token 6.0 against 3.6 us, 61 6.6 against 4.2, 200 7.0
+// against 5.3, 400 7.8 against 7.2, 2048 17.8 against 20.7).
 template <int HD, class KT>
 int launch_rows(const sdy_rope_at_args &a, hipStream_t st) {
     constexpr int RPP = 256 / (HD / 4);
     const int all = (a.q ? a.n_head : 0) + (a.k ? 2 * a.n_kv_head : 0), parts = (all + RPP - 1) / RPP;
-    const bool few = (long)a.n_tok * parts <= 1024 && parts <= 65535;
+    const bool few = (long)a.n_tok * parts <= 2048 && parts <= 65535;
     hipLaunchKernelGGL((k_rope_rows<HD, KT>), dim3(a.n_tok, few ? parts : 1), dim3(256), 0, st, a, few ? RPP : all);
     return sdy_check_launch("qk_rope_at");
 }
