@@ -406,14 +406,25 @@ SDY_DEV void pick_listed(const Args &A, int row, const Row &r, int n, Lds &k) {
     if (tid == 0) take(A, row, MAX_VOCAB - 1 - (int)f.key, f.val, sum);
 }
 
-// Of the tokens [lo, hi) the one at which the running sum of kept(i) passes `left`
+// Of the tokens [lo, hi) of x the one at which the running sum of kept(logit, index) passes `left` (lo a multiple of 4)
 template <class F>
-SDY_DEV int narrow(int lo, int hi, uint64_t left, const F &kept, Lds &k) {
+SDY_DEV int narrow(const float *x, int lo, int hi, uint64_t left, const F &kept, Lds &k) {
     while (hi - lo > 1) {
-        const int per = (hi - lo + THREADS - 1) / THREADS, b = lo + (int)threadIdx.x * per, e = b + per < hi ? b + per : hi;
+        int per = (hi - lo + THREADS - 1) / THREADS;
+        const bool wide = per >= 4 && ((uintptr_t)x & 15) == 0;
+        if (wide) per = (per + 3) & ~3;
+        const int b = lo + (int)threadIdx.x * per, e = b + per < hi ? b + per : hi;
         uint64_t sum = 0;
+        int i = b;
+        if (wide) {
 #pragma unroll 4
-        for (int i = b; i < e; i++) sum += kept(i);
+            for (; i + 4 <= e; i += 4) {
+                const float4 v = *reinterpret_cast<const float4 *>(x + i);
+                sum += kept(v.x, i) + kept(v.y, i + 1) + (kept(v.z, i + 2) + kept(v.w, i + 3));
+            }
+        }
+#pragma unroll 4
+        for (; i < e; i++) sum += kept(x[i], i);
         reach(sum, 0, left + 1, k.parts);
         lo = lo + (int)k.parts.key * per < hi ? lo + (int)k.parts.key * per : hi - 1;
         hi = lo + per < hi ? lo + per : hi;
@@ -555,14 +566,10 @@ __global__ __launch_bounds__(BINS) void k_sample_cut(Args A) {
     Work &w = A.work[row];
     Row r;
     r.params(A, row);
-    r.maxima(A, row);
-    if (r.alone || !r.cut()) {
-        if (tid == 0) w.mode = r.alone ? ROW_ALONE : ROW_ALL;
-        return;
-    }
     const bool sums = r.sums();
     count_of[tid] = 0;
     sum_of[tid] = 0;
+    // (on their way before the row's greatest logit is known; a row that needs no cut has left them as they were)
     unsigned n[EACH];
     unsigned long long s[EACH];
     const size_t at = ((size_t)row * A.pieces + p) * BINS + lane;
@@ -570,6 +577,11 @@ __global__ __launch_bounds__(BINS) void k_sample_cut(Args A) {
     for (int e = 0; e < EACH; e++) {
         n[e] = p < A.pieces ? A.count[at + 64 * e] : 0;
         s[e] = sums && p < A.pieces ? A.sum[at + 64 * e] : 0;
+    }
+    r.maxima(A, row);
+    if (r.alone || !r.cut()) {
+        if (tid == 0) w.mode = r.alone ? ROW_ALONE : ROW_ALL;
+        return;
     }
     __syncthreads();
 #pragma unroll
@@ -695,8 +707,8 @@ __global__ __launch_bounds__(THREADS) void k_sample_pick(Args A) {
     }
     const float u = A.a.u[row];
     uint64_t least = 0;  // the place that the prefix ends at
-    auto kept = [&](int i) -> uint64_t {
-        const uint64_t at = place_of(r.x[i], i);
+    auto kept = [&](float x, int i) -> uint64_t {
+        const uint64_t at = place_of(x, i);
         return at < least ? 0 : r.fixed_kept(at);
     };
     auto place = [&](int i) -> uint64_t { return k.list[i]; };
@@ -787,8 +799,8 @@ __global__ __launch_bounds__(THREADS) void k_sample_pick(Args A) {
         uint64_t left = share(u, whole);
         int p = 0;
         while (p < A.pieces - 1 && k.sums[p] <= left) left -= k.sums[p++];
-        const int lo = p * A.len, i = narrow(lo, lo + A.len < r.n ? lo + A.len : r.n, left, kept, k);
-        if (tid == 0) take(A, row, i, kept(i), whole);
+        const int lo = p * A.len, i = narrow(r.x, lo, lo + A.len < r.n ? lo + A.len : r.n, left, kept, k);
+        if (tid == 0) take(A, row, i, kept(r.x[i], i), whole);
         return;
     }
     if (mode == ROW_SLOW) {
@@ -804,10 +816,10 @@ __global__ __launch_bounds__(THREADS) void k_sample_pick(Args A) {
         }
     }
     uint64_t whole = 0;
-    for (int i = tid; i < r.n; i += THREADS) whole += kept(i);
+    each(r.x, 0, r.n, [&](float x, int i) { whole += kept(x, i); });
     whole = block_sum(whole, k.parts);
-    const int i = narrow(0, r.n, share(u, whole), kept, k);
-    if (tid == 0) take(A, row, i, kept(i), whole);
+    const int i = narrow(r.x, 0, r.n, share(u, whole), kept, k);
+    if (tid == 0) take(A, row, i, kept(r.x[i], i), whole);
 }
 
 int pieces_of(int n_vocab) {
