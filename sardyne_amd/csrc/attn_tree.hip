@@ -18,8 +18,18 @@
 // taken as they are; of the split products low x low, at most 2^-22 of the whole, is left out. A row of q goes by its own
 // greatest value. A span's K and V go by fixed powers, which suit a greatest value of 2^-5 to 2^10 (K) or 2^-9 to 2^6 (V): its
 // low part's least bit is then 2^-24 of it or less; a span outside of that is computed again with its own powers. Powers of
-// two go back exactly: K's and q's into the scores' factor, V's into O (ldexp). The running maximum m is kept as a whole number, so that its rescales are exact too, and grows
-// only when a score passes it by 2^LAG: P is 2^4 to 2^15 at the greatest weight, f16's least bit 2^-28 of it or less.
+// two go back exactly: K's and q's into the scores' factor, V's into O (ldexp). The running maximum m is kept as a whole
+// number, so that its rescales are exact too, and grows only when a score passes it by 2^LAG: P is 2^4 to 2^15 at the greatest
+// weight, f16's least bit 2^-28 of it or less.
+//
+// What bounds it. A full tree over a long cache: the matrix cores. 64 nodes of 32 heads (4 kv heads of 128 dims) over 40000
+// f32 positions are 126 GFLOP of f16 products and 164 MB of K and V: 131 us, k_tree_part 122 of them, 1.03 PFLOP/s (a large
+// f16 matrix product of the library reaches 1.28; matrix units busy 61% of the cycles, at about 2.0 GHz). Products and other
+// work are written side by side (fix() below) because a wave's own order decides what overlaps: in the
+// compiler's order, with four waves to a tile, the same case took 159 us. Few nodes over a short cache: latency. 5 nodes of 16 heads over 700 positions 13.9 us, k_tree_part
+// 10.3 (a launch, the chain past -> K -> scores -> O, and code that every launch fetches anew, about 40 ns per 64 bytes),
+// k_tree_merge 3.4. Between them both: 61 nodes of 32 heads over 4099 positions 33 us, 12.5 GFLOP and 28 MB of parts written and
+// read again. With f32 products on the f32 matrix cores (146 TFLOP/s at best) the first case would take 290 us.
 #include <type_traits>
 
 #include "sdy_attn_dev.h"
@@ -659,7 +669,8 @@ __global__ __launch_bounds__(64 * RW * KW, 1) void k_tree_part(TreeArgs A) {
     }
 }
 
-// The parts of one node and head in part order: 256 / (HD / 4) groups of lanes take parts in turn.
+// The parts of one node and head in part order: 256 / (HD / 4) groups of lanes take parts in turn. Bound by reading them: 64
+// nodes of 32 heads, 32 parts each, 34 MB (just written, so from the caches) 9.2 us, 3.7 TB/s; few nodes 3.4 us.
 template <int HD>
 __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs A) {
     constexpr int LN = HD / 4, NG = 256 / LN;

@@ -476,7 +476,14 @@ SDY_DEV uint64_t prefix_end(const Row &r, uint64_t least, bool by_sum, uint64_t 
 }
 
 // ---- the kernels
+//
+// Times of one row of 151936 logits with top-k and top-p, and of 61 rows of all kinds of parameters (37 MB): together 27 and
+// 63 us. One row is bound by its five launches and what each waits for before its work (the row's maximum, the listed bins);
+// 61 rows by reading 37 MB (max: 3.5 TB/s), by 64-bit exponentials of rows that need every token's w (bins), and by the
+// chains of searches of a workgroup per row (cut, pick). Sorting a row is never needed; a row in one workgroup's hands from
+// start to end took 800 us.
 
+// 1000 tokens 15.5 us, 1000 such rows 33: the searches' steps, each a few barriers.
 __global__ __launch_bounds__(THREADS) void k_sample_small(Args A) {
     extern __shared__ __align__(16) unsigned char lds_bytes[];
     Lds &k = *reinterpret_cast<Lds *>(lds_bytes);
@@ -497,6 +504,7 @@ __global__ __launch_bounds__(THREADS) void k_sample_small(Args A) {
     pick_listed(A, row, r, r.n, k);
 }
 
+// One row 4.1 us, 61 rows 10.6.
 template <int W>
 __global__ __launch_bounds__(64 * W) void k_sample_max(Args A) {
     __shared__ Parts<W> sh;
@@ -520,6 +528,7 @@ __global__ __launch_bounds__(64 * W) void k_sample_max(Args A) {
     }
 }
 
+// One row 3.9 us, 61 rows 13.
 template <int W>
 __global__ __launch_bounds__(64 * W) void k_sample_bins(Args A) {
     __shared__ Parts<W> sh;
@@ -555,7 +564,7 @@ __global__ __launch_bounds__(64 * W) void k_sample_bins(Args A) {
     }
 }
 
-// A wave per piece, 16 bins a lane; then a bin per thread.
+// A wave per piece, 16 bins a lane; then a bin per thread. One row 7.0 us, 61 rows 9.7.
 __global__ __launch_bounds__(BINS) void k_sample_cut(Args A) {
     constexpr int W = BINS / 64, EACH = BINS / 64;
     static_assert(W == MAX_PIECES, "a wave per piece");
@@ -664,6 +673,7 @@ __global__ __launch_bounds__(BINS) void k_sample_cut(Args A) {
     }
 }
 
+// One row 3.1 us, 61 rows 8.4.
 template <int W>
 __global__ __launch_bounds__(64 * W) void k_sample_list(Args A) {
     __shared__ unsigned next;
@@ -685,6 +695,7 @@ __global__ __launch_bounds__(64 * W) void k_sample_list(Args A) {
     });
 }
 
+// One row 5.6 us, 61 rows 16 to 19.
 __global__ __launch_bounds__(THREADS) void k_sample_pick(Args A) {
     extern __shared__ __align__(16) unsigned char lds_bytes[];
     Lds &k = *reinterpret_cast<Lds *>(lds_bytes);

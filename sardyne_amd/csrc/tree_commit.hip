@@ -11,7 +11,8 @@ namespace {
 
 constexpr int MAX_NODES = 256, THREADS = 256;
 
-// One workgroup per layer, K or V, and kv head. Each walks the tree itself (a node's next one by an LDS minimum over its
+// Bound by its launch: 8 nodes into 36 layers of 2 kv heads 2.9 us, 61 into 48 layers of 4 (f16 rows of 128) 3.0 us; what it
+// moves is under 1 MB. One workgroup per layer, K or V, and kv head. Each walks the tree itself (a node's next one by an LDS minimum over its
 // children, whose order does not matter), so one launch does it all. U: the unit that rows are copied in.
 template <class U>
 __global__ __launch_bounds__(THREADS) void k_tree_commit(sdy_tree_commit_args a, int row_units) {
