@@ -26,7 +26,7 @@
 // f32 positions are 126 GFLOP of f16 products and 164 MB of K and V: 131 us, k_tree_part 122 of them, 1.03 PFLOP/s (a large
 // f16 matrix product of the library reaches 1.28; matrix units busy 61% of the cycles, at about 2.0 GHz). Products and other
 // work are written side by side (fix() below) because a wave's own order decides what overlaps: in the
-// compiler's order, with four waves to a tile, the same case took 159 us. Few nodes over a short cache: latency. 5 nodes of 16 heads over 700 positions 13.9 us, k_tree_part
+// compiler's order, with four waves to a tile, the same case took 159 us. Few nodes over a short cache: latency. 5 nodes of 16 heads over 700 positions 13.4 us, k_tree_part
 // 10.3 (a launch, the chain past -> K -> scores -> O, and code that every launch fetches anew, about 40 ns per 64 bytes),
 // k_tree_merge 3.4. Between them both: 61 nodes of 32 heads over 4099 positions 33 us, 12.5 GFLOP and 28 MB of parts written and
 // read again. With f32 products on the f32 matrix cores (146 TFLOP/s at best) the first case would take 290 us.
@@ -63,16 +63,19 @@ struct TreeArgs {
     int n_block;    // row blocks
     int n_draft;    // spans of drafted rows
     int n_span;     // spans of cached positions (the grid's; those in use follow from n_past)
-    int least;      // turns of such a span, at least
+    int least;      // turns of such a span, at least, where there are many
     int granule;    // positions of one turn of a workgroup: 32 KW
     float log_scale;  // log2(e) / sqrt(head_dim)
     float *part;    // [n_draft + n_span][n_kv_head * rows][HD], then the (m, l) [n_draft + n_span][n_kv_head * rows][2]
 };
 
-// The rounds (granules) per span and the spans in use for so many positions.
+// The rounds (granules) per span and the spans in use for so many positions. One group of waves takes two tiles where there
+// are more than 128 of them over the kv heads, half the parts to merge (24 nodes of 16 heads over 2500: 19.7 against 22.8 us with
+// one, 32 of 32 heads over 1500 23.1 against 28.0; 5 of 16 heads over 700 13.9 against 13.2, 16 of them 16.3 against 15.9).
 SDY_DEV int span_rounds(const TreeArgs &A, int past) {
     const int n = (past + A.granule - 1) / A.granule, per = (n + A.n_span - 1) / A.n_span;
-    return per > A.least ? per : A.least;
+    const int least = (long)n * A.a.n_kv_head > 128 ? A.least : 1;
+    return per > least ? per : least;
 }
 SDY_DEV int spans_used(const TreeArgs &A, int past) {
     const int per = span_rounds(A, past), n = (past + A.granule - 1) / A.granule;
@@ -835,7 +838,6 @@ extern "C" int sdy_attn_tree(const sdy_attn_tree_args *a, sdy_stream s) {
     A.n_span = p.n_span;
     A.granule = KB * p.kw;
     A.n_draft = p.n_draft;
-    // two turns where they are of 32 positions: half the parts to merge (24 nodes of 16 heads over 2500: 22.2 -> 19.7 us)
     A.least = p.kw == 1 ? 2 : 1;
     A.log_scale = (float)(1.4426950408889634074 / sqrt((double)a->hd));
     A.part = a->part;
