@@ -323,7 +323,7 @@ struct Span {
         sk.load(rk, at_round(0), tg);
         sv.load(rv, at_round(0), tg);
 #pragma unroll 1
-        for (int it = 0; it < 2; it++) {
+        for (int it = 0; it < 2 && it < rounds; it++) {  // (the scores of a turn that is none are masked, whatever K is)
             drafted(sk, it);
 #pragma unroll
             for (int j = 0; j < PAIRS; j++) greatest_k = sk.most_of(j, greatest_k), sk.split(j, fk);
