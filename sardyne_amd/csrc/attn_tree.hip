@@ -23,13 +23,14 @@
 // weight, f16's least bit 2^-28 of it or less.
 //
 // What bounds it. A full tree over a long cache: the matrix cores. 64 nodes of 32 heads (4 kv heads of 128 dims) over 40000
-// f32 positions are 126 GFLOP of f16 products and 164 MB of K and V: 131 us, k_tree_part 122 of them, 1.03 PFLOP/s (a large
-// f16 matrix product of the library reaches 1.28; matrix units busy 61% of the cycles, at about 2.0 GHz). Products and other
-// work are written side by side (fix() below) because a wave's own order decides what overlaps: in the
-// compiler's order, with four waves to a tile, the same case took 159 us. Few nodes over a short cache: latency. 5 nodes of 16 heads over 700 positions 13.4 us, k_tree_part
-// 10.3 (a launch, the chain past -> K -> scores -> O, and code that every launch fetches anew, about 40 ns per 64 bytes),
-// k_tree_merge 3.4. Between them both: 61 nodes of 32 heads over 4099 positions 33 us, 12.5 GFLOP and 28 MB of parts written and
-// read again. With f32 products on the f32 matrix cores (146 TFLOP/s at best) the first case would take 290 us.
+// f32 positions are 126 GFLOP of f16 products and 164 MB of K and V: 130 to 133 us, k_tree_part 124 of them, 1.02 PFLOP/s (a
+// large f16 matrix product of the library reaches 1.28; matrix units busy 61% of the cycles, at about 2.0 GHz). Products and
+// other work are written side by side (fix() below) because a wave's own order decides what overlaps: in the compiler's order,
+// with four waves to a tile, the same case took 159 us. Few nodes over a short cache: latency. 5 nodes of 16 heads over 700
+// positions 13.1 us, k_tree_part 8.2 to 10 (a launch, the chain past -> K -> scores -> O, and code that every launch fetches
+// anew, about 40 ns per 64 bytes), k_tree_merge 3.8. Between them both: 61 nodes of 32 heads over 4099 positions 33 us, 12.5
+// GFLOP and 28 MB of parts written and read again. With f32 products on the f32 matrix cores (146 TFLOP/s at best) the first
+// case would take 290 us.
 #include <type_traits>
 
 #include "sdy_attn_dev.h"
