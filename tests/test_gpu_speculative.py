@@ -31,11 +31,11 @@ def as_kv(x, kv):
 # ----------------------------------------------------------------------------------- rotary
 
 def run_rope(x, n_head, n_kv_head, hd, pos, slot, freq, mscale, n_rot, interleaved, kv, n_slot, qn=None, kn=None, eps=1e-6,
-             in_place=False, pad=0, rows0=None):
+             in_place=False, pad=0, rows0=None, slot_at=0):
     """x [n][(n_head + 2 n_kv_head) hd + pad]: rows of stacked q|k|v -> q_out, k_rows, v_rows (as stored)."""
     n = x.shape[0]
     bx, bp, bf = up(x), up(pos.astype(np.int32)), up(freq)
-    bs = up(slot.astype(np.int32)) if slot is not None else None
+    bs = up(np.concatenate([np.zeros(slot_at), slot]).astype(np.int32)) if slot is not None else None
     elt = np.float16 if kv else np.float32
     rows0 = np.full((2, n_kv_head, n_slot, hd), 7, elt) if rows0 is None else rows0
     bk, bv, bq = up(rows0[0]), up(rows0[1]), up(np.full((n, n_head * hd), 9, np.float32))
@@ -44,7 +44,7 @@ def run_rope(x, n_head, n_kv_head, hd, pos, slot, freq, mscale, n_rot, interleav
     a = capi.SdyRopeAtArgs(q=bx.ptr, k=bx.ptr + 4 * q_dim, v=bx.ptr + 4 * (q_dim + kv_dim), q_stride=x.shape[1],
                            k_stride=x.shape[1], v_stride=x.shape[1], q_out=bx.ptr if in_place else bq.ptr,
                            q_out_stride=x.shape[1] if in_place else q_dim, k_rows=bk.ptr, v_rows=bv.ptr,
-                           head_stride=n_slot * hd, kv_type=kv, n_slot=n_slot, pos=bp.ptr, slot=bs.ptr if bs else None,
+                           head_stride=n_slot * hd, kv_type=kv, n_slot=n_slot, pos=bp.ptr, slot=bs.ptr + 4 * slot_at if bs else None,
                            freq=bf.ptr, mscale=mscale, n_rot=n_rot, interleaved=interleaved,
                            q_norm=norms[0].ptr if norms[0] else None, k_norm=norms[1].ptr if norms[1] else None, eps=eps,
                            n_tok=n, n_head=n_head, n_kv_head=n_kv_head, hd=hd)
@@ -123,14 +123,15 @@ def test_rope_at_is_the_consecutive_form(interleaved, kv):
         assert v.tobytes() == bv.to_array(elt, zero.shape[1:]).tobytes()
 
 
-def test_rope_at_one_slot_for_several_tokens():
-    """The last of them stays, wherever the others ran."""
-    n, nkv, hd = 600, 2, 64
+@pytest.mark.parametrize("n,at", [(600, 0), (601, 0), (603, 1), (5, 0), (2, 3), (2050, 2), (4103, 0)])
+def test_rope_at_one_slot_for_several_tokens(n, at):
+    """The last of them stays, wherever the others ran, and wherever the slots lie."""
+    nkv, hd = 2, 64
     rng = np.random.default_rng(8)
     x = rng.standard_normal((n, 3 * nkv * hd)).astype(np.float32)
     slot = rng.integers(0, 7, n)
     freq, mscale = rope_freq(hd)
-    _, _, v = run_rope(x, nkv, nkv, hd, np.arange(n), slot, freq, mscale, hd, 0, 0, 8)
+    _, _, v = run_rope(x, nkv, nkv, hd, np.arange(n), slot, freq, mscale, hd, 0, 0, 8, slot_at=at)
     want = np.full((nkv, 8, hd), 7, np.float32)
     for t in range(n):
         want[:, slot[t]] = x[t, 2 * nkv * hd:].reshape(nkv, hd)
