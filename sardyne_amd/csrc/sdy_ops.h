@@ -123,8 +123,8 @@ typedef struct {
     long head_stride;
     int kv_type, n_slot;
     const int32_t *pos, *slot;   /* [n_tok]; slot NULL: pos. A slot outside [0, n_slot): no row is written; of several
-                                    tokens with one slot the last one's row is (found by comparing all: tens of
-                                    thousands of tokens are better given in calls of some). Any int32 position */
+                                    tokens with one slot the last one's row is (found by comparing all: give
+                                    tens of thousands of tokens in several calls). Any int32 position */
     const double *freq;          /* [n_rot / 2] (sdy_rope_freqs): angle pos * freq[i] */
     float mscale;                /* the factor on cos and sin */
     int n_rot, interleaved;      /* dims of a head that turn, the first; pairs (2i, 2i+1) or (i, i + n_rot/2) */
